@@ -57,6 +57,8 @@ typedef enum {
 typedef struct mp_ctx mp_ctx;
 typedef struct mp_weight mp_weight;
 typedef struct mp_modset mp_modset;
+typedef struct mp_adapters mp_adapters;
+typedef struct mp_requests mp_requests;
 
 /* One projection weight, torch Linear layout [n out, k in]. */
 typedef struct {
@@ -94,7 +96,8 @@ const char* mp_last_error(const mp_ctx* ctx);
 /* Name of a status code. */
 const char* mp_status_string(int status);
 /* Synchronizes `stream` and reports device-side failures: MP_ETIMEOUT when
- * any kernel of this context gave up a bounded wait since the last check.
+ * any kernel of this context gave up a bounded wait since the last check,
+ * MP_EINVAL when a request plan met a length or an adapter out of range.
  * Replaces: the commit/wait of the forward (src/ming-dit.cc:2564-2571). */
 int mp_sync_check(mp_ctx* ctx, void* stream);
 /* Device-side wait limit in nanoseconds (default 2e9). */
@@ -345,6 +348,93 @@ int mp_pack_quantize(const char* src, const char* dst, int bits, int* n_quantize
 int mp_linear_lora_static(mp_ctx* ctx, const mp_weight* w, const void* x, int64_t ldx,
                           const uint16_t* a, const uint16_t* b, int rank, float strength,
                           void* y, int64_t ldy, int m, void* stream);
+
+/* ---- adapters by request -------------------------------------------------- */
+
+/* A batch whose rows belong to requests, each with a low-rank adapter of its
+ * own out of a bank of many, beside one shared projection; and the backward
+ * pass of that, for training the adapters. No counterpart in the reference,
+ * whose slots apply to every row.
+ *
+ * A bank holds `capacity` adapters (up to 4096) of rank <= max_rank (up to
+ * 128) for a projection of shape [n, k]; one that was never set adds nothing.
+ * With `training` the transposed factors are kept too, which the backward pass
+ * reads (twice the memory). */
+int mp_adapters_create(mp_ctx* ctx, int n, int k, int capacity, int max_rank, int training,
+                       mp_adapters** out);
+int mp_adapters_free(mp_ctx* ctx, mp_adapters* bank);
+/* Sets adapter `index`: a = bf16 [rank, k] with alpha / rank folded in, b =
+ * bf16 [n, rank], host or device, read in the order of `stream`. Where a
+ * factor holds a value that is not finite, every row of a request that uses
+ * the adapter comes out NaN, and no other row is touched by it. */
+int mp_adapters_set(mp_ctx* ctx, mp_adapters* bank, int index, const uint16_t* a,
+                    const uint16_t* b, int rank, void* stream);
+/* Columns of the bank's rank-space rows: max_rank rounded up to 16. */
+int mp_adapters_rank_pad(const mp_adapters* bank);
+
+/* The plan of a batch: which rows belong to which request and adapter. Made
+ * once per batch and shared by every projection and bank of it; its memory is
+ * allocated here, for up to max_requests (<= 4096) requests over up to
+ * max_rows (< 2^19) rows and adapters below `capacity`. */
+int mp_requests_create(mp_ctx* ctx, int max_requests, int max_rows, int capacity,
+                       mp_requests** out);
+int mp_requests_free(mp_ctx* ctx, mp_requests* req);
+/* Plans a batch of m rows on the GPU: request q has lengths[q] rows (0 is
+ * allowed), right after those of request q - 1, adapter adapters[q] (-1: none)
+ * and strength strengths[q] (NULL: all 1; exactly 0 drops the adapter); rows
+ * after the last request have no adapter. All three: device arrays. A negative
+ * length, lengths that pass m, and an adapter outside [-1, capacity) are cut
+ * to what is valid, and the next mp_sync_check reports MP_EINVAL. Calls that
+ * use the plan follow on the same stream, or are ordered after it. */
+int mp_requests_plan(mp_ctx* ctx, mp_requests* req, const int32_t* lengths,
+                     const int32_t* adapters, const float* strengths, int n_requests, int m,
+                     void* stream);
+
+/* y[t] = x[t] deq(W)^T + s_q (x[t] A_a^T) B_a^T for every row t of every
+ * request q, a its adapter; x, y as in mp_linear. Slots bound to `w` are not
+ * applied. A row without an adapter has the bits of the same call with an empty
+ * plan. `ranks` (nullable): f32 [m, >= mp_adapters_rank_pad], 16-byte aligned,
+ * ldr a multiple of 4: s_q x[t] A_a^T (0 without an adapter), which the
+ * backward pass takes as v. */
+int mp_linear_requests(mp_ctx* ctx, const mp_weight* w, const void* x, int64_t ldx,
+                       const mp_adapters* bank, const mp_requests* req, void* y, int64_t ldy,
+                       float* ranks, int64_t ldr, int m, void* stream);
+
+/* The dense bf16 transpose [k, n] of a projection weight [n, k]: the values
+ * the projections multiply with. Freed with mp_weight_free. */
+int mp_weight_transpose(mp_ctx* ctx, const mp_weight* w, void* stream, mp_weight** out);
+
+/* The backward pass of mp_linear_requests, W held fixed. With u[t] =
+ * s_q dy[t] B_a:
+ *   dx[t] = dy[t] W + u[t] A_a                     bf16 [m, k]
+ *   da[a] = sum over the rows t of a of u[t]^T x[t]   f32 [plan capacity, max_rank, k]
+ *   db[a] = sum over the rows t of a of dy[t]^T v[t]  f32 [plan capacity, n, max_rank]
+ * Each of dx, da, db may be NULL (not computed). wt: mp_weight_transpose of the
+ * weight; dy bf16 [m, n]; v f32 [m, >= max_rank] from the forward call's
+ * `ranks`. x is bf16 [m, k], or with xq != NULL the checkpoint (xq, xscale) of
+ * it. da and db are written whole, zero for adapters without rows. Sums are in
+ * f32, in an order that depends on the plan alone. */
+int mp_linear_requests_grad(mp_ctx* ctx, const mp_weight* wt, const void* dy, int64_t ldy,
+                            const void* x, int64_t ldx, const int8_t* xq, int64_t ldq,
+                            const float* xscale, const float* v, int64_t ldv,
+                            const mp_adapters* bank, const mp_requests* req, void* dx,
+                            int64_t lddx, float* da, float* db, int m, void* stream);
+
+/* ---- activation checkpoints in 8 bits --------------------------------------- */
+
+#define MP_CHECKPOINT_GROUP 128 /* features of a row that share a scale */
+
+/* Keeps bf16 rows x [m, k] as signed 8-bit codes q [m, ldq] (16-byte aligned,
+ * ldq >= k and a multiple of 16) and f32 scales scale[g * m + row] for the
+ * features [128 g, 128 g + 128):
+ *   scale = max|x| / 127,  q = rint(x * (127 * (1 / max|x|)))      (each op in f32)
+ * A group whose max|x| is below 2^-110 is kept as zeros; one that holds an
+ * infinity or a NaN comes back as NaN. */
+int mp_checkpoint(mp_ctx* ctx, const void* x, int64_t ldx, int m, int k, int8_t* q, int64_t ldq,
+                  float* scale, void* stream);
+/* x = bf16(q * scale). */
+int mp_restore(mp_ctx* ctx, const int8_t* q, int64_t ldq, const float* scale, int m, int k,
+               void* x, int64_t ldx, void* stream);
 
 /* ---- engagement -------------------------------------------------------- */
 

@@ -12,6 +12,7 @@
 #include <cstdlib>
 #include <cstring>
 #include <map>
+#include <new>
 #include <string>
 #include <vector>
 
@@ -28,6 +29,15 @@ cudaError_t launch_mod(const ModParams& p, cudaStream_t stream);
 int mod_tokens_per_launch(int n, int k, int n_blocks);
 cudaError_t launch_rms_residual(const RmsResidualParams& p, cudaStream_t stream);
 cudaError_t launch_attention(const AttnParams& p, cudaStream_t stream);
+cudaError_t launch_plan_requests(const PlanParams& p, cudaStream_t stream);
+cudaError_t launch_bank_set(const BankSetParams& p, cudaStream_t stream);
+cudaError_t launch_rank_rows(const RankParams& p, cudaStream_t stream);
+cudaError_t launch_adapter_grad(const GradParams& p, cudaStream_t stream);
+cudaError_t launch_checkpoint(const CheckpointParams& p, cudaStream_t stream);
+cudaError_t launch_restore(const CheckpointParams& p, cudaStream_t stream);
+cudaError_t launch_weight_transpose(const void* w, const uint32_t* sb, int sb_stride, int n, int k, int kp,
+                                    int bits, uint32_t code_xor, float code_offset, uint16_t* dst, int np,
+                                    cudaStream_t stream);
 }  // namespace mp
 
 using mp::ProjParams;
@@ -95,6 +105,28 @@ struct mp_modset {
   std::vector<void*> owned;  // bias / gain copies
 };
 
+// Factors of up to `cap` adapters for one projection shape, each padded to rp
+// ranks (zeros), and for training their transposed copies.
+struct mp_adapters {
+  int n = 0, k = 0, cap = 0, max_rank = 0;
+  int rp = 0;              // max_rank rounded up to 16
+  int kp = 0, np = 0;      // k, n rounded up to 8
+  uint16_t* a = nullptr;   // [cap][rp][kp]
+  uint16_t* b = nullptr;   // [cap][n][rp]
+  uint16_t* at = nullptr;  // [cap][k][rp] (training)
+  uint16_t* bt = nullptr;  // [cap][rp][np] (training)
+  int32_t* bad = nullptr;  // [cap]: a factor held a value that is not finite
+  CUtensorMap tm_b;        // [cap * n, rp], box {64, 128}, SW128
+  CUtensorMap tm_at;       // [cap * k, rp]
+};
+
+struct mp_requests {
+  int max_req = 0, max_rows = 0;
+  int32_t* buf = nullptr;
+  mp::RequestPlan plan{};
+  bool planned = false;
+};
+
 namespace {
 
 struct SharedStack {
@@ -134,6 +166,10 @@ struct mp_ctx {
   cudaStream_t side = nullptr;
   cudaEvent_t ev_fork = nullptr;
   cudaEvent_t ev_join = nullptr;
+  uint16_t* req_blk = nullptr;  // adapters by request: rank-space blocks (bf16) of a projection
+  size_t req_blk_cap = 0;
+  float* req_u = nullptr;       // their backward pass: u = s dy B (f32)
+  size_t req_u_cap = 0;
   uint32_t* flags = nullptr;    // fused-prologue ready flags (zeroed on allocation)
   size_t flags_cap = 0;         // entries
   uint32_t epoch = 0;           // value of a flag that is set, per fused launch
@@ -697,12 +733,28 @@ struct HeadsLaunch {
   const float* rope_sin = nullptr;
 };
 
+// With `ext` (count 1, no stack) every request of the plan adds its own
+// adapter: the rank-space rows are computed first, as blocks of the launch's
+// token tile, and appended as K tiles.
+struct RequestsLaunch {
+  const mp_requests* req = nullptr;
+  const mp_adapters* bank = nullptr;
+  const uint16_t* f = nullptr;  // rank-space factor [cap][rp][fp]
+  int fp = 0;
+  const CUtensorMap* tm_b = nullptr;
+  float* v32 = nullptr;         // also kept in f32 (nullable)
+  int64_t ld32 = 0;
+};
+
+int launch_request_ranks(mp_ctx* c, ProjParams* p, const RequestsLaunch& ext, const void* x, int64_t ldx,
+                         cudaStream_t stream);
+
 int launch_projections(mp_ctx* c, const mp_weight* const* ws, void* const* ys,
                        const int64_t* ldys, const Stack* const* sts, const int* t_cols, int t_ld,
                        int count, const void* x, int64_t ldx, int m, cudaStream_t stream,
                        const Prologue* pro = nullptr, const SwiGluLaunch* swi = nullptr,
                        const HeadsLaunch* hds = nullptr, bool may_alloc = true,
-                       const Prologue* sep = nullptr) {
+                       const Prologue* sep = nullptr, const RequestsLaunch* ext = nullptr) {
   ProjParams p;
   int ns[mp::kMaxMembers] = {0, 0, 0, 0};
   for (int i = 0; i < count; ++i) ns[i] = ws[i]->d.n;
@@ -845,6 +897,10 @@ int launch_projections(mp_ctx* c, const mp_weight* const* ws, void* const* ys,
         mb.rope_sin = hds->rope_sin;
       }
     }
+  }
+  if (ext != nullptr) {
+    rc = launch_request_ranks(c, &p, *ext, x, ldx, stream);
+    if (rc != MP_OK) return rc;
   }
   if (pro != nullptr) {
     p.pre_ttiles = (m + mp::kPreTok - 1) / mp::kPreTok;
@@ -1110,6 +1166,8 @@ int mp_destroy(mp_ctx* c) {
   cudaFree(c->part);
   cudaFree(c->part_side);
   cudaFree(c->flags);
+  cudaFree(c->req_blk);
+  cudaFree(c->req_u);
   if (c->side != nullptr) cudaStreamDestroy(c->side);
   if (c->ev_fork != nullptr) cudaEventDestroy(c->ev_fork);
   if (c->ev_join != nullptr) cudaEventDestroy(c->ev_join);
@@ -1139,6 +1197,10 @@ int mp_sync_check(mp_ctx* c, void* stream) {
   MP_CUDA(c, cudaMemcpy(&word, c->err_word, sizeof(word), cudaMemcpyDeviceToHost));
   if (word != 0) {
     MP_CUDA(c, cudaMemset(c->err_word, 0, sizeof(uint32_t)));
+    if ((word & mp::kErrTimeout) == 0)
+      return fail(c, MP_EINVAL,
+                  "a request plan met a length or an adapter index out of range (the rows concerned "
+                  "ran without an adapter)");
     return fail(c, MP_ETIMEOUT, "a kernel gave up a bounded device-side wait (word 0x%x)", word);
   }
   return MP_OK;
@@ -1943,3 +2005,458 @@ extern "C" int mp_linear_lora_static(mp_ctx* c, const mp_weight* w, const void* 
   count_projection(c, w, m, ranks);
   return MP_OK;
 }
+
+// ---- adapters by request -------------------------------------------------------
+
+namespace {
+
+// The rank-space rows of a batch of requests: v = s_q (x F_q^T), into `p`'s
+// outputs.
+int launch_ranks(mp_ctx* c, const mp::RankParams& p, cudaStream_t stream) {
+  cudaError_t e = mp::launch_rank_rows(p, stream);
+  if (e != cudaSuccess) return cuda_fail(c, e, "rank_rows_kernel");
+  c->eng.kernels += 1;
+  c->eng.lora_down += 1;
+  return MP_OK;
+}
+
+mp::RankParams rank_params(const mp_ctx* c, const RequestsLaunch& ext, const void* x, int64_t ldx, int k) {
+  mp::RankParams r;
+  std::memset(&r, 0, sizeof(r));
+  r.x = static_cast<const uint16_t*>(x);
+  r.ldx = ldx;
+  r.f = ext.f;
+  r.fp = ext.fp;
+  r.k = k;
+  r.rp = ext.bank->rp;
+  r.bad = ext.bank->bad;
+  r.plan = ext.req->plan;
+  r.v32 = ext.v32;
+  r.ld32 = ext.ld32;
+  r.wait_limit_ns = c->wait_limit_ns;
+  r.err = c->err_word;
+  return r;
+}
+
+// Member 0 of the launch `p` takes its appended K tiles from the plan's lists:
+// computes the rank-space rows as blocks of the launch's token tile.
+int launch_request_ranks(mp_ctx* c, ProjParams* p, const RequestsLaunch& ext, const void* x, int64_t ldx,
+                         cudaStream_t stream) {
+  const mp::RequestPlan& pl = ext.req->plan;
+  int level = 0;
+  while ((64 << level) < p->n_tok) ++level;
+  const int chunks = (ext.bank->rp + mp::kBlockK - 1) / mp::kBlockK;
+  const int ldb = chunks * mp::kBlockK;
+  const size_t rows = static_cast<size_t>(mp::plan_blocks(pl.m, pl.n_req, level)) << (6 + level);
+  int rc = ensure_buf(c, &c->req_blk, &c->req_blk_cap, rows * ldb, stream);
+  if (rc != MP_OK) return rc;
+  mp::RankParams r = rank_params(c, ext, x, ldx, p->K);
+  r.vblk = c->req_blk;
+  r.lvl = level;
+  r.ldb = ldb;
+  MP_CUDA(c, cudaMemsetAsync(c->req_blk, 0, rows * ldb * sizeof(uint16_t), stream));
+  rc = launch_ranks(c, r, stream);
+  if (rc != MP_OK) return rc;
+  mp::ProjMember& mb = p->mem[0];
+  if (!encode_2d(&mb.tm_t, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, c->req_blk, ldb, rows,
+                 static_cast<uint64_t>(ldb) * 2, 64, static_cast<uint32_t>(sub_tok(p->n_tok) / 2),
+                 CU_TENSOR_MAP_SWIZZLE_128B))
+    return fail(c, MP_ECUDA, "tensor map encode failed (rank-space blocks)");
+  mb.tm_b = *ext.tm_b;
+  p->ext_first = pl.first[level];
+  p->ext_live = pl.live[level];
+  p->ext_list = pl.list[level];
+  p->ext_chunks = chunks;
+  return MP_OK;
+}
+
+int check_requests(mp_ctx* c, const mp_adapters* bank, const mp_requests* req, int n, int k, int m) {
+  if (bank->n != n || bank->k != k)
+    return fail(c, MP_EINVAL, "the adapters are for [%d, %d], the weight is [%d, %d]", bank->n, bank->k, n, k);
+  if (!req->planned) return fail(c, MP_EINVAL, "the requests have not been planned");
+  if (req->plan.m != m)
+    return fail(c, MP_EINVAL, "m = %d, but %d rows were planned", m, req->plan.m);
+  if (req->plan.cap > bank->cap)
+    return fail(c, MP_EINVAL, "the plan allows adapters below %d, there are %d", req->plan.cap, bank->cap);
+  return MP_OK;
+}
+
+int check_rank_rows(mp_ctx* c, const void* v, int64_t ld, int cols) {
+  if (reinterpret_cast<uintptr_t>(v) % 16 != 0 || ld % 4 != 0 || ld < cols)
+    return fail(c, MP_EINVAL, "rank-space rows: 16-byte aligned, pitch >= %d and a multiple of 4 (got %lld)",
+                cols, static_cast<long long>(ld));
+  return MP_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int mp_adapters_create(mp_ctx* c, int n, int k, int capacity, int max_rank, int training, mp_adapters** out) {
+  if (c == nullptr || out == nullptr) return MP_EINVAL;
+  *out = nullptr;
+  if (n <= 0 || k <= 0) return fail(c, MP_EINVAL, "adapter shape [%d, %d]: n > 0 and k > 0 required", n, k);
+  if (capacity <= 0 || capacity > mp::kMaxAdapters)
+    return fail(c, MP_EINVAL, "capacity %d outside [1, %d]", capacity, mp::kMaxAdapters);
+  if (max_rank <= 0 || max_rank > mp::kMaxAdapterRank)
+    return fail(c, MP_EINVAL, "max_rank %d outside [1, %d]", max_rank, mp::kMaxAdapterRank);
+  if (static_cast<int64_t>(capacity) * std::max(n, k) > INT_MAX)
+    return fail(c, MP_EINVAL, "capacity * max(n, k) exceeds 2^31 rows");
+  int rc = use_device(c);
+  if (rc != MP_OK) return rc;
+  mp_adapters* b = new (std::nothrow) mp_adapters();
+  if (b == nullptr) return fail(c, MP_ENOMEM, "out of host memory");
+  b->n = n;
+  b->k = k;
+  b->cap = capacity;
+  b->max_rank = max_rank;
+  b->rp = (max_rank + 15) / 16 * 16;
+  b->kp = (k + 7) / 8 * 8;
+  b->np = (n + 7) / 8 * 8;
+  auto cleanup = [&](int code) {
+    cudaFree(b->a);
+    cudaFree(b->b);
+    cudaFree(b->at);
+    cudaFree(b->bt);
+    cudaFree(b->bad);
+    delete b;
+    return code;
+  };
+  // zeroed: an adapter that was never set adds nothing
+  auto zeros = [&](auto** p, size_t elems) {
+    cudaError_t e = cudaMalloc(p, elems * sizeof(**p));
+    return e == cudaSuccess ? cudaMemset(*p, 0, elems * sizeof(**p)) : e;
+  };
+  const size_t cr = static_cast<size_t>(capacity) * b->rp;
+  cudaError_t e = zeros(&b->a, cr * b->kp);
+  if (e == cudaSuccess) e = zeros(&b->b, cr * n);
+  if (e == cudaSuccess && training) e = zeros(&b->at, cr * k);
+  if (e == cudaSuccess && training) e = zeros(&b->bt, cr * b->np);
+  if (e == cudaSuccess) e = zeros(&b->bad, capacity);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(nullptr);  // set on any stream may follow
+  if (e != cudaSuccess) return cleanup(cuda_fail(c, e, "cudaMalloc(adapters)"));
+  const uint64_t pitch = static_cast<uint64_t>(b->rp) * 2, cap = static_cast<uint64_t>(capacity);
+  if (!encode_2d(&b->tm_b, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, b->b, b->rp, cap * n, pitch, 64, 128,
+                 CU_TENSOR_MAP_SWIZZLE_128B) ||
+      (training && !encode_2d(&b->tm_at, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, b->at, b->rp, cap * k, pitch, 64, 128,
+                              CU_TENSOR_MAP_SWIZZLE_128B)))
+    return cleanup(fail(c, MP_ECUDA, "tensor map encode failed (adapters)"));
+  *out = b;
+  return MP_OK;
+}
+
+int mp_adapters_free(mp_ctx* c, mp_adapters* b) {
+  if (c == nullptr || b == nullptr) return MP_EINVAL;
+  cudaSetDevice(c->device);
+  cudaDeviceSynchronize();
+  cudaFree(b->a);
+  cudaFree(b->b);
+  cudaFree(b->at);
+  cudaFree(b->bt);
+  cudaFree(b->bad);
+  delete b;
+  return MP_OK;
+}
+
+int mp_adapters_set(mp_ctx* c, mp_adapters* b, int index, const uint16_t* fa, const uint16_t* fb, int rank,
+                    void* stream) {
+  if (c == nullptr || b == nullptr) return MP_EINVAL;
+  if (index < 0 || index >= b->cap) return fail(c, MP_EINVAL, "adapter %d outside [0, %d)", index, b->cap);
+  if (fa == nullptr || fb == nullptr) return fail(c, MP_EINVAL, "adapter factor is NULL");
+  if (rank <= 0 || rank > b->max_rank)
+    return fail(c, MP_EINVAL, "rank %d outside [1, %d]", rank, b->max_rank);
+  int rc = use_device(c);
+  if (rc != MP_OK) return rc;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  mp::BankSetParams p;
+  const size_t i = static_cast<size_t>(index) * b->rp;
+  p.a = b->a + i * b->kp;
+  p.b = b->b + i * b->n;
+  p.at = b->at != nullptr ? b->at + i * b->k : nullptr;
+  p.bt = b->bt != nullptr ? b->bt + i * b->np : nullptr;
+  p.bad = b->bad + index;
+  p.n = b->n;
+  p.k = b->k;
+  p.rank = rank;
+  p.rp = b->rp;
+  p.kp = b->kp;
+  p.np = b->np;
+  const size_t ka = static_cast<size_t>(b->k) * 2, rb = static_cast<size_t>(rank) * 2;
+  MP_CUDA(c, cudaMemcpy2DAsync(p.a, static_cast<size_t>(b->kp) * 2, fa, ka, ka, rank, cudaMemcpyDefault, s));
+  MP_CUDA(c, cudaMemcpy2DAsync(p.b, static_cast<size_t>(b->rp) * 2, fb, rb, rb, b->n, cudaMemcpyDefault, s));
+  MP_CUDA(c, cudaMemsetAsync(p.bad, 0, sizeof(int32_t), s));
+  MP_CUDA(c, mp::launch_bank_set(p, s));
+  c->eng.kernels += 1;
+  return MP_OK;
+}
+
+int mp_adapters_rank_pad(const mp_adapters* b) { return b == nullptr ? 0 : b->rp; }
+
+int mp_requests_create(mp_ctx* c, int max_requests, int max_rows, int capacity, mp_requests** out) {
+  if (c == nullptr || out == nullptr) return MP_EINVAL;
+  *out = nullptr;
+  if (max_requests <= 0 || max_requests > mp::kMaxRequests)
+    return fail(c, MP_EINVAL, "max_requests %d outside [1, %d]", max_requests, mp::kMaxRequests);
+  if (max_rows <= 0 || max_rows >= INT_MAX / mp::kMaxRequests)
+    return fail(c, MP_EINVAL, "max_rows %d outside [1, %d)", max_rows, INT_MAX / mp::kMaxRequests);
+  if (capacity <= 0 || capacity > mp::kMaxAdapters)
+    return fail(c, MP_EINVAL, "capacity %d outside [1, %d]", capacity, mp::kMaxAdapters);
+  int rc = use_device(c);
+  if (rc != MP_OK) return rc;
+  mp_requests* r = new (std::nothrow) mp_requests();
+  if (r == nullptr) return fail(c, MP_ENOMEM, "out of host memory");
+  r->max_req = max_requests;
+  r->max_rows = max_rows;
+  r->plan.cap = capacity;
+  // one allocation; the parts in 16-byte units, the 16-byte entries first
+  const size_t q = max_requests;
+  size_t words = 0;
+  size_t at_block[mp::kPlanLevels], at_s[mp::kPlanLevels], at_list[mp::kPlanLevels], at_first[mp::kPlanLevels],
+      at_live[mp::kPlanLevels];
+  auto take = [&](size_t n) {
+    const size_t at = words;
+    words += (n + 3) / 4 * 4;
+    return at;
+  };
+  for (int l = 0; l < mp::kPlanLevels; ++l) {
+    const size_t tiles = mp::plan_tiles(max_rows, l), blocks = tiles + q;
+    at_block[l] = take(4 * blocks);
+    at_s[l] = take(blocks);
+    at_list[l] = take(2 * blocks);
+    at_first[l] = take(tiles);
+    at_live[l] = take(tiles);
+  }
+  const size_t at_chunk = take(4 * static_cast<size_t>(mp::plan_chunks(max_rows, max_requests)));
+  const size_t at_seg = take(2 * q), at_begin = take(capacity + 1), at_row = take(max_rows);
+  cudaError_t e = cudaMalloc(&r->buf, words * sizeof(int32_t));
+  if (e != cudaSuccess) {
+    delete r;
+    return cuda_fail(c, e, "cudaMalloc(requests)");
+  }
+  for (int l = 0; l < mp::kPlanLevels; ++l) {
+    r->plan.block[l] = reinterpret_cast<int4*>(r->buf + at_block[l]);
+    r->plan.block_s[l] = reinterpret_cast<float*>(r->buf + at_s[l]);
+    r->plan.list[l] = reinterpret_cast<int2*>(r->buf + at_list[l]);
+    r->plan.first[l] = r->buf + at_first[l];
+    r->plan.live[l] = r->buf + at_live[l];
+  }
+  r->plan.chunk = reinterpret_cast<int4*>(r->buf + at_chunk);
+  r->plan.seg = reinterpret_cast<int2*>(r->buf + at_seg);
+  r->plan.begin = r->buf + at_begin;
+  r->plan.row_adapter = r->buf + at_row;
+  *out = r;
+  return MP_OK;
+}
+
+int mp_requests_free(mp_ctx* c, mp_requests* r) {
+  if (c == nullptr || r == nullptr) return MP_EINVAL;
+  cudaSetDevice(c->device);
+  cudaDeviceSynchronize();
+  cudaFree(r->buf);
+  delete r;
+  return MP_OK;
+}
+
+int mp_requests_plan(mp_ctx* c, mp_requests* r, const int32_t* lengths, const int32_t* adapters,
+                     const float* strengths, int n_requests, int m, void* stream) {
+  if (c == nullptr || r == nullptr) return MP_EINVAL;
+  if (n_requests < 0 || n_requests > r->max_req)
+    return fail(c, MP_EINVAL, "%d requests outside [0, %d]", n_requests, r->max_req);
+  if (n_requests > 0 && (lengths == nullptr || adapters == nullptr))
+    return fail(c, MP_EINVAL, "lengths and adapters are required");
+  if (m <= 0 || m > r->max_rows) return fail(c, MP_EINVAL, "m = %d outside [1, %d]", m, r->max_rows);
+  int rc = use_device(c);
+  if (rc != MP_OK) return rc;
+  r->plan.n_req = n_requests;
+  r->plan.m = m;
+  mp::PlanParams p;
+  p.plan = r->plan;
+  p.lengths = lengths;
+  p.adapters = adapters;
+  p.strengths = strengths;
+  p.err = c->err_word;
+  MP_CUDA(c, mp::launch_plan_requests(p, static_cast<cudaStream_t>(stream)));
+  c->eng.kernels += 1;
+  r->planned = true;
+  return MP_OK;
+}
+
+int mp_linear_requests(mp_ctx* c, const mp_weight* w, const void* x, int64_t ldx, const mp_adapters* b,
+                       const mp_requests* r, void* y, int64_t ldy, float* ranks, int64_t ldr, int m,
+                       void* stream) {
+  if (c == nullptr || w == nullptr || b == nullptr || r == nullptr) return MP_EINVAL;
+  int rc = check_x(c, x, ldx, w->d.k, m);
+  if (rc == MP_OK) rc = check_y(c, y, ldy, w->d.n);
+  if (rc == MP_OK) rc = check_requests(c, b, r, w->d.n, w->d.k, m);
+  if (rc == MP_OK && ranks != nullptr) rc = check_rank_rows(c, ranks, ldr, b->rp);
+  if (rc == MP_OK) rc = use_device(c);
+  if (rc != MP_OK) return rc;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  RequestsLaunch ext;
+  ext.req = r;
+  ext.bank = b;
+  ext.f = b->a;
+  ext.fp = b->kp;
+  ext.tm_b = &b->tm_b;
+  ext.v32 = ranks;
+  ext.ld32 = ldr;
+  if (ranks != nullptr)  // rows without an adapter
+    MP_CUDA(c, cudaMemset2DAsync(ranks, static_cast<size_t>(ldr) * 4, 0, static_cast<size_t>(b->rp) * 4, m, s));
+  const mp_weight* wl[1] = {w};
+  void* yl[1] = {y};
+  const int64_t ll[1] = {ldy};
+  const Stack* sl[1] = {nullptr};
+  const int cl[1] = {0};
+  rc = launch_projections(c, wl, yl, ll, sl, cl, 0, 1, x, ldx, m, s, nullptr, nullptr, nullptr, true, nullptr, &ext);
+  if (rc == MP_OK) c->eng.lora_proj += 1;
+  return rc;
+}
+
+int mp_weight_transpose(mp_ctx* c, const mp_weight* w, void* stream, mp_weight** out) {
+  if (c == nullptr || w == nullptr || out == nullptr) return MP_EINVAL;
+  *out = nullptr;
+  int rc = use_device(c);
+  if (rc != MP_OK) return rc;
+  mp_weight* t = new (std::nothrow) mp_weight();
+  if (t == nullptr) return fail(c, MP_ENOMEM, "out of host memory");
+  const int n = w->d.n, k = w->d.k;
+  t->d = mp_weight_desc{k, n, 0, 0, MP_QUANT_AFFINE};
+  t->w_bytes = static_cast<size_t>(n) * k * 2;
+  t->kp = (n + 7) / 8 * 8;
+  cudaError_t e = cudaMalloc(&t->w, static_cast<size_t>(k) * t->kp * 2);
+  if (e == cudaSuccess) {
+    const bool sym = w->d.bits == 8 && w->d.mode == MP_QUANT_SYMMETRIC;
+    e = mp::launch_weight_transpose(w->w, w->sb, w->sb_stride, n, k, w->kp, w->d.bits, sym ? 0x80u : 0u,
+                                    sym ? 32896.0f : 32768.0f, static_cast<uint16_t*>(t->w), t->kp,
+                                    static_cast<cudaStream_t>(stream));
+  }
+  const bool ok = e == cudaSuccess &&
+                  encode_2d(&t->tm_w, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, t->w, n, k,
+                            static_cast<uint64_t>(t->kp) * 2, 64, 128, CU_TENSOR_MAP_SWIZZLE_128B);
+  if (!ok) {
+    cudaFree(t->w);
+    delete t;
+    return e != cudaSuccess ? cuda_fail(c, e, "weight_transpose_kernel")
+                            : fail(c, MP_ECUDA, "tensor map encode failed (transposed weight)");
+  }
+  c->eng.kernels += 1;
+  *out = t;
+  return MP_OK;
+}
+
+int mp_linear_requests_grad(mp_ctx* c, const mp_weight* wt, const void* dy, int64_t ldy, const void* x, int64_t ldx,
+                            const int8_t* xq, int64_t ldq, const float* xscale, const float* v, int64_t ldv,
+                            const mp_adapters* b, const mp_requests* r, void* dx, int64_t lddx, float* da,
+                            float* db, int m, void* stream) {
+  if (c == nullptr || wt == nullptr || b == nullptr || r == nullptr) return MP_EINVAL;
+  const int n = wt->d.k, k = wt->d.n;
+  if (b->at == nullptr) return fail(c, MP_EINVAL, "the adapters were not created for training");
+  if (wt->d.bits != 0) return fail(c, MP_EINVAL, "the transposed weight must be dense");
+  int rc = check_x(c, dy, ldy, n, m);
+  if (rc == MP_OK && dx != nullptr) rc = check_y(c, dx, lddx, k);
+  if (rc == MP_OK) rc = check_requests(c, b, r, n, k, m);
+  if (rc == MP_OK && da != nullptr) {
+    if (xq != nullptr) {
+      if (xscale == nullptr || reinterpret_cast<uintptr_t>(xq) % 16 != 0 || ldq < k || ldq % 16 != 0)
+        rc = fail(c, MP_EINVAL, "checkpoint: codes 16-byte aligned, pitch >= k and a multiple of 16, and scales");
+    } else {
+      rc = check_x(c, x, ldx, k, m);
+    }
+  }
+  if (rc == MP_OK && db != nullptr && (v == nullptr || ldv < b->max_rank))
+    rc = fail(c, MP_EINVAL, "v: f32 rows of at least %d ranks are required", b->max_rank);
+  if (rc == MP_OK) rc = use_device(c);
+  if (rc != MP_OK) return rc;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  RequestsLaunch ext;
+  ext.req = r;
+  ext.bank = b;
+  ext.f = b->bt;
+  ext.fp = b->np;
+  ext.tm_b = &b->tm_at;
+  if (da != nullptr) {
+    rc = ensure_buf(c, &c->req_u, &c->req_u_cap, static_cast<size_t>(m) * b->rp, s);
+    if (rc != MP_OK) return rc;
+    ext.v32 = c->req_u;
+    ext.ld32 = b->rp;
+  }
+  if (dx != nullptr) {
+    const mp_weight* wl[1] = {wt};
+    void* yl[1] = {dx};
+    const int64_t ll[1] = {lddx};
+    const Stack* sl[1] = {nullptr};
+    const int cl[1] = {0};
+    rc = launch_projections(c, wl, yl, ll, sl, cl, 0, 1, dy, ldy, m, s, nullptr, nullptr, nullptr, true, nullptr,
+                            &ext);
+    if (rc == MP_OK) c->eng.lora_proj += 1;
+  } else if (da != nullptr) {
+    rc = launch_ranks(c, rank_params(c, ext, dy, ldy, n), s);
+  }
+  if (rc != MP_OK) return rc;
+  mp::GradParams g;
+  std::memset(&g, 0, sizeof(g));
+  g.r = b->max_rank;
+  g.plan = r->plan;
+  if (da != nullptr) {
+    mp::GradMember& mb = g.mem[g.n_mem++];
+    mb.x = xq != nullptr ? nullptr : static_cast<const uint16_t*>(x);
+    mb.ldx = ldx;
+    mb.q = xq;
+    mb.ldq = ldq;
+    mb.scale = xscale;
+    mb.u = c->req_u;
+    mb.ldu = b->rp;
+    mb.out = da;
+    mb.width = k;
+    mb.rank_major = 1;
+  }
+  if (db != nullptr) {
+    mp::GradMember& mb = g.mem[g.n_mem++];
+    mb.x = static_cast<const uint16_t*>(dy);
+    mb.ldx = ldy;
+    mb.u = v;
+    mb.ldu = ldv;
+    mb.out = db;
+    mb.width = n;
+  }
+  if (g.n_mem > 0) {
+    MP_CUDA(c, mp::launch_adapter_grad(g, s));
+    c->eng.kernels += 1;
+  }
+  return MP_OK;
+}
+
+int mp_checkpoint(mp_ctx* c, const void* x, int64_t ldx, int m, int k, int8_t* q, int64_t ldq, float* scale,
+                  void* stream) {
+  if (c == nullptr) return MP_EINVAL;
+  if (k <= 0) return fail(c, MP_EINVAL, "k must be positive (got %d)", k);
+  int rc = check_x(c, x, ldx, k, m);
+  if (rc != MP_OK) return rc;
+  if (q == nullptr || scale == nullptr || reinterpret_cast<uintptr_t>(q) % 16 != 0 || ldq < k || ldq % 16 != 0)
+    return fail(c, MP_EINVAL, "checkpoint: codes 16-byte aligned, pitch >= k and a multiple of 16, and scales");
+  rc = use_device(c);
+  if (rc != MP_OK) return rc;
+  const mp::CheckpointParams p{static_cast<const uint16_t*>(x), nullptr, ldx, q, ldq, scale, m, k};
+  MP_CUDA(c, mp::launch_checkpoint(p, static_cast<cudaStream_t>(stream)));
+  c->eng.kernels += 1;
+  return MP_OK;
+}
+
+int mp_restore(mp_ctx* c, const int8_t* q, int64_t ldq, const float* scale, int m, int k, void* x, int64_t ldx,
+               void* stream) {
+  if (c == nullptr) return MP_EINVAL;
+  if (k <= 0) return fail(c, MP_EINVAL, "k must be positive (got %d)", k);
+  int rc = check_x(c, x, ldx, k, m);
+  if (rc != MP_OK) return rc;
+  if (q == nullptr || scale == nullptr || reinterpret_cast<uintptr_t>(q) % 16 != 0 || ldq < k || ldq % 16 != 0)
+    return fail(c, MP_EINVAL, "checkpoint: codes 16-byte aligned, pitch >= k and a multiple of 16, and scales");
+  rc = use_device(c);
+  if (rc != MP_OK) return rc;
+  const mp::CheckpointParams p{nullptr, static_cast<uint16_t*>(x), ldx, const_cast<int8_t*>(q), ldq,
+                               const_cast<float*>(scale), m, k};
+  MP_CUDA(c, mp::launch_restore(p, static_cast<cudaStream_t>(stream)));
+  c->eng.kernels += 1;
+  return MP_OK;
+}
+
+}  // extern "C"

@@ -6,6 +6,7 @@
 
 #include <cuda.h>
 #include <stdint.h>
+#include <vector_types.h>
 
 namespace mp {
 
@@ -27,6 +28,7 @@ constexpr int kHeadDim = 128;      // attention head width (one CTA's features)
 
 // Device-side error word bits (OR-ed by kernels, read by mp_sync_check).
 constexpr uint32_t kErrTimeout = 1u;
+constexpr uint32_t kErrRequests = 2u;  // a request plan met a length or adapter index out of range
 
 // Optional epilogue scaling of the rank-space intermediate: the value in
 // token row t and rank column j is multiplied by
@@ -116,6 +118,15 @@ struct ProjParams {
   int32_t lora_apart;
   int32_t z_first;
   int32_t z_count;
+  // Adapters by request (ext_first != null, a single member): the appended K
+  // tiles of token tile tt are those of the list entries ext_list[ext_first[tt]]
+  // .. [+ ext_live[tt] - 1], ext_chunks 64-wide tiles each. An entry {b, a}
+  // takes its rank-space rows from the n_tok rows of tm_t from row b * n_tok
+  // (zero in the rows of other requests) and the factor B from row a * N of tm_b.
+  const int32_t* ext_first;
+  const int32_t* ext_live;
+  const int2* ext_list;
+  int32_t ext_chunks;
   // Fused rank-space prologue (n_pre > 0): before their member tiles, the
   // pairs with the fewest member tiles run n_pre prologue units, each the
   // full-K product of 512 token rows x 256 rank rows of T = scale ⊙ (x ·
@@ -131,6 +142,78 @@ struct ProjParams {
   uint32_t epoch;
   ProjMember pre;
   ProjMember mem[kMaxMembers];
+};
+
+// A batch of requests with adapters of their own, on the device (built by
+// plan_requests_kernel from the requests' lengths, adapters and strengths). A
+// request is LIVE when it has rows, an adapter and a strength that is not 0.
+// Per level l, for token tiles of T = 64 << l rows:
+//   block[l][t + q] = {t, first row, row past the last, adapter} for the rows
+//     of live request q in tile t, block_s its strength; adapter -1 where
+//     there are none. (Rows are in request order, so t + q is one pair's only.)
+//   list[l][first[l][t] + i], i < live[l][t]: tile t's {block, adapter}.
+// chunk[i]: the live requests' rows in runs of at most kChunkRows, as {first
+//   row, rows | q << 8, adapter, strength bits}; unused: 0 rows.
+// seg[begin[a]] .. seg[begin[a + 1] - 1]: the row ranges of adapter a.
+// row_adapter[row]: the adapter of the row's live request, else -1.
+constexpr int kPlanLevels = 4;      // token tiles of 64, 128, 256 and 512 rows
+constexpr int kChunkRows = 8;
+constexpr int kMaxRequests = 4096;
+constexpr int kMaxAdapters = 4096;
+constexpr int kMaxAdapterRank = 128;
+
+struct RequestPlan {
+  int32_t n_req, m, cap;
+  int4* block[kPlanLevels];
+  float* block_s[kPlanLevels];
+  int2* list[kPlanLevels];
+  int32_t* first[kPlanLevels];
+  int32_t* live[kPlanLevels];
+  int4* chunk;
+  int2* seg;
+  int32_t* begin;
+  int32_t* row_adapter;
+};
+
+inline __host__ __device__ int plan_tiles(int m, int level) { return (m + (64 << level) - 1) / (64 << level); }
+inline __host__ __device__ int plan_blocks(int m, int n_req, int level) { return plan_tiles(m, level) + n_req; }
+inline __host__ __device__ int plan_chunks(int m, int n_req) { return m / kChunkRows + n_req; }
+
+struct PlanParams {
+  RequestPlan plan;
+  const int32_t* lengths;   // [n_req]
+  const int32_t* adapters;  // [n_req], -1: none
+  const float* strengths;   // [n_req], or null: all 1
+  uint32_t* err;
+};
+
+// Finishes adapter `index` of a bank after its factors' valid parts were
+// copied in: zeros past rank, zeros in place of values that are not finite
+// (then bad[index] = 1), and the transposed copies of a training bank.
+struct BankSetParams {
+  uint16_t* a;   // [rp][kp] of this adapter
+  uint16_t* b;   // [n][rp]
+  uint16_t* at;  // [k][rp] or null
+  uint16_t* bt;  // [rp][np] or null
+  int32_t* bad;
+  int32_t n, k, rank, rp, kp, np;
+};
+
+// Rank-space rows of a batch of requests: v = s_q (x F_q^T), F_q [rp][k].
+struct RankParams {
+  const uint16_t* x;  // bf16 [m][ldx]
+  int64_t ldx;
+  const uint16_t* f;  // bf16 [cap][rp][fp]
+  int32_t fp, k, rp;
+  const int32_t* bad;
+  RequestPlan plan;
+  // outputs (either may be null)
+  float* v32;         // f32 [m][ld32], columns < rp; live rows only
+  int64_t ld32;
+  uint16_t* vblk;     // bf16 blocks of 64 << lvl rows by plan block, width ldb
+  int32_t lvl, ldb;
+  uint64_t wait_limit_ns;
+  uint32_t* err;
 };
 
 constexpr int kPreTok = 512;  // token rows of a prologue unit (two accumulators, as member tiles)
@@ -205,6 +288,46 @@ struct AttnParams {
   float scale_log2;  // softmax scale · log2(e)
   uint64_t wait_limit_ns;
   uint32_t* err;
+};
+
+// 8-bit activation checkpoint (mp_checkpoint.cu): per row and group of
+// kCkGroup features, scale = max|x| / 127 and q = rint(x * (127 / max|x|));
+// groups whose max|x| is below kCkTiny hold zeros.
+constexpr int kCkGroup = 128;
+constexpr float kCkTiny = 7.703719777548943e-34f;  // 2^-110
+
+struct CheckpointParams {
+  const uint16_t* x;  // bf16 [m][ldx] (store)
+  uint16_t* y;        // bf16 [m][ldx] (restore)
+  int64_t ldx;
+  int8_t* q;          // [m][ldq]
+  int64_t ldq;
+  float* scale;       // [groups][m]
+  int32_t m, k;
+};
+
+// Gradients of the adapters' factors: for every adapter a,
+//   out[a] = sum over its rows t of u[t] (outer) x[t],  u f32 [m][ldu].
+// Two products in one launch: dA (out [cap][r][k], features fastest) from x
+// and u = s dy B, dB (out [cap][n][r], ranks fastest) from dy and v.
+struct GradMember {
+  const uint16_t* x;   // bf16 [m][ldx], or null: the checkpoint below
+  int64_t ldx;
+  const int8_t* q;     // codes [m][ldq]
+  int64_t ldq;
+  const float* scale;  // [groups][m]
+  const float* u;      // f32 [m][ldu]
+  int64_t ldu;
+  float* out;
+  int32_t width;       // features
+  int32_t rank_major;  // 1: out [cap][r][width]; 0: out [cap][width][r]
+};
+
+struct GradParams {
+  GradMember mem[2];
+  int32_t n_mem;
+  int32_t r;  // ranks written
+  RequestPlan plan;
 };
 struct RmsResidualParams {
   uint16_t* x;

@@ -204,6 +204,7 @@ struct Tile {
   int half;      // token rows of each sub-tile this CTA loads
   int kt_begin;  // K tiles [kt_begin, kt_end); those >= base_kt are appended LoRA tiles
   int kt_end;
+  int ext0;      // adapters by request: the tile's first list entry
 };
 
 __device__ __forceinline__ Tile decode_tile(const ProjParams& p, int tile, int rank, int base_kt) {
@@ -245,6 +246,11 @@ __device__ __forceinline__ Tile decode_tile(const ProjParams& p, int tile, int r
   t.n_sub = (most == 2 && t.t0 + t.sub >= p.M) ? 1 : most;
   t.kt_begin = 0;
   t.kt_end = base_kt + p.mem[mi].lora_ktiles;
+  t.ext0 = 0;
+  if (p.ext_first != nullptr) {
+    t.ext0 = p.ext_first[tt];
+    t.kt_end = base_kt + p.ext_live[tt] * p.ext_chunks;
+  }
   if (p.ksplit > 1) {
     const int base_splits = p.lora_apart ? p.ksplit - 1 : p.ksplit;
     if (t.z >= base_splits) {
@@ -273,6 +279,7 @@ __device__ __forceinline__ Tile decode_pre(const ProjParams& p, int v, int rank,
   t.n_sub = t.t0 + kSubTok < p.M ? 2 : 1;
   t.kt_begin = 0;
   t.kt_end = base_kt;
+  t.ext0 = 0;
   return t;
 }
 
@@ -393,7 +400,16 @@ __device__ void pair_producer(const ProjParams& p, const PairSmem& sm, bool lead
         break;
       }
       const CUtensorMap* xmap = lora ? &mb.tm_t : &p.tm_x;
-      const int xk = (lora ? kt - base_kt : kt) * kBlockK;
+      int xk = (lora ? kt - base_kt : kt) * kBlockK;
+      int xrow = t.t0;                               // first row of the tile in xmap
+      int brow = mb.swiglu ? 2 * t.f0 : t.f0;        // SwiGLU: the interleaved B stack holds 128 rows per 64 features
+      if (lora && p.ext_first != nullptr) {          // adapters by request
+        const int e = (kt - base_kt) / p.ext_chunks;
+        xk = (kt - base_kt - e * p.ext_chunks) * kBlockK;
+        const int2 ent = p.ext_list[t.ext0 + e];
+        xrow = ent.x * p.n_tok;
+        brow = ent.y * mb.N + t.f0;
+      }
       if (!lora && quant) {
         if (leader) mbar_arrive_expect_tx(full_local, xbytes_pair);
         const uint32_t cbar = smem_u32(&sm.cfull[s]);
@@ -415,8 +431,7 @@ __device__ void pair_producer(const ProjParams& p, const PairSmem& sm, bool lead
           mbar_arrive_count(full_local, 2 * kDeqThreads / 32);  // no dequant: the dequantizers' share
         }
         if (lora) {
-          // SwiGLU: the interleaved B stack holds 128 rows per 64 features
-          tma_load_2d_pair(wb, &mb.tm_b, full_leader, xk, mb.swiglu ? 2 * t.f0 : t.f0);
+          tma_load_2d_pair(wb, &mb.tm_b, full_leader, xk, brow);
         } else if (mb.swiglu) {
           tma_load_2d_pair(wb, &mb.tm_w, full_leader, xk, t.f0);
           tma_load_2d_pair(wb + kWStageBytes / 2, &mb.tm_w3, full_leader, xk, t.f0);
@@ -426,7 +441,7 @@ __device__ void pair_producer(const ProjParams& p, const PairSmem& sm, bool lead
       }
       for (int j = 0; j < t.n_sub; ++j)
         tma_load_2d_pair(xb + j * sub_bytes, xmap, full_leader, xk,
-                         t.t0 + j * t.sub + rank * t.half);
+                         xrow + j * t.sub + rank * t.half);
       pend_full |= bit;
       pend_full_par = (pend_full_par & ~bit) | ((ph & 1u) << s);
     }

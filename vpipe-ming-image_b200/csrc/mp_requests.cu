@@ -1,0 +1,404 @@
+// Adapters by request: the plan of a batch, the adapter bank's layout, and the
+// rank-space rows of a batch whose requests each have an adapter of their own.
+//
+//   y[t] = W x[t] + s_q B_a (A_a x[t])      row t of request q, adapter a = a_q
+//
+// The product with W and the one with B_a are one pass of the projection
+// kernel (mp_proj.cu), which takes each token tile's adapters as appended K
+// tiles; what is here computes v[t] = s_q A_a x[t] for it and, in the backward
+// pass, u[t] = s_q B_a^T dy[t] (the same kernel on the transposed factors).
+#include <cuda_runtime.h>
+
+#include "mp_device.cuh"
+#include "mp_kernels.h"
+
+namespace mp {
+
+namespace {
+
+// ---- plan --------------------------------------------------------------------
+
+constexpr int kPlanThreads = 1024;
+constexpr int kPerThread = kMaxRequests / kPlanThreads;
+
+// Exclusive prefix sum over the block of each thread's kPerThread values, in place.
+__device__ void scan_block(int (&v)[kPerThread], int* warp_sums) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int sum = 0;
+#pragma unroll
+  for (int i = 0; i < kPerThread; ++i) sum += v[i];
+  int inc = sum;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int o = __shfl_up_sync(0xFFFFFFFFu, inc, d);
+    if (lane >= d) inc += o;
+  }
+  if (lane == 31) warp_sums[warp] = inc;
+  __syncthreads();
+  if (warp == 0) {
+    const int w = warp_sums[lane];
+    int wi = w;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int o = __shfl_up_sync(0xFFFFFFFFu, wi, d);
+      if (lane >= d) wi += o;
+    }
+    warp_sums[lane] = wi - w;
+  }
+  __syncthreads();
+  int at = warp_sums[warp] + inc - sum;
+#pragma unroll
+  for (int i = 0; i < kPerThread; ++i) {
+    const int x = v[i];
+    v[i] = at;
+    at += x;
+  }
+  __syncthreads();
+}
+
+// Largest q with start[q] <= row, over start[0 .. n] (start[0] = 0).
+__device__ __forceinline__ int last_at(const int* start, int n, int row) {
+  int lo = 0, hi = n;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (start[mid] <= row)
+      lo = mid;
+    else
+      hi = mid - 1;
+  }
+  return lo;
+}
+
+// One block: lengths are clamped to [0, what is left of m] and adapters
+// outside [-1, cap) dropped (kErrRequests then tells the host). All outputs
+// are integers in a fixed order, the same for the same inputs.
+__global__ void __launch_bounds__(kPlanThreads) plan_requests_kernel(const __grid_constant__ PlanParams p) {
+  __shared__ int start[kMaxRequests + 1];
+  __shared__ int adapter[kMaxRequests];
+  __shared__ int warp_sums[32];
+  const RequestPlan& pl = p.plan;
+  const int n = pl.n_req, tid = threadIdx.x;
+  pdl_wait();
+  pdl_release();
+
+  int len[kPerThread], at[kPerThread];
+  bool bad = false;
+#pragma unroll
+  for (int i = 0; i < kPerThread; ++i) {
+    const int q = tid * kPerThread + i;
+    int l = q < n ? p.lengths[q] : 0;
+    if (l < 0 || l > pl.m) {
+      bad = true;
+      l = l < 0 ? 0 : pl.m;
+    }
+    len[i] = at[i] = l;
+  }
+  // lengths are at most m < 2^31 / kMaxRequests, so their sum fits
+  scan_block(at, warp_sums);
+#pragma unroll
+  for (int i = 0; i < kPerThread; ++i) {
+    const int q = tid * kPerThread + i;
+    if (at[i] + len[i] > pl.m) bad = true;
+    if (q < n) start[q] = min(at[i], pl.m);
+    if (q == n - 1) start[n] = min(at[i] + len[i], pl.m);
+  }
+  if (n == 0 && tid == 0) start[0] = 0;
+  __syncthreads();
+  int chunks[kPerThread];
+#pragma unroll
+  for (int i = 0; i < kPerThread; ++i) {
+    const int q = tid * kPerThread + i;
+    chunks[i] = 0;
+    if (q >= n) continue;
+    int a = p.adapters[q];
+    if (a < -1 || a >= pl.cap) {
+      bad = true;
+      a = -1;
+    }
+    const int rows = start[q + 1] - start[q];
+    if (rows == 0 || (p.strengths != nullptr && p.strengths[q] == 0.0f)) a = -1;
+    adapter[q] = a;
+    if (a >= 0) chunks[i] = (rows + kChunkRows - 1) / kChunkRows;
+  }
+  if (bad) atomicOr(p.err, kErrRequests);
+  __syncthreads();
+
+  // chunks of the live requests' rows
+  const int n_chunk = plan_chunks(pl.m, n);
+  int chunk_at[kPerThread];
+#pragma unroll
+  for (int i = 0; i < kPerThread; ++i) chunk_at[i] = chunks[i];
+  scan_block(chunk_at, warp_sums);
+#pragma unroll
+  for (int i = 0; i < kPerThread; ++i) {
+    const int q = tid * kPerThread + i;
+    if (q >= n) continue;
+    const float s = p.strengths != nullptr ? p.strengths[q] : 1.0f;
+    for (int c = 0; c < chunks[i]; ++c) {
+      const int r0 = start[q] + c * kChunkRows;
+      const int rows = min(kChunkRows, start[q + 1] - r0);
+      pl.chunk[chunk_at[i] + c] = make_int4(r0, rows | (q << 8), adapter[q], __float_as_int(s));
+    }
+  }
+  if (tid == kPlanThreads - 1) warp_sums[0] = chunk_at[kPerThread - 1] + chunks[kPerThread - 1];
+  __syncthreads();
+  for (int i = warp_sums[0] + tid; i < n_chunk; i += kPlanThreads) pl.chunk[i] = make_int4(0, 0, -1, 0);
+
+  // row ranges by adapter: a live request's place is the number of live ones
+  // that have a lower adapter, or the same one and come before it
+  for (int q = tid; q < n; q += kPlanThreads) {
+    const int a = adapter[q];
+    if (a < 0) continue;
+    int place = 0;
+    for (int j = 0; j < n; ++j) {
+      const int b = adapter[j];
+      place += (b >= 0 && (b < a || (b == a && j < q))) ? 1 : 0;
+    }
+    pl.seg[place] = make_int2(start[q], start[q + 1]);
+  }
+  for (int a = tid; a <= pl.cap; a += kPlanThreads) {
+    int below = 0;
+    for (int j = 0; j < n; ++j) below += (adapter[j] >= 0 && adapter[j] < a) ? 1 : 0;
+    pl.begin[a] = below;
+  }
+
+  for (int r = tid; r < pl.m; r += kPlanThreads)
+    pl.row_adapter[r] = r < start[n] ? adapter[last_at(start, n, r)] : -1;
+
+  // blocks and lists of every level's token tiles
+  for (int l = 0; l < kPlanLevels; ++l) {
+    const int tile = 64 << l, tiles = plan_tiles(pl.m, l), blocks = plan_blocks(pl.m, n, l);
+    for (int b = tid; b < blocks; b += kPlanThreads) pl.block[l][b] = make_int4(-1, 0, 0, -1);
+    __syncthreads();
+    for (int t = tid; t < tiles; t += kPlanThreads) {
+      const int row0 = t * tile, row1 = min(row0 + tile, pl.m);
+      int live = 0, first = 0;
+      if (n > 0 && row0 < start[n]) {
+        const int q0 = last_at(start, n, row0);
+        first = t + q0;
+        for (int q = q0; q < n && start[q] < row1; ++q) {
+          if (adapter[q] < 0) continue;
+          const int lo = max(start[q], row0), hi = min(start[q + 1], row1);
+          if (lo >= hi) continue;
+          pl.block[l][t + q] = make_int4(t, lo, hi, adapter[q]);
+          pl.block_s[l][t + q] = p.strengths != nullptr ? p.strengths[q] : 1.0f;
+          pl.list[l][first + live] = make_int2(t + q, adapter[q]);
+          ++live;
+        }
+      }
+      pl.first[l][t] = first;
+      pl.live[l][t] = live;
+    }
+  }
+}
+
+// ---- adapter bank -------------------------------------------------------------
+
+__device__ __forceinline__ bool finite_bf16(uint16_t v) { return (v & 0x7F80u) != 0x7F80u; }
+
+// 32 x 32 tiles over [rows][cols]: `src` (pitch ld) in place, zeros past
+// (rows_ok, cols_ok) and for values that are not finite; the transposed tile
+// into `dst` ([cols_t][rows], pitch ld_t) when it is not null.
+__device__ void finish_tile(uint16_t* src, int ld, uint16_t* dst, int ld_t, int rows, int cols, int rows_ok,
+                            int cols_ok, int cols_t, int r0, int c0, int32_t* bad, uint16_t (&sm)[32][33]) {
+  const int c = threadIdx.x & 31;
+  for (int r = threadIdx.x >> 5; r < 32; r += 8) {
+    uint16_t v = 0;
+    if (r0 + r < rows && c0 + c < cols) {
+      uint16_t* at = src + static_cast<size_t>(r0 + r) * ld + c0 + c;
+      if (r0 + r < rows_ok && c0 + c < cols_ok) v = *at;
+      if (!finite_bf16(v)) {
+        v = 0;
+        *bad = 1;
+      }
+      *at = v;
+    }
+    sm[r][c] = v;
+  }
+  __syncthreads();
+  if (dst != nullptr) {
+    for (int r = threadIdx.x >> 5; r < 32; r += 8)
+      if (c0 + r < cols_t && r0 + c < rows) dst[static_cast<size_t>(c0 + r) * ld_t + r0 + c] = sm[c][r];
+  }
+}
+
+__global__ void __launch_bounds__(256) bank_set_kernel(const __grid_constant__ BankSetParams p) {
+  __shared__ uint16_t sm[32][33];
+  const int rt = (p.rp + 31) / 32, kt = (p.kp + 31) / 32, nt = (p.n + 31) / 32;
+  int i = blockIdx.x;
+  if (i < rt * kt) {  // A [rp][kp], transposed [k][rp]
+    finish_tile(p.a, p.kp, p.at, p.rp, p.rp, p.kp, p.rank, p.k, p.k, i / kt * 32, i % kt * 32, p.bad, sm);
+  } else {  // B [n][rp], transposed [rp][np]
+    i -= rt * kt;
+    if (i < rt * nt)
+      finish_tile(p.b, p.rp, p.bt, p.np, p.n, p.rp, p.n, p.rank, p.rp, i / rt * 32, i % rt * 32, p.bad, sm);
+  }
+}
+
+// ---- rank-space rows, few at a time --------------------------------------------
+
+// D[16][8] += A[16][16] B[16][8]: bf16 in, f32 out (the warp-wide fragments of mma.sync).
+__device__ __forceinline__ void mma_16x8x16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                            uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// 16 bf16 values of a row from column c (a multiple of 16; the row is 16-byte
+// aligned), zeros from column k on and where !ok: nothing past the k-th value
+// is read.
+__device__ __forceinline__ void load16(const uint16_t* row, int c, int k, bool ok, uint32_t (&w)[8]) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int at = c + 8 * h;
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (ok && at + 8 <= k) {
+      v = *reinterpret_cast<const uint4*>(row + at);
+    } else if (ok && at < k) {
+      uint16_t e[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) e[j] = at + j < k ? row[at + j] : static_cast<uint16_t>(0);
+      v = make_uint4(e[0] | (e[1] << 16), e[2] | (e[3] << 16), e[4] | (e[5] << 16), e[6] | (e[7] << 16));
+    }
+    w[4 * h] = v.x;
+    w[4 * h + 1] = v.y;
+    w[4 * h + 2] = v.z;
+    w[4 * h + 3] = v.w;
+  }
+}
+
+constexpr int kRankWarps = 8;
+
+// One block: 16 ranks of one chunk (at most 8 rows of one request); its warps
+// take the 64-wide K groups in turn and their sums are added in warp order.
+// Within a group lane (g, j) (g = lane / 4, j = lane % 4) holds columns
+// 16 j .. 16 j + 15 of ranks g and g + 8 and of row g: both operands of the
+// four MMAs of a group then come from two 16-byte loads each, the K columns
+// taken in the same order in both.
+__global__ void __launch_bounds__(32 * kRankWarps) rank_rows_kernel(const __grid_constant__ RankParams p) {
+  __shared__ float part[kRankWarps][16][kChunkRows];
+  pdl_wait();
+  pdl_release();
+  const int4 ch = p.plan.chunk[blockIdx.x];
+  const int rows = ch.y & 0xFF;
+  if (rows == 0) return;
+  const int req = ch.y >> 8, adapter = ch.z;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, j = lane & 3;
+  const int r0 = blockIdx.y * 16;
+  const uint16_t* fa = p.f + (static_cast<size_t>(adapter) * p.rp + r0 + g) * p.fp;
+  const uint16_t* fb = fa + static_cast<size_t>(8) * p.fp;
+  const uint16_t* xr = p.x + static_cast<int64_t>(ch.x + min(g, rows - 1)) * p.ldx;
+  float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  const int groups = (p.k + 63) / 64;
+  for (int i = warp; i < groups; i += kRankWarps) {
+    const int c = 64 * i + 16 * j;
+    uint32_t wa[8], wb[8], wx[8];
+    load16(fa, c, p.k, true, wa);
+    load16(fb, c, p.k, true, wb);
+    load16(xr, c, p.k, g < rows, wx);
+#pragma unroll
+    for (int s = 0; s < 4; ++s)
+      mma_16x8x16(d, wa[2 * s], wb[2 * s], wa[2 * s + 1], wb[2 * s + 1], wx[2 * s], wx[2 * s + 1]);
+  }
+  part[warp][g][2 * j] = d[0];
+  part[warp][g][2 * j + 1] = d[1];
+  part[warp][g + 8][2 * j] = d[2];
+  part[warp][g + 8][2 * j + 1] = d[3];
+  __syncthreads();
+  const int r = threadIdx.x & 15, row = threadIdx.x >> 4;
+  if (row >= rows) return;
+  float sum = part[0][r][row];
+#pragma unroll
+  for (int w = 1; w < kRankWarps; ++w) sum += part[w][r][row];
+  sum *= __int_as_float(ch.w);
+  // a factor that is not finite is stored as zeros; its request's rows are NaN
+  if (p.bad[adapter] != 0) sum = __int_as_float(0x7FC00000);
+  const int t = ch.x + row;
+  if (p.v32 != nullptr) p.v32[static_cast<int64_t>(t) * p.ld32 + r0 + r] = sum;
+  if (p.vblk != nullptr) {
+    const int tile = t >> (6 + p.lvl);
+    const int64_t at = (static_cast<int64_t>(tile + req) << (6 + p.lvl)) + (t & ((64 << p.lvl) - 1));
+    p.vblk[at * p.ldb + r0 + r] = __bfloat16_as_ushort(__float2bfloat16_rn(sum));
+  }
+}
+
+// ---- dense transpose of a projection weight -------------------------------------
+
+// dst[k][n] (pitch np) = bf16 weight [n][k]: the values the projection kernel
+// multiplies with (packed codes dequantized with its arithmetic and rounding).
+__global__ void __launch_bounds__(256) weight_transpose_kernel(const uint8_t* w, const uint32_t* sb, int sb_stride,
+                                                               int n, int k, int kp, int bits, uint32_t code_xor,
+                                                               float code_offset, uint16_t* dst, int np) {
+  __shared__ uint16_t sm[32][33];
+  const int c = threadIdx.x & 31, n0 = blockIdx.y * 32, k0 = blockIdx.x * 32;
+  for (int r = threadIdx.x >> 5; r < 32; r += 8) {
+    uint16_t v = 0;
+    if (n0 + r < n && k0 + c < k) {
+      const size_t row = n0 + r;
+      const int col = k0 + c;
+      if (bits == 0) {
+        v = reinterpret_cast<const uint16_t*>(w)[row * kp + col];
+      } else {
+        const uint32_t word = sb[row * sb_stride + (col >> 6)];
+        const float sc = bf16_bits_to_f32(word & 0xFFFFu), bi = bf16_bits_to_f32(word >> 16);
+        const float bf = fmaf(-sc, code_offset, bi);
+        uint32_t q;
+        if (bits == 8)
+          q = w[row * k + col] ^ (code_xor & 0xFFu);
+        else
+          q = (w[row * (k / 2) + (col >> 1)] >> (4 * (col & 1))) & 0xFu;
+        v = __bfloat16_as_ushort(__float2bfloat16_rn(fmaf(32768.0f + static_cast<float>(q), sc, bf)));
+      }
+    }
+    sm[r][c] = v;
+  }
+  __syncthreads();
+  for (int r = threadIdx.x >> 5; r < 32; r += 8)
+    if (k0 + r < k && n0 + c < np) dst[static_cast<size_t>(k0 + r) * np + n0 + c] = sm[c][r];
+}
+
+// A launch that may begin its set-up while the one before it on the stream ends.
+template <class P>
+cudaError_t launch_overlapped(void (*kernel)(P), dim3 grid, dim3 block, const P& p, cudaStream_t stream) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, p);
+}
+
+}  // namespace
+
+cudaError_t launch_plan_requests(const PlanParams& p, cudaStream_t stream) {
+  return launch_overlapped(plan_requests_kernel, dim3(1), dim3(kPlanThreads), p, stream);
+}
+
+cudaError_t launch_bank_set(const BankSetParams& p, cudaStream_t stream) {
+  const int rt = (p.rp + 31) / 32, kt = (p.kp + 31) / 32, nt = (p.n + 31) / 32;
+  bank_set_kernel<<<rt * (kt + nt), 256, 0, stream>>>(p);
+  return cudaGetLastError();
+}
+
+cudaError_t launch_rank_rows(const RankParams& p, cudaStream_t stream) {
+  const dim3 grid(plan_chunks(p.plan.m, p.plan.n_req), p.rp / 16);
+  if (grid.x == 0) return cudaSuccess;  // no request
+  return launch_overlapped(rank_rows_kernel, grid, dim3(32 * kRankWarps), p, stream);
+}
+
+cudaError_t launch_weight_transpose(const void* w, const uint32_t* sb, int sb_stride, int n, int k, int kp, int bits,
+                                    uint32_t code_xor, float code_offset, uint16_t* dst, int np,
+                                    cudaStream_t stream) {
+  const dim3 grid((k + 31) / 32, (np + 31) / 32);
+  weight_transpose_kernel<<<grid, 256, 0, stream>>>(static_cast<const uint8_t*>(w), sb, sb_stride, n, k, kp, bits,
+                                                    code_xor, code_offset, dst, np);
+  return cudaGetLastError();
+}
+
+}  // namespace mp

@@ -89,6 +89,21 @@ SIGNATURES = {
     "mp_pack_upload": (C.c_int, [_vp, _vp, C.c_char_p, C.POINTER(_vp)]),
     "mp_pack_quantize": (C.c_int, [C.c_char_p, C.c_char_p, C.c_int, C.POINTER(C.c_int),
                                    C.POINTER(C.c_int)]),
+    "mp_adapters_create": (C.c_int, [_vp, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int,
+                                     C.POINTER(_vp)]),
+    "mp_adapters_free": (C.c_int, [_vp, _vp]),
+    "mp_adapters_set": (C.c_int, [_vp, _vp, C.c_int, _vp, _vp, C.c_int, _vp]),
+    "mp_adapters_rank_pad": (C.c_int, [_vp]),
+    "mp_requests_create": (C.c_int, [_vp, C.c_int, C.c_int, C.c_int, C.POINTER(_vp)]),
+    "mp_requests_free": (C.c_int, [_vp, _vp]),
+    "mp_requests_plan": (C.c_int, [_vp, _vp, _vp, _vp, _vp, C.c_int, C.c_int, _vp]),
+    "mp_linear_requests": (C.c_int, [_vp, _vp, _vp, _i64, _vp, _vp, _vp, _i64, _vp, _i64, C.c_int,
+                                     _vp]),
+    "mp_weight_transpose": (C.c_int, [_vp, _vp, _vp, C.POINTER(_vp)]),
+    "mp_linear_requests_grad": (C.c_int, [_vp, _vp, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _i64,
+                                          _vp, _vp, _vp, _i64, _vp, _vp, C.c_int, _vp]),
+    "mp_checkpoint": (C.c_int, [_vp, _vp, _i64, C.c_int, C.c_int, _vp, _i64, _vp, _vp]),
+    "mp_restore": (C.c_int, [_vp, _vp, _i64, _vp, C.c_int, C.c_int, _vp, _i64, _vp]),
     "mp_engagement_get": (C.c_int, [_vp, C.POINTER(Engagement)]),
     "mp_engagement_reset": (C.c_int, [_vp]),
 }

@@ -14,6 +14,11 @@ reference's per-projection surface.
   fill_mod (:2266-2273), all blocks at once         Context.modulation(set, temb)
   DitEngagement (src/ming-dit.h:55-103)             Context.engagement()
 
+Without a counterpart there: a batch of requests with an adapter each
+(Context.adapters, .requests, .linear_requests), its backward pass
+(.linear_requests_grad, .transposed) and 8-bit activation checkpoints
+(.checkpoint, .restore).
+
 Device memory, streams and tensors are torch's; every computation is a call
 into libmingproj.so. There is no CPU path here.
 """
@@ -143,6 +148,102 @@ class ModSet:
         if self.handle:
             self.ctx.lib.mp_modulation_free(self.ctx.h, self.handle)
             self.handle = None
+
+
+class Adapters:
+    """A bank of low-rank adapters for projections of one shape [n, k]."""
+
+    def __init__(self, ctx: "Context", handle: C.c_void_p, n: int, k: int, capacity: int,
+                 max_rank: int, training: bool):
+        self.ctx, self.handle = ctx, handle
+        self.n, self.k, self.capacity, self.max_rank = n, k, capacity, max_rank
+        self.training = training
+        self.rank_pad = int(ctx.lib.mp_adapters_rank_pad(handle))
+
+    def set(self, index: int, a, b, stream=None) -> None:
+        """a: bf16 [rank, k] (alpha folded in), b: bf16 [n, rank]; torch bf16
+        tensors or uint16 numpy arrays, host or device."""
+        a = _as_bf16_bits(a)
+        b = _as_bf16_bits(b)
+        rank = a.shape[0]
+        if tuple(a.shape) != (rank, self.k) or tuple(b.shape) != (self.n, rank):
+            raise MPError(_lib.MP_EINVAL,
+                          f"adapter factors {tuple(a.shape)} / {tuple(b.shape)} do not fit "
+                          f"[{self.n}, {self.k}]")
+        self.ctx._check(self.ctx.lib.mp_adapters_set(self.ctx.h, self.handle, index, _ptr(a),
+                                                     _ptr(b), rank, _stream_handle(stream)))
+        _keep_for(stream, a, b)
+
+    def free(self) -> None:
+        if self.handle:
+            self.ctx.lib.mp_adapters_free(self.ctx.h, self.handle)
+            self.handle = None
+
+
+class Requests:
+    """The plan of a batch: the rows and the adapter of each request."""
+
+    def __init__(self, ctx: "Context", handle: C.c_void_p, capacity: int):
+        self.ctx, self.handle, self.capacity = ctx, handle, capacity
+
+    def plan(self, lengths, adapters, strengths=None, m: int | None = None, stream=None) -> None:
+        """lengths, adapters: int32 [requests]; strengths: f32 [requests] or
+        None (all 1); sequences, or tensors on the device. m: rows of the
+        batch (rows past the last request have no adapter); by default the
+        sum of the lengths, which has to be on the host then."""
+        dev = torch.device("cuda", self.ctx.device)
+        if m is None:
+            if isinstance(lengths, torch.Tensor) and lengths.is_cuda:
+                raise ValueError("m is required with lengths on the device")
+            m = int(sum(int(v) for v in lengths))
+        lengths = torch.as_tensor(lengths, dtype=torch.int32, device=dev).contiguous()
+        adapters = torch.as_tensor(adapters, dtype=torch.int32, device=dev).contiguous()
+        if strengths is not None:
+            strengths = torch.as_tensor(strengths, dtype=torch.float32, device=dev).contiguous()
+        n = lengths.numel()
+        if adapters.numel() != n or (strengths is not None and strengths.numel() != n):
+            raise ValueError("lengths, adapters and strengths must have one entry per request")
+        self.ctx._check(self.ctx.lib.mp_requests_plan(
+            self.ctx.h, self.handle, _ptr(lengths), _ptr(adapters), _ptr(strengths), n, int(m),
+            _stream_handle(stream)))
+        _keep_for(stream, lengths, adapters, strengths)
+
+    def free(self) -> None:
+        if self.handle:
+            self.ctx.lib.mp_requests_free(self.ctx.h, self.handle)
+            self.handle = None
+
+
+@dataclass
+class Checkpoint:
+    """bf16 rows [m, k] kept in 8 bits: int8 codes [m, k] (a view of rows padded
+    to 16) and f32 scales [m, groups], one for every 128 features of a row."""
+    codes: torch.Tensor
+    scales: torch.Tensor
+
+    @property
+    def shape(self):
+        return self.codes.shape
+
+
+def _keep_for(stream, *tensors) -> None:
+    """Memory read on `stream` is not reused before that stream has read it."""
+    if stream is not None:
+        for t in tensors:
+            if isinstance(t, torch.Tensor) and t.is_cuda:
+                t.record_stream(stream)
+
+
+def _rows(name: str, t: torch.Tensor, m: int, k: int, dtype=torch.bfloat16) -> None:
+    if not t.is_cuda or t.dtype != dtype or t.dim() != 2 or tuple(t.shape) != (m, k) or (
+            k > 1 and t.stride(1) != 1):
+        raise ValueError(f"{name} must be {dtype} [{m}, {k}] on the device, its rows contiguous "
+                         f"(got {t.dtype} {tuple(t.shape)}, strides {t.stride()})")
+
+
+def _pitch(t: torch.Tensor) -> int:
+    """Row pitch in elements; one row may have any stride, so its own length counts."""
+    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), (t.shape[1] + 15) // 16 * 16)
 
 
 class Context:
@@ -389,6 +490,116 @@ class Context:
             float(strength), _ptr(out), out.stride(0), m, _stream_handle(stream)))
         return out
 
+    # -- adapters by request ---------------------------------------------------
+    def adapters(self, n: int, k: int, capacity: int, max_rank: int,
+                 training: bool = False) -> Adapters:
+        """A bank of `capacity` adapters for projections [n, k]; `training`
+        also keeps what the backward pass reads."""
+        h = C.c_void_p()
+        self._check(self.lib.mp_adapters_create(self.h, n, k, capacity, max_rank, int(training),
+                                                C.byref(h)))
+        return Adapters(self, h, n, k, capacity, max_rank, training)
+
+    def requests(self, max_requests: int, max_rows: int, capacity: int) -> Requests:
+        """A plan for batches of up to max_requests requests over up to
+        max_rows rows, with adapters below `capacity`."""
+        h = C.c_void_p()
+        self._check(self.lib.mp_requests_create(self.h, max_requests, max_rows, capacity,
+                                                C.byref(h)))
+        return Requests(self, h, capacity)
+
+    def linear_requests(self, w: Weight, x: torch.Tensor, bank: Adapters, plan: Requests,
+                        out: torch.Tensor | None = None, ranks=False, stream=None):
+        """y[t] = x[t] · deq(W)^T + s_q (x[t] A_a^T) B_a^T, a the adapter of row
+        t's request q; x bf16 [m, k], m as planned. With ranks=True (or an f32
+        [m, bank.rank_pad] tensor) returns (y, v), v = s_q x A_a^T, which
+        linear_requests_grad takes."""
+        m = x.shape[0]
+        _rows("x", x, m, w.k)
+        if out is None:
+            out = _alloc_out(m, w.n, x.device)
+        else:
+            _rows("out", out, m, w.n)
+        v = None
+        if ranks is not False and ranks is not None:
+            v = ranks
+            if ranks is True:
+                v = torch.empty((m, bank.rank_pad), dtype=torch.float32, device=x.device)
+            _rows("ranks", v, m, bank.rank_pad, torch.float32)
+        self._check(self.lib.mp_linear_requests(
+            self.h, w.handle, _ptr(x), _pitch(x), bank.handle, plan.handle, _ptr(out), _pitch(out),
+            _ptr(v), _pitch(v) if v is not None else 0, m, _stream_handle(stream)))
+        return out if v is None else (out, v)
+
+    def transposed(self, w: Weight, stream=None) -> Weight:
+        """The dense bf16 transpose [k, n] of a projection weight [n, k]."""
+        h = C.c_void_p()
+        self._check(self.lib.mp_weight_transpose(self.h, w.handle, _stream_handle(stream),
+                                                 C.byref(h)))
+        return Weight(self, h, WeightInfo(w.k, w.n, 0, MP_QUANT_AFFINE))
+
+    def linear_requests_grad(self, wt: Weight, dy: torch.Tensor, x, v: torch.Tensor,
+                             bank: Adapters, plan: Requests, need_dx: bool = True,
+                             need_factors: bool = True, stream=None):
+        """The backward pass of linear_requests, W held fixed: (dx bf16 [m, k],
+        da f32 [capacity, max_rank, k], db f32 [capacity, n, max_rank]), None
+        for what is not needed; capacity is the plan's. wt: transposed(w); x:
+        bf16 [m, k] or its Checkpoint; v: the forward call's ranks."""
+        m, n, k = dy.shape[0], wt.k, wt.n
+        _rows("dy", dy, m, n)
+        dx = da = db = xt = xq = xs = None
+        if need_dx:
+            dx = _alloc_out(m, k, dy.device)
+        if need_factors:
+            if isinstance(x, Checkpoint):
+                xq, xs = x.codes, x.scales
+                _rows("x.codes", xq, m, k, torch.int8)
+                if xs.shape != (m, (k + 127) // 128) or xs.stride(0) != 1 or (
+                        xs.shape[1] > 1 and xs.stride(1) != m):
+                    raise ValueError("x.scales must be f32 [m, groups], a row of the batch apart "
+                                     "along the groups")
+            else:
+                xt = x
+                _rows("x", xt, m, k)
+            if v.dim() != 2 or v.shape[1] < bank.max_rank:
+                raise ValueError(f"v must have at least {bank.max_rank} columns")
+            _rows("v", v, m, v.shape[1], torch.float32)
+            da = torch.empty((plan.capacity, bank.max_rank, k), dtype=torch.float32,
+                             device=dy.device)
+            db = torch.empty((plan.capacity, n, bank.max_rank), dtype=torch.float32,
+                             device=dy.device)
+        self._check(self.lib.mp_linear_requests_grad(
+            self.h, wt.handle, _ptr(dy), _pitch(dy), _ptr(xt), _pitch(xt) if xt is not None else 0,
+            _ptr(xq), _pitch(xq) if xq is not None else 0, _ptr(xs),
+            _ptr(v) if need_factors else None, _pitch(v) if need_factors else 0, bank.handle,
+            plan.handle, _ptr(dx), _pitch(dx) if dx is not None else 0, _ptr(da), _ptr(db), m,
+            _stream_handle(stream)))
+        return dx, da, db
+
+    # -- activation checkpoints --------------------------------------------------
+    def checkpoint(self, x: torch.Tensor, stream=None) -> Checkpoint:
+        """bf16 rows [m, k] in 8 bits, a scale for every 128 features of a row."""
+        m, k = x.shape
+        _rows("x", x, m, k)
+        q = torch.empty((m, (k + 15) // 16 * 16), dtype=torch.int8, device=x.device)
+        scale = torch.empty(((k + 127) // 128, m), dtype=torch.float32, device=x.device)
+        self._check(self.lib.mp_checkpoint(self.h, _ptr(x), _pitch(x), m, k, _ptr(q), q.stride(0),
+                                           _ptr(scale), _stream_handle(stream)))
+        return Checkpoint(q[:, :k], scale.t())
+
+    def restore(self, saved: Checkpoint, out: torch.Tensor | None = None,
+                stream=None) -> torch.Tensor:
+        """The bf16 rows a checkpoint stands for."""
+        m, k = saved.shape
+        if out is None:
+            out = _alloc_out(m, k, saved.codes.device)
+        else:
+            _rows("out", out, m, k)
+        self._check(self.lib.mp_restore(self.h, _ptr(saved.codes), _pitch(saved.codes),
+                                        _ptr(saved.scales), m, k, _ptr(out), _pitch(out),
+                                        _stream_handle(stream)))
+        return out
+
     # -- modulation ----------------------------------------------------------
     def modulation_set(self, ada: list[Weight], biases, an1=None, fn1=None) -> ModSet:
         nb = len(ada)
@@ -433,4 +644,4 @@ class Context:
             pass
 
 
-__all__ = ["Context", "Weight", "ModSet", "MPError", "MP_QUANT_AFFINE", "MP_QUANT_SYMMETRIC"]
+__all__ = ["Context", "Weight", "ModSet", "Adapters", "Requests", "Checkpoint", "MPError", "MP_QUANT_AFFINE", "MP_QUANT_SYMMETRIC"]
