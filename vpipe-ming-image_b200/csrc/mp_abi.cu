@@ -2397,13 +2397,23 @@ int mp_linear_requests_grad(mp_ctx* c, const mp_weight* wt, const void* dy, int6
   std::memset(&g, 0, sizeof(g));
   g.r = b->max_rank;
   g.plan = r->plan;
+  g.rp = b->rp;
+  g.wait_limit_ns = c->wait_limit_ns;
+  g.err = c->err_word;
+  auto rows_map = [&](CUtensorMap* map, const void* base, int64_t ld, int width) {
+    return encode_2d(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, base, width, m, static_cast<uint64_t>(ld) * 2, 64, 64,
+                     CU_TENSOR_MAP_SWIZZLE_128B);
+  };
+  bool maps = true;
   if (da != nullptr) {
     mp::GradMember& mb = g.mem[g.n_mem++];
-    mb.x = xq != nullptr ? nullptr : static_cast<const uint16_t*>(x);
-    mb.ldx = ldx;
-    mb.q = xq;
-    mb.ldq = ldq;
-    mb.scale = xscale;
+    if (xq != nullptr) {
+      maps = encode_2d(&mb.tm_x, CU_TENSOR_MAP_DATA_TYPE_UINT8, xq, k, m, static_cast<uint64_t>(ldq), 128, 64,
+                       CU_TENSOR_MAP_SWIZZLE_NONE);
+      mb.scale = xscale;
+    } else {
+      maps = rows_map(&mb.tm_x, x, ldx, k);
+    }
     mb.u = c->req_u;
     mb.ldu = b->rp;
     mb.out = da;
@@ -2412,13 +2422,13 @@ int mp_linear_requests_grad(mp_ctx* c, const mp_weight* wt, const void* dy, int6
   }
   if (db != nullptr) {
     mp::GradMember& mb = g.mem[g.n_mem++];
-    mb.x = static_cast<const uint16_t*>(dy);
-    mb.ldx = ldy;
+    maps = maps && rows_map(&mb.tm_x, dy, ldy, n);
     mb.u = v;
     mb.ldu = ldv;
     mb.out = db;
     mb.width = n;
   }
+  if (!maps) return fail(c, MP_ECUDA, "tensor map encode failed (gradient rows)");
   if (g.n_mem > 0) {
     MP_CUDA(c, mp::launch_adapter_grad(g, s));
     c->eng.kernels += 1;

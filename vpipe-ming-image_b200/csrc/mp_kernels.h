@@ -311,11 +311,9 @@ struct CheckpointParams {
 // Two products in one launch: dA (out [cap][r][k], features fastest) from x
 // and u = s dy B, dB (out [cap][n][r], ranks fastest) from dy and v.
 struct GradMember {
-  const uint16_t* x;   // bf16 [m][ldx], or null: the checkpoint below
-  int64_t ldx;
-  const int8_t* q;     // codes [m][ldq]
-  int64_t ldq;
-  const float* scale;  // [groups][m]
+  CUtensorMap tm_x;    // bf16 [m, width] (box {64, 64}, SW128), or with `scale`
+                       // codes u8 [m, width] (box {128, 64}, no swizzle)
+  const float* scale;  // null, or the checkpoint's scales [groups][m]
   const float* u;      // f32 [m][ldu]
   int64_t ldu;
   float* out;
@@ -326,9 +324,13 @@ struct GradMember {
 struct GradParams {
   GradMember mem[2];
   int32_t n_mem;
-  int32_t r;  // ranks written
+  int32_t r, rp;    // ranks written, and rounded up to 16
+  int32_t splits;   // CTAs that share an adapter's rows (set by the launch)
   RequestPlan plan;
+  uint64_t wait_limit_ns;
+  uint32_t* err;
 };
+
 struct RmsResidualParams {
   uint16_t* x;
   int64_t ldx;
