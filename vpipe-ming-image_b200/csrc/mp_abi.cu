@@ -32,6 +32,7 @@ cudaError_t launch_attention(const AttnParams& p, cudaStream_t stream);
 cudaError_t launch_plan_requests(const PlanParams& p, cudaStream_t stream);
 cudaError_t launch_bank_set(const BankSetParams& p, cudaStream_t stream);
 cudaError_t launch_rank_rows(const RankParams& p, cudaStream_t stream);
+cudaError_t launch_few_rows(const FewParams& p, int bits, cudaStream_t stream);
 cudaError_t launch_adapter_grad(const GradParams& p, cudaStream_t stream);
 cudaError_t launch_checkpoint(const CheckpointParams& p, cudaStream_t stream);
 cudaError_t launch_restore(const CheckpointParams& p, cudaStream_t stream);
@@ -741,6 +742,7 @@ struct RequestsLaunch {
   const mp_adapters* bank = nullptr;
   const uint16_t* f = nullptr;  // rank-space factor [cap][rp][fp]
   int fp = 0;
+  const uint16_t* b = nullptr;  // the other factor [cap][n][rp]
   const CUtensorMap* tm_b = nullptr;
   float* v32 = nullptr;         // also kept in f32 (nullable)
   int64_t ld32 = 0;
@@ -2070,6 +2072,57 @@ int launch_request_ranks(mp_ctx* c, ProjParams* p, const RequestsLaunch& ext, co
   return MP_OK;
 }
 
+// One projection with its requests' adapters.
+int run_requests(mp_ctx* c, const mp_weight* w, const void* x, int64_t ldx, void* y, int64_t ldy, int m,
+                 RequestsLaunch* ext, cudaStream_t stream) {
+  if (m <= mp::kFewRows) {
+    if (ext->v32 == nullptr) {
+      int rc = ensure_buf(c, &c->req_u, &c->req_u_cap, static_cast<size_t>(m) * ext->bank->rp, stream);
+      if (rc != MP_OK) return rc;
+      ext->v32 = c->req_u;
+      ext->ld32 = ext->bank->rp;
+    }
+    int rc = launch_ranks(c, rank_params(c, *ext, x, ldx, w->d.k), stream);
+    if (rc != MP_OK) return rc;
+    mp::FewParams p;
+    p.x = static_cast<const uint16_t*>(x);
+    p.ldx = ldx;
+    p.w = static_cast<const uint8_t*>(w->w);
+    p.w_pitch = w->d.bits == 0 ? static_cast<size_t>(w->kp) * 2 : static_cast<size_t>(w->d.k) * w->d.bits / 8;
+    p.sb = w->sb;
+    p.sb_stride = w->sb_stride;
+    p.m = m;
+    p.n = w->d.n;
+    p.k = w->d.k;
+    const bool sym = w->d.bits == 8 && w->d.mode == MP_QUANT_SYMMETRIC;
+    p.code_xor = sym ? 0x80808080u : 0u;
+    p.zero = w->d.bits == 4 || sym ? 128.0f : 0.0f;
+    p.v = ext->v32;
+    p.ldv = ext->ld32;
+    p.b = ext->b;
+    p.rp = ext->bank->rp;
+    p.row_adapter = ext->req->plan.row_adapter;
+    p.y = static_cast<uint16_t*>(y);
+    p.ldy = ldy;
+    p.chunks = mp::plan_chunks(m, ext->req->plan.n_req);
+    cudaError_t e = mp::launch_few_rows(p, w->d.bits, stream);
+    if (e != cudaSuccess) return cuda_fail(c, e, "few_rows_kernel");
+    c->eng.kernels += 1;
+    count_projection(c, w, m, nullptr);
+  } else {
+    const mp_weight* wl[1] = {w};
+    void* yl[1] = {y};
+    const int64_t ll[1] = {ldy};
+    const Stack* sl[1] = {nullptr};
+    const int cl[1] = {0};
+    int rc = launch_projections(c, wl, yl, ll, sl, cl, 0, 1, x, ldx, m, stream, nullptr, nullptr, nullptr, true,
+                                nullptr, ext);
+    if (rc != MP_OK) return rc;
+  }
+  c->eng.lora_proj += 1;
+  return MP_OK;
+}
+
 int check_requests(mp_ctx* c, const mp_adapters* bank, const mp_requests* req, int n, int k, int m) {
   if (bank->n != n || bank->k != k)
     return fail(c, MP_EINVAL, "the adapters are for [%d, %d], the weight is [%d, %d]", bank->n, bank->k, n, k);
@@ -2297,19 +2350,13 @@ int mp_linear_requests(mp_ctx* c, const mp_weight* w, const void* x, int64_t ldx
   ext.bank = b;
   ext.f = b->a;
   ext.fp = b->kp;
+  ext.b = b->b;
   ext.tm_b = &b->tm_b;
   ext.v32 = ranks;
   ext.ld32 = ldr;
   if (ranks != nullptr)  // rows without an adapter
     MP_CUDA(c, cudaMemset2DAsync(ranks, static_cast<size_t>(ldr) * 4, 0, static_cast<size_t>(b->rp) * 4, m, s));
-  const mp_weight* wl[1] = {w};
-  void* yl[1] = {y};
-  const int64_t ll[1] = {ldy};
-  const Stack* sl[1] = {nullptr};
-  const int cl[1] = {0};
-  rc = launch_projections(c, wl, yl, ll, sl, cl, 0, 1, x, ldx, m, s, nullptr, nullptr, nullptr, true, nullptr, &ext);
-  if (rc == MP_OK) c->eng.lora_proj += 1;
-  return rc;
+  return run_requests(c, w, x, ldx, y, ldy, m, &ext, s);
 }
 
 int mp_weight_transpose(mp_ctx* c, const mp_weight* w, void* stream, mp_weight** out) {
@@ -2373,6 +2420,7 @@ int mp_linear_requests_grad(mp_ctx* c, const mp_weight* wt, const void* dy, int6
   ext.bank = b;
   ext.f = b->bt;
   ext.fp = b->np;
+  ext.b = b->at;
   ext.tm_b = &b->tm_at;
   if (da != nullptr) {
     rc = ensure_buf(c, &c->req_u, &c->req_u_cap, static_cast<size_t>(m) * b->rp, s);
@@ -2381,14 +2429,7 @@ int mp_linear_requests_grad(mp_ctx* c, const mp_weight* wt, const void* dy, int6
     ext.ld32 = b->rp;
   }
   if (dx != nullptr) {
-    const mp_weight* wl[1] = {wt};
-    void* yl[1] = {dx};
-    const int64_t ll[1] = {lddx};
-    const Stack* sl[1] = {nullptr};
-    const int cl[1] = {0};
-    rc = launch_projections(c, wl, yl, ll, sl, cl, 0, 1, dy, ldy, m, s, nullptr, nullptr, nullptr, true, nullptr,
-                            &ext);
-    if (rc == MP_OK) c->eng.lora_proj += 1;
+    rc = run_requests(c, wt, dy, ldy, dx, lddx, m, &ext, s);
   } else if (da != nullptr) {
     rc = launch_ranks(c, rank_params(c, ext, dy, ldy, n), s);
   }

@@ -216,6 +216,29 @@ struct RankParams {
   uint32_t* err;
 };
 
+// y = x W^T + v B^T of at most kFewRows rows (few_rows_kernel).
+constexpr int kFewRows = 32;
+
+struct FewParams {
+  const uint16_t* x;  // bf16 [m][ldx]
+  int64_t ldx;
+  const uint8_t* w;   // weight rows: codes, or bf16
+  size_t w_pitch;     // bytes
+  const uint32_t* sb; // (scale | bias << 16) per row and group, packed weights
+  int32_t sb_stride;
+  int32_t m, n, k;
+  uint32_t code_xor;  // 0x80808080: signed codes
+  float zero;         // what stands for 0 among the kernel's whole-number codes
+  const float* v;     // f32 [m][ldv], strengths in
+  int64_t ldv;
+  const uint16_t* b;  // bf16 [cap][n][rp]
+  int32_t rp;
+  const int32_t* row_adapter;
+  uint16_t* y;
+  int64_t ldy;
+  int32_t chunks;     // of the rank-space launch right before (0: there was none)
+};
+
 constexpr int kPreTok = 512;  // token rows of a prologue unit (two accumulators, as member tiles)
 
 // Second pass of a split-K launch: out[t, j] = bf16(scale(t, j) * sum_z

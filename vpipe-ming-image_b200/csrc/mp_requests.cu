@@ -269,14 +269,17 @@ __device__ __forceinline__ void load16(const uint16_t* row, int c, int k, bool o
   }
 }
 
-constexpr int kRankWarps = 8;
+constexpr int kRankWarps = 16;
+constexpr int kRankBatch = 4;  // K groups a warp has in flight
 
 // One block: 16 ranks of one chunk (at most 8 rows of one request); its warps
 // take the 64-wide K groups in turn and their sums are added in warp order.
 // Within a group lane (g, j) (g = lane / 4, j = lane % 4) holds columns
 // 16 j .. 16 j + 15 of ranks g and g + 8 and of row g: both operands of the
 // four MMAs of a group then come from two 16-byte loads each, the K columns
-// taken in the same order in both.
+// taken in the same order in both. With few rows a block or two have to fetch
+// the whole factor, so what counts is the bytes each keeps in flight: 16 warps
+// of four groups.
 __global__ void __launch_bounds__(32 * kRankWarps) rank_rows_kernel(const __grid_constant__ RankParams p) {
   __shared__ float part[kRankWarps][16][kChunkRows];
   pdl_wait();
@@ -292,15 +295,20 @@ __global__ void __launch_bounds__(32 * kRankWarps) rank_rows_kernel(const __grid
   const uint16_t* xr = p.x + static_cast<int64_t>(ch.x + min(g, rows - 1)) * p.ldx;
   float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
   const int groups = (p.k + 63) / 64;
-  for (int i = warp; i < groups; i += kRankWarps) {
-    const int c = 64 * i + 16 * j;
-    uint32_t wa[8], wb[8], wx[8];
-    load16(fa, c, p.k, true, wa);
-    load16(fb, c, p.k, true, wb);
-    load16(xr, c, p.k, g < rows, wx);
+  for (int i0 = warp; i0 < groups; i0 += kRankWarps * kRankBatch) {
+    uint32_t wa[kRankBatch][8], wb[kRankBatch][8], wx[kRankBatch][8];
 #pragma unroll
-    for (int s = 0; s < 4; ++s)
-      mma_16x8x16(d, wa[2 * s], wb[2 * s], wa[2 * s + 1], wb[2 * s + 1], wx[2 * s], wx[2 * s + 1]);
+    for (int b = 0; b < kRankBatch; ++b) {
+      const int i = i0 + b * kRankWarps, c = 64 * i + 16 * j;
+      load16(fa, c, p.k, i < groups, wa[b]);
+      load16(fb, c, p.k, i < groups, wb[b]);
+      load16(xr, c, p.k, i < groups && g < rows, wx[b]);
+    }
+#pragma unroll
+    for (int b = 0; b < kRankBatch; ++b)
+#pragma unroll
+      for (int s = 0; s < 4; ++s)
+        mma_16x8x16(d, wa[b][2 * s], wb[b][2 * s], wa[b][2 * s + 1], wb[b][2 * s + 1], wx[b][2 * s], wx[b][2 * s + 1]);
   }
   part[warp][g][2 * j] = d[0];
   part[warp][g][2 * j + 1] = d[1];
@@ -321,6 +329,188 @@ __global__ void __launch_bounds__(32 * kRankWarps) rank_rows_kernel(const __grid
     const int tile = t >> (6 + p.lvl);
     const int64_t at = (static_cast<int64_t>(tile + req) << (6 + p.lvl)) + (t & ((64 << p.lvl) - 1));
     p.vblk[at * p.ldb + r0 + r] = __bfloat16_as_ushort(__float2bfloat16_rn(sum));
+  }
+}
+
+// ---- the whole projection, few rows ------------------------------------------------
+
+constexpr int kFewWarps = 8;
+
+// The 16 weights of one row that a lane holds of a 64-wide K group, as loaded.
+template <int BITS>
+struct FewCodes {
+  static constexpr int kWords = BITS == 0 ? 8 : BITS == 8 ? 4 : 2;
+  uint32_t w[kWords];
+};
+
+template <int BITS>
+__device__ __forceinline__ void few_load(const uint8_t* row, int group, int j, int k, bool ok, FewCodes<BITS>& c) {
+  if constexpr (BITS == 0) {
+    load16(reinterpret_cast<const uint16_t*>(row), 64 * group + 16 * j, k, ok, c.w);
+  } else if constexpr (BITS == 8) {
+    const uint4 v = ok ? ld_global_nc_v4(row + 64 * group + 16 * j) : make_uint4(0, 0, 0, 0);
+    c.w[0] = v.x, c.w[1] = v.y, c.w[2] = v.z, c.w[3] = v.w;
+  } else {
+    const uint2 v = ok ? __ldg(reinterpret_cast<const uint2*>(row + 32 * group + 8 * j)) : make_uint2(0, 0);
+    c.w[0] = v.x, c.w[1] = v.y;
+  }
+}
+
+// Weights 4 s .. 4 s + 3 as two bf16 pairs. Packed codes come out as whole
+// numbers, exact in bf16: w8 as q (0 .. 255), w4 as 128 + q (the code put into
+// the low mantissa bits of 128).
+template <int BITS>
+__device__ __forceinline__ void few_pairs(const FewCodes<BITS>& c, int s, uint32_t code_xor, uint32_t& p0,
+                                          uint32_t& p1) {
+  if constexpr (BITS == 0) {
+    p0 = c.w[2 * s];
+    p1 = c.w[2 * s + 1];
+  } else if constexpr (BITS == 8) {
+    const uint32_t w = c.w[s] ^ code_xor;
+    auto code = [&](uint32_t sel) { return __uint_as_float(__byte_perm(w, 0x4700u, sel)) - 32768.0f; };
+    p0 = pack_bf16x2(code(0x5404u), code(0x5414u));
+    p1 = pack_bf16x2(code(0x5424u), code(0x5434u));
+  } else {
+    const uint32_t v = c.w[s >> 1] >> (16 * (s & 1)), u = v >> 8;
+    p0 = (v & 0xFu) | (v << 12 & 0xF0000u) | 0x43004300u;
+    p1 = (u & 0xFu) | (u << 12 & 0xF0000u) | 0x43004300u;
+  }
+}
+
+// y[t] = W x[t] + B_a v[t] for up to 8 NT rows: bound by reading W once. A
+// block takes 16 features, its warps the 64-wide K groups in turn, lanes as in
+// rank_rows_kernel. Packed weights are not dequantized: a group's MMAs run on
+// the codes, and with the sum of the group's x (one more MMA, against ones)
+//   sum_k W x = scale (sum_k q x - zero sum_k x) + bias sum_k x
+// in f32, exact codes and one scale per group. The kernel starts beside
+// rank_rows_kernel (it reads x and W, which are complete when that one runs) and
+// waits for it before the adapters' part.
+template <int BITS, int NT>
+__global__ void __launch_bounds__(32 * kFewWarps) few_rows_kernel(const __grid_constant__ FewParams p) {
+  constexpr int kBatch = BITS == 0 ? 2 : 4;
+  __shared__ float part[kFewWarps][16][8 * NT + 1];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, j = lane & 3;
+  const int f0 = blockIdx.x * 16;
+  const int na = min(f0 + g, p.n - 1), nb = min(f0 + g + 8, p.n - 1);  // rows past n repeat the last
+  const uint8_t* wa = p.w + static_cast<size_t>(na) * p.w_pitch;
+  const uint8_t* wb = p.w + static_cast<size_t>(nb) * p.w_pitch;
+  const uint32_t* sa = p.sb + static_cast<size_t>(na) * p.sb_stride;
+  const uint32_t* sb = p.sb + static_cast<size_t>(nb) * p.sb_stride;
+  const int groups = (p.k + 63) / 64;
+  constexpr int kStep = kFewWarps * kBatch;
+
+  FewCodes<BITS> ca[2][kBatch], cb[2][kBatch];
+  uint32_t za[2][kBatch], zb[2][kBatch];
+  auto load = [&](int i0, int buf) {
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) {
+      const int i = i0 + b * kFewWarps;
+      const bool ok = i < groups;
+      few_load<BITS>(wa, i, j, p.k, ok, ca[buf][b]);
+      few_load<BITS>(wb, i, j, p.k, ok, cb[buf][b]);
+      if constexpr (BITS != 0) {
+        za[buf][b] = ok ? __ldg(sa + i) : 0u;
+        zb[buf][b] = ok ? __ldg(sb + i) : 0u;
+      }
+    }
+  };
+  load(warp, 0);
+  float y[NT][4];
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[t][e] = 0.0f;
+  const uint32_t ones = 0x3F803F80u;
+  // whole pairs of batches, so that the buffers' indices are constants
+  for (int i0 = warp; i0 < groups; i0 += 2 * kStep) {
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const int ih = i0 + half * kStep;
+      if (ih >= groups) break;
+      load(ih + kStep, half ^ 1);
+#pragma unroll
+      for (int b = 0; b < kBatch; ++b) {
+        const int i = ih + b * kFewWarps;
+        uint32_t x[NT][8];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          const int tok = 8 * t + g;
+          load16(p.x + static_cast<int64_t>(min(tok, p.m - 1)) * p.ldx, 64 * i + 16 * j, p.k, i < groups && tok < p.m,
+                 x[t]);
+        }
+        if constexpr (BITS == 0) {
+#pragma unroll
+          for (int s = 0; s < 4; ++s) {
+            uint32_t a0, a1, b0, b1;
+            few_pairs<BITS>(ca[half][b], s, 0, a0, a1);
+            few_pairs<BITS>(cb[half][b], s, 0, b0, b1);
+#pragma unroll
+            for (int t = 0; t < NT; ++t) mma_16x8x16(y[t], a0, b0, a1, b1, x[t][2 * s], x[t][2 * s + 1]);
+          }
+        } else {
+          float d[NT][4], e[NT][4];
+#pragma unroll
+          for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) d[t][q] = e[t][q] = 0.0f;
+#pragma unroll
+          for (int s = 0; s < 4; ++s) {
+            uint32_t a0, a1, b0, b1;
+            few_pairs<BITS>(ca[half][b], s, p.code_xor, a0, a1);
+            few_pairs<BITS>(cb[half][b], s, p.code_xor, b0, b1);
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+              mma_16x8x16(d[t], a0, b0, a1, b1, x[t][2 * s], x[t][2 * s + 1]);
+              mma_16x8x16(e[t], ones, ones, ones, ones, x[t][2 * s], x[t][2 * s + 1]);
+            }
+          }
+          const float s0 = bf16_bits_to_f32(za[half][b] & 0xFFFFu), o0 = bf16_bits_to_f32(za[half][b] >> 16);
+          const float s1 = bf16_bits_to_f32(zb[half][b] & 0xFFFFu), o1 = bf16_bits_to_f32(zb[half][b] >> 16);
+#pragma unroll
+          for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              y[t][q] = fmaf(q < 2 ? s0 : s1, fmaf(-p.zero, e[t][q], d[t][q]), fmaf(q < 2 ? o0 : o1, e[t][q], y[t][q]));
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    part[warp][g][8 * t + 2 * j] = y[t][0];
+    part[warp][g][8 * t + 2 * j + 1] = y[t][1];
+    part[warp][g + 8][8 * t + 2 * j] = y[t][2];
+    part[warp][g + 8][8 * t + 2 * j + 1] = y[t][3];
+  }
+  __syncthreads();
+  pdl_wait();  // v is complete; y may be written
+  pdl_release();
+  const int f = threadIdx.x & 15;
+  if (f0 + f >= p.n) return;
+  for (int t = threadIdx.x >> 4; t < p.m; t += 32 * kFewWarps / 16) {
+    float sum = part[0][f][t];
+#pragma unroll
+    for (int w = 1; w < kFewWarps; ++w) sum += part[w][f][t];
+    const int a = p.row_adapter[t];
+    if (a >= 0) {
+      const uint16_t* br = p.b + (static_cast<size_t>(a) * p.n + f0 + f) * p.rp;
+      const float* v = p.v + static_cast<int64_t>(t) * p.ldv;
+      float low = 0.0f;
+      for (int r = 0; r < p.rp; r += 8) {
+        const uint4 bw = *reinterpret_cast<const uint4*>(br + r);
+        const float4 v0 = *reinterpret_cast<const float4*>(v + r), v1 = *reinterpret_cast<const float4*>(v + r + 4);
+        low = fmaf(__uint_as_float(bw.x << 16), v0.x, low);
+        low = fmaf(__uint_as_float(bw.x & 0xFFFF0000u), v0.y, low);
+        low = fmaf(__uint_as_float(bw.y << 16), v0.z, low);
+        low = fmaf(__uint_as_float(bw.y & 0xFFFF0000u), v0.w, low);
+        low = fmaf(__uint_as_float(bw.z << 16), v1.x, low);
+        low = fmaf(__uint_as_float(bw.z & 0xFFFF0000u), v1.y, low);
+        low = fmaf(__uint_as_float(bw.w << 16), v1.z, low);
+        low = fmaf(__uint_as_float(bw.w & 0xFFFF0000u), v1.w, low);
+      }
+      sum += low;
+    }
+    p.y[static_cast<int64_t>(t) * p.ldy + f0 + f] = __bfloat16_as_ushort(__float2bfloat16_rn(sum));
   }
 }
 
@@ -361,14 +551,15 @@ __global__ void __launch_bounds__(256) weight_transpose_kernel(const uint8_t* w,
 
 // A launch that may begin its set-up while the one before it on the stream ends.
 template <class P>
-cudaError_t launch_overlapped(void (*kernel)(P), dim3 grid, dim3 block, const P& p, cudaStream_t stream) {
+cudaError_t launch_overlapped(void (*kernel)(P), dim3 grid, dim3 block, const P& p, cudaStream_t stream,
+                              bool overlap = true) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = block;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[0].val.programmaticStreamSerializationAllowed = overlap ? 1 : 0;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, kernel, p);
@@ -390,6 +581,30 @@ cudaError_t launch_rank_rows(const RankParams& p, cudaStream_t stream) {
   const dim3 grid(plan_chunks(p.plan.m, p.plan.n_req), p.rp / 16);
   if (grid.x == 0) return cudaSuccess;  // no request
   return launch_overlapped(rank_rows_kernel, grid, dim3(32 * kRankWarps), p, stream);
+}
+
+namespace {
+
+template <int BITS>
+cudaError_t launch_few(const FewParams& p, cudaStream_t stream) {
+  const dim3 grid((p.n + 15) / 16), block(32 * kFewWarps);
+  // it may start beside rank_rows_kernel, never beside what comes before that
+  const bool over = p.chunks > 0;
+  if (p.m <= 8) return launch_overlapped(few_rows_kernel<BITS, 1>, grid, block, p, stream, over);
+  if (p.m <= 16) return launch_overlapped(few_rows_kernel<BITS, 2>, grid, block, p, stream, over);
+  if (p.m <= 32) return launch_overlapped(few_rows_kernel<BITS, 4>, grid, block, p, stream, over);
+  return cudaErrorInvalidValue;
+}
+
+}  // namespace
+
+cudaError_t launch_few_rows(const FewParams& p, int bits, cudaStream_t stream) {
+  switch (bits) {
+    case 0: return launch_few<0>(p, stream);
+    case 8: return launch_few<8>(p, stream);
+    case 4: return launch_few<4>(p, stream);
+    default: return cudaErrorInvalidValue;
+  }
 }
 
 cudaError_t launch_weight_transpose(const void* w, const uint32_t* sb, int sb_stride, int n, int k, int kp, int bits,

@@ -58,13 +58,16 @@ def _alloc_out(m: int, n: int, device) -> torch.Tensor:
     """bf16 [m, n] output view whose row pitch is rounded up to 8 elements (the
     kernels store rows with TMA, which wants 16-byte row strides)."""
     ld = (n + 7) // 8 * 8
-    return torch.empty((m, ld), dtype=torch.bfloat16, device=device)[:, :n]
+    out = torch.empty((m, ld), dtype=torch.bfloat16, device=device)
+    return out if ld == n else out[:, :n]
 
 
-def _stream_handle(stream) -> C.c_void_p:
+def _stream_handle(stream) -> int:
     if stream is None:
-        stream = torch.cuda.current_stream()
-    return C.c_void_p(stream.cuda_stream)
+        # torch.cuda.current_stream().cuda_stream without building a Stream
+        # object: 0.3 us instead of 5 on the host, of calls that take 10
+        return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
+    return stream.cuda_stream
 
 
 @dataclass
@@ -234,16 +237,29 @@ def _keep_for(stream, *tensors) -> None:
                 t.record_stream(stream)
 
 
-def _rows(name: str, t: torch.Tensor, m: int, k: int, dtype=torch.bfloat16) -> None:
-    if not t.is_cuda or t.dtype != dtype or t.dim() != 2 or tuple(t.shape) != (m, k) or (
-            k > 1 and t.stride(1) != 1):
-        raise ValueError(f"{name} must be {dtype} [{m}, {k}] on the device, its rows contiguous "
-                         f"(got {t.dtype} {tuple(t.shape)}, strides {t.stride()})")
+def _rows(name: str, t: torch.Tensor, m: int, k: int, dtype=torch.bfloat16) -> int:
+    """Checks rows [m, k] on the device; returns their pitch in elements."""
+    if t.dtype is dtype and t.shape == (m, k) and t.is_cuda:
+        if m == 1:  # one row: whatever its stride
+            return (k + 15) // 16 * 16 if k == 1 or t.stride(1) == 1 else _bad_rows(name, t, m, k, dtype)
+        ld, one = t.stride()
+        if one == 1 or k == 1:
+            return ld
+    return _bad_rows(name, t, m, k, dtype)
 
 
-def _pitch(t: torch.Tensor) -> int:
-    """Row pitch in elements; one row may have any stride, so its own length counts."""
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), (t.shape[1] + 15) // 16 * 16)
+def _check_scales(t: torch.Tensor, m: int, k: int) -> None:
+    groups = (k + 127) // 128
+    if not (t.dtype is torch.float32 and t.shape == (m, groups) and t.is_cuda
+            and (m == 1 or t.stride(0) == 1) and (groups == 1 or t.stride(1) == m)):
+        raise ValueError(f"the checkpoint's scales must be f32 [{m}, {groups}] on the device, a "
+                         f"group's rows side by side (got {t.dtype} {tuple(t.shape)}, strides "
+                         f"{t.stride()})")
+
+
+def _bad_rows(name, t, m, k, dtype):
+    raise ValueError(f"{name} must be {dtype} [{m}, {k}] on the device, its rows contiguous "
+                     f"(got {t.dtype} {tuple(t.shape)}, strides {t.stride()}, {t.device})")
 
 
 class Context:
@@ -515,20 +531,23 @@ class Context:
         [m, bank.rank_pad] tensor) returns (y, v), v = s_q x A_a^T, which
         linear_requests_grad takes."""
         m = x.shape[0]
-        _rows("x", x, m, w.k)
+        n, k = w.info.n, w.info.k
+        ldx = _rows("x", x, m, k)
         if out is None:
-            out = _alloc_out(m, w.n, x.device)
-        else:
-            _rows("out", out, m, w.n)
-        v = None
+            out = _alloc_out(m, n, x.device)
+        ldy = _rows("out", out, m, n)
+        v, vp, ldv = None, None, 0
         if ranks is not False and ranks is not None:
             v = ranks
             if ranks is True:
                 v = torch.empty((m, bank.rank_pad), dtype=torch.float32, device=x.device)
-            _rows("ranks", v, m, bank.rank_pad, torch.float32)
-        self._check(self.lib.mp_linear_requests(
-            self.h, w.handle, _ptr(x), _pitch(x), bank.handle, plan.handle, _ptr(out), _pitch(out),
-            _ptr(v), _pitch(v) if v is not None else 0, m, _stream_handle(stream)))
+            ldv = _rows("ranks", v, m, bank.rank_pad, torch.float32)
+            vp = v.data_ptr()
+        rc = self.lib.mp_linear_requests(
+            self.h, w.handle, x.data_ptr(), ldx, bank.handle, plan.handle, out.data_ptr(), ldy, vp,
+            ldv, m, _stream_handle(stream))
+        if rc != MP_OK:
+            self._check(rc)
         return out if v is None else (out, v)
 
     def transposed(self, w: Weight, stream=None) -> Weight:
@@ -545,59 +564,66 @@ class Context:
         da f32 [capacity, max_rank, k], db f32 [capacity, n, max_rank]), None
         for what is not needed; capacity is the plan's. wt: transposed(w); x:
         bf16 [m, k] or its Checkpoint; v: the forward call's ranks."""
-        m, n, k = dy.shape[0], wt.k, wt.n
-        _rows("dy", dy, m, n)
-        dx = da = db = xt = xq = xs = None
+        m, n, k = dy.shape[0], wt.info.k, wt.info.n
+        ldy = _rows("dy", dy, m, n)
+        dx = da = db = None
+        dxp = dap = dbp = xp = qp = sp = vp = None
+        lddx = ldx = ldq = ldv = 0
         if need_dx:
             dx = _alloc_out(m, k, dy.device)
+            lddx = _rows("dx", dx, m, k)
+            dxp = dx.data_ptr()
         if need_factors:
             if isinstance(x, Checkpoint):
-                xq, xs = x.codes, x.scales
-                _rows("x.codes", xq, m, k, torch.int8)
-                if xs.shape != (m, (k + 127) // 128) or xs.stride(0) != 1 or (
-                        xs.shape[1] > 1 and xs.stride(1) != m):
-                    raise ValueError("x.scales must be f32 [m, groups], a row of the batch apart "
-                                     "along the groups")
+                ldq = _rows("x.codes", x.codes, m, k, torch.int8)
+                _check_scales(x.scales, m, k)
+                qp, sp = x.codes.data_ptr(), x.scales.data_ptr()
             else:
-                xt = x
-                _rows("x", xt, m, k)
+                ldx = _rows("x", x, m, k)
+                xp = x.data_ptr()
             if v.dim() != 2 or v.shape[1] < bank.max_rank:
                 raise ValueError(f"v must have at least {bank.max_rank} columns")
-            _rows("v", v, m, v.shape[1], torch.float32)
+            ldv = _rows("v", v, m, v.shape[1], torch.float32)
+            vp = v.data_ptr()
             da = torch.empty((plan.capacity, bank.max_rank, k), dtype=torch.float32,
                              device=dy.device)
             db = torch.empty((plan.capacity, n, bank.max_rank), dtype=torch.float32,
                              device=dy.device)
-        self._check(self.lib.mp_linear_requests_grad(
-            self.h, wt.handle, _ptr(dy), _pitch(dy), _ptr(xt), _pitch(xt) if xt is not None else 0,
-            _ptr(xq), _pitch(xq) if xq is not None else 0, _ptr(xs),
-            _ptr(v) if need_factors else None, _pitch(v) if need_factors else 0, bank.handle,
-            plan.handle, _ptr(dx), _pitch(dx) if dx is not None else 0, _ptr(da), _ptr(db), m,
-            _stream_handle(stream)))
+            dap, dbp = da.data_ptr(), db.data_ptr()
+        rc = self.lib.mp_linear_requests_grad(
+            self.h, wt.handle, dy.data_ptr(), ldy, xp, ldx, qp, ldq, sp, vp, ldv, bank.handle,
+            plan.handle, dxp, lddx, dap, dbp, m, _stream_handle(stream))
+        if rc != MP_OK:
+            self._check(rc)
         return dx, da, db
 
     # -- activation checkpoints --------------------------------------------------
     def checkpoint(self, x: torch.Tensor, stream=None) -> Checkpoint:
         """bf16 rows [m, k] in 8 bits, a scale for every 128 features of a row."""
         m, k = x.shape
-        _rows("x", x, m, k)
-        q = torch.empty((m, (k + 15) // 16 * 16), dtype=torch.int8, device=x.device)
+        ldx = _rows("x", x, m, k)
+        ldq = (k + 15) // 16 * 16
+        q = torch.empty((m, ldq), dtype=torch.int8, device=x.device)
         scale = torch.empty(((k + 127) // 128, m), dtype=torch.float32, device=x.device)
-        self._check(self.lib.mp_checkpoint(self.h, _ptr(x), _pitch(x), m, k, _ptr(q), q.stride(0),
-                                           _ptr(scale), _stream_handle(stream)))
-        return Checkpoint(q[:, :k], scale.t())
+        rc = self.lib.mp_checkpoint(self.h, x.data_ptr(), ldx, m, k, q.data_ptr(), ldq,
+                                    scale.data_ptr(), _stream_handle(stream))
+        if rc != MP_OK:
+            self._check(rc)
+        return Checkpoint(q if ldq == k else q[:, :k], scale.t())
 
     def restore(self, saved: Checkpoint, out: torch.Tensor | None = None,
                 stream=None) -> torch.Tensor:
         """The bf16 rows a checkpoint stands for."""
-        m, k = saved.shape
+        m, k = saved.codes.shape
+        ldq = _rows("codes", saved.codes, m, k, torch.int8)
+        _check_scales(saved.scales, m, k)
         if out is None:
             out = _alloc_out(m, k, saved.codes.device)
-        else:
-            _rows("out", out, m, k)
-        self._check(self.lib.mp_restore(self.h, _ptr(saved.codes), _pitch(saved.codes),
-                                        _ptr(saved.scales), m, k, _ptr(out), _pitch(out),
-                                        _stream_handle(stream)))
+        ldx = _rows("out", out, m, k)
+        rc = self.lib.mp_restore(self.h, saved.codes.data_ptr(), ldq, saved.scales.data_ptr(), m, k,
+                                 out.data_ptr(), ldx, _stream_handle(stream))
+        if rc != MP_OK:
+            self._check(rc)
         return out
 
     # -- modulation ----------------------------------------------------------
