@@ -24,15 +24,6 @@ constexpr int kCkThreads = 256;
 constexpr int kPerLane = 8;                         // features of a lane
 constexpr int kGroupLanes = kCkGroup / kPerLane;    // 16
 
-__device__ __forceinline__ void unpack8(const uint4& v, float (&f)[8]) {
-  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    f[2 * i] = __uint_as_float(w[i] << 16);
-    f[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
-  }
-}
-
 constexpr int kCkRows = 4;
 
 // Block (x, y): rows [4 x, 4 x + 4), groups [16 y, 16 y + 16), one per half-warp.
@@ -60,28 +51,33 @@ __global__ void __launch_bounds__(kCkThreads) checkpoint_kernel(const __grid_con
   }
 #pragma unroll
   for (int r = 0; r < kCkRows; ++r) {
-    float f[8];
-    unpack8(raw[r], f);
-    float top = 0.0f;
-    bool finite = true;
+    // max|x| on the bf16 patterns, two at a time: without the sign they order
+    // like the values, infinities and NaNs last
+    const uint32_t v[4] = {raw[r].x, raw[r].y, raw[r].z, raw[r].w};
+    uint32_t top2 = __vmaxu2(__vmaxu2(v[0] & 0x7FFF7FFFu, v[1] & 0x7FFF7FFFu),
+                             __vmaxu2(v[2] & 0x7FFF7FFFu, v[3] & 0x7FFF7FFFu));
 #pragma unroll
-    for (int i = 0; i < kPerLane; ++i) {
-      top = fmaxf(top, fabsf(f[i]));
-      finite = finite && fabsf(f[i]) <= 3.3895314e38f;  // false for NaN
-    }
-    if (!finite) top = __int_as_float(0x7F800000);  // fmaxf drops a NaN
-#pragma unroll
-    for (int d = 1; d < kGroupLanes; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
-    finite = top <= 3.3895314e38f;
+    for (int d = 1; d < kGroupLanes; d <<= 1) top2 = __vmaxu2(top2, __shfl_xor_sync(0xFFFFFFFFu, top2, d));
+    const uint32_t top_bits = max(top2 & 0xFFFFu, top2 >> 16);
+    const float top = bf16_bits_to_f32(top_bits);
+    const bool finite = top_bits < 0x7F80u;
     if (c >= p.k || row0 + r >= p.m) continue;
     const bool live = finite && top >= kCkTiny;
     const float inv = live ? __fmul_rn(127.0f, __frcp_rn(top)) : 0.0f;
-    uint32_t w[2] = {0, 0};
+    // x inv, then the nearest whole number (ties to even) in the low mantissa
+    // bits of 1.5 2^23; |x| inv <= 127 (1 + 2^-24)^3 rounds to 127 at most. The
+    // two roundings are the definition's, so never one FMA (packed f32x2 products
+    // and sums were joined into one: a code in 1400 moved).
+    auto code = [&](uint32_t pattern) {
+      return __float_as_uint(__fadd_rn(__fmul_rn(__uint_as_float(pattern), inv), 12582912.0f));
+    };
+    uint32_t w[2];
 #pragma unroll
-    for (int i = 0; i < kPerLane; ++i) {
-      // |x| inv <= 127 (1 + 2^-24)^3: rounds to 127 at most
-      const int q = live ? __float2int_rn(__fmul_rn(f[i], inv)) : 0;
-      w[i >> 2] |= (static_cast<uint32_t>(q) & 0xFFu) << (8 * (i & 3));
+    for (int h = 0; h < 2; ++h) {
+      const uint32_t a = v[2 * h], b = v[2 * h + 1];
+      const uint32_t lo = __byte_perm(code(a << 16), code(a & 0xFFFF0000u), 0x0040);
+      const uint32_t hi = __byte_perm(code(b << 16), code(b & 0xFFFF0000u), 0x0040);
+      w[h] = live ? __byte_perm(lo, hi, 0x5410) : 0u;
     }
     int8_t* out = p.q + static_cast<int64_t>(row0 + r) * p.ldq + c;  // the pitch is a multiple of 16
     *reinterpret_cast<uint2*>(out) = make_uint2(w[0], w[1]);

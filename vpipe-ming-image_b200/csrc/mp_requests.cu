@@ -246,6 +246,15 @@ __device__ __forceinline__ void mma_16x8x16(float (&d)[4], uint32_t a0, uint32_t
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+// D = A B (no accumulator to start from).
+__device__ __forceinline__ void mma_16x8x16_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                                  uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+}
+
 // 16 bf16 values of a row from column c (a multiple of 16; the row is 16-byte
 // aligned), zeros from column k on and where !ok: nothing past the k-th value
 // is read.
@@ -356,70 +365,98 @@ __device__ __forceinline__ void few_load(const uint8_t* row, int group, int j, i
   }
 }
 
-// Weights 4 s .. 4 s + 3 as two bf16 pairs. Packed codes come out as whole
-// numbers, exact in bf16: w8 as q (0 .. 255), w4 as 128 + q (the code put into
-// the low mantissa bits of 128).
+// The lane's 16 weights as eight bf16 pairs, in MMA order: pairs 2 s and 2 s + 1
+// are K step s. Packed codes come out as whole numbers, exact in bf16: w8 as q
+// (0 .. 255) in order; w4 as 128 + q, the code put into the low mantissa bits of
+// 128, two at a time where they lie 16 bits apart: pair i of a word is (i, i + 4).
 template <int BITS>
-__device__ __forceinline__ void few_pairs(const FewCodes<BITS>& c, int s, uint32_t code_xor, uint32_t& p0,
-                                          uint32_t& p1) {
+__device__ __forceinline__ void few_pairs(const FewCodes<BITS>& c, uint32_t code_xor, uint32_t (&p)[8]) {
   if constexpr (BITS == 0) {
-    p0 = c.w[2 * s];
-    p1 = c.w[2 * s + 1];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) p[i] = c.w[i];
   } else if constexpr (BITS == 8) {
-    const uint32_t w = c.w[s] ^ code_xor;
-    auto code = [&](uint32_t sel) { return __uint_as_float(__byte_perm(w, 0x4700u, sel)) - 32768.0f; };
-    p0 = pack_bf16x2(code(0x5404u), code(0x5414u));
-    p1 = pack_bf16x2(code(0x5424u), code(0x5434u));
+    const uint64_t less = f32x2(-32768.0f, -32768.0f);
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      const uint32_t w = c.w[s] ^ code_xor;
+      auto code = [&](uint32_t sel) { return __uint_as_float(__byte_perm(w, 0x4700u, sel)); };  // 32768 + q
+      p[2 * s] = f32x2_to_bf16x2(add_f32x2(f32x2(code(0x5404u), code(0x5414u)), less));
+      p[2 * s + 1] = f32x2_to_bf16x2(add_f32x2(f32x2(code(0x5424u), code(0x5434u)), less));
+    }
   } else {
-    const uint32_t v = c.w[s >> 1] >> (16 * (s & 1)), u = v >> 8;
-    p0 = (v & 0xFu) | (v << 12 & 0xF0000u) | 0x43004300u;
-    p1 = (u & 0xFu) | (u << 12 & 0xF0000u) | 0x43004300u;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) p[i] = (c.w[i >> 2] >> (4 * (i & 3)) & 0x000F000Fu) | 0x43004300u;
+  }
+}
+
+// The lane's 16 values of x in the same order.
+template <int BITS>
+__device__ __forceinline__ void few_x(const uint16_t* row, int group, int j, int k, uint32_t (&x)[8]) {
+  if constexpr (BITS == 0) {
+    load16(row, 64 * group + 16 * j, k, true, x);
+  } else {
+    const uint4* at = reinterpret_cast<const uint4*>(row + 64 * group + 16 * j);
+    const uint4 a = __ldg(at), b = __ldg(at + 1);
+    if constexpr (BITS == 8) {
+      x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w;
+      x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+    } else {
+      x[0] = __byte_perm(a.x, a.z, 0x5410), x[1] = __byte_perm(a.x, a.z, 0x7632);
+      x[2] = __byte_perm(a.y, a.w, 0x5410), x[3] = __byte_perm(a.y, a.w, 0x7632);
+      x[4] = __byte_perm(b.x, b.z, 0x5410), x[5] = __byte_perm(b.x, b.z, 0x7632);
+      x[6] = __byte_perm(b.y, b.w, 0x5410), x[7] = __byte_perm(b.y, b.w, 0x7632);
+    }
   }
 }
 
 // y[t] = W x[t] + B_a v[t] for up to 8 NT rows: bound by reading W once. A
-// block takes 16 features, its warps the 64-wide K groups in turn, lanes as in
+// block takes 16 MT features, its warps the 64-wide K groups in turn, lanes as in
 // rank_rows_kernel. Packed weights are not dequantized: a group's MMAs run on
 // the codes, and with the sum of the group's x (one more MMA, against ones)
 //   sum_k W x = scale (sum_k q x - zero sum_k x) + bias sum_k x
 // in f32, exact codes and one scale per group. The kernel starts beside
 // rank_rows_kernel (it reads x and W, which are complete when that one runs) and
-// waits for it before the adapters' part.
-template <int BITS, int NT>
-__global__ void __launch_bounds__(32 * kFewWarps) few_rows_kernel(const __grid_constant__ FewParams p) {
-  constexpr int kBatch = BITS == 0 ? 2 : 4;
-  __shared__ float part[kFewWarps][16][8 * NT + 1];
+// waits for it before the adapters' part. Rows past m repeat the last one: the
+// MMA's columns are independent, theirs are not stored.
+template <int BITS, int MT, int NT>
+__global__ void __launch_bounds__(32 * kFewWarps, NT <= 2 ? 2 : 1)
+    few_rows_kernel(const __grid_constant__ FewParams p) {
+  constexpr int kBatch = (BITS == 0 ? 2 : 4) / MT;  // K groups a warp has in flight, twice
+  constexpr int kFeat = 16 * MT;
+  __shared__ float part[kFewWarps][kFeat][8 * NT + 1];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, j = lane & 3;
-  const int f0 = blockIdx.x * 16;
-  const int na = min(f0 + g, p.n - 1), nb = min(f0 + g + 8, p.n - 1);  // rows past n repeat the last
-  const uint8_t* wa = p.w + static_cast<size_t>(na) * p.w_pitch;
-  const uint8_t* wb = p.w + static_cast<size_t>(nb) * p.w_pitch;
-  const uint32_t* sa = p.sb + static_cast<size_t>(na) * p.sb_stride;
-  const uint32_t* sb = p.sb + static_cast<size_t>(nb) * p.sb_stride;
+  const int f0 = blockIdx.x * kFeat;
+  const uint8_t* wrow[2 * MT];
+  const uint32_t* srow[2 * MT];
+#pragma unroll
+  for (int h = 0; h < 2 * MT; ++h) {
+    const int n = min(f0 + 8 * h + g, p.n - 1);  // rows past n repeat the last
+    wrow[h] = p.w + static_cast<size_t>(n) * p.w_pitch;
+    srow[h] = p.sb + static_cast<size_t>(n) * p.sb_stride;
+  }
+  const uint16_t* xrow[NT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) xrow[t] = p.x + static_cast<int64_t>(min(8 * t + g, p.m - 1)) * p.ldx;
   const int groups = (p.k + 63) / 64;
   constexpr int kStep = kFewWarps * kBatch;
 
-  FewCodes<BITS> ca[2][kBatch], cb[2][kBatch];
-  uint32_t za[2][kBatch], zb[2][kBatch];
+  FewCodes<BITS> codes[2][kBatch][2 * MT];
+  uint32_t sb[2][kBatch][2 * MT];
   auto load = [&](int i0, int buf) {
 #pragma unroll
     for (int b = 0; b < kBatch; ++b) {
       const int i = i0 + b * kFewWarps;
-      const bool ok = i < groups;
-      few_load<BITS>(wa, i, j, p.k, ok, ca[buf][b]);
-      few_load<BITS>(wb, i, j, p.k, ok, cb[buf][b]);
-      if constexpr (BITS != 0) {
-        za[buf][b] = ok ? __ldg(sa + i) : 0u;
-        zb[buf][b] = ok ? __ldg(sb + i) : 0u;
+#pragma unroll
+      for (int h = 0; h < 2 * MT; ++h) {
+        few_load<BITS>(wrow[h], i, j, p.k, i < groups, codes[buf][b][h]);
+        if constexpr (BITS != 0) sb[buf][b][h] = i < groups ? __ldg(srow[h] + i) : 0u;
       }
     }
   };
   load(warp, 0);
-  float y[NT][4];
+  float y[MT][NT][4];
 #pragma unroll
-  for (int t = 0; t < NT; ++t)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) y[t][e] = 0.0f;
+  for (int e = 0; e < MT * NT * 4; ++e) y[e / (4 * NT)][e / 4 % NT][e % 4] = 0.0f;
   const uint32_t ones = 0x3F803F80u;
   // whole pairs of batches, so that the buffers' indices are constants
   for (int i0 = warp; i0 < groups; i0 += 2 * kStep) {
@@ -431,63 +468,63 @@ __global__ void __launch_bounds__(32 * kFewWarps) few_rows_kernel(const __grid_c
 #pragma unroll
       for (int b = 0; b < kBatch; ++b) {
         const int i = ih + b * kFewWarps;
+        if (i >= groups) break;
         uint32_t x[NT][8];
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          const int tok = 8 * t + g;
-          load16(p.x + static_cast<int64_t>(min(tok, p.m - 1)) * p.ldx, 64 * i + 16 * j, p.k, i < groups && tok < p.m,
-                 x[t]);
-        }
-        if constexpr (BITS == 0) {
+        for (int t = 0; t < NT; ++t) few_x<BITS>(xrow[t], i, j, p.k, x[t]);
+        float sum[NT][4];  // of the group's x: a column each, the same in every row
+        if constexpr (BITS != 0) {
 #pragma unroll
-          for (int s = 0; s < 4; ++s) {
-            uint32_t a0, a1, b0, b1;
-            few_pairs<BITS>(ca[half][b], s, 0, a0, a1);
-            few_pairs<BITS>(cb[half][b], s, 0, b0, b1);
+          for (int t = 0; t < NT; ++t) {
+            mma_16x8x16_first(sum[t], ones, ones, ones, ones, x[t][0], x[t][1]);
 #pragma unroll
-            for (int t = 0; t < NT; ++t) mma_16x8x16(y[t], a0, b0, a1, b1, x[t][2 * s], x[t][2 * s + 1]);
+            for (int s = 1; s < 4; ++s) mma_16x8x16(sum[t], ones, ones, ones, ones, x[t][2 * s], x[t][2 * s + 1]);
           }
-        } else {
-          float d[NT][4], e[NT][4];
+        }
 #pragma unroll
-          for (int t = 0; t < NT; ++t)
+        for (int m = 0; m < MT; ++m) {
+          uint32_t lo[8], hi[8];
+          few_pairs<BITS>(codes[half][b][2 * m], p.code_xor, lo);
+          few_pairs<BITS>(codes[half][b][2 * m + 1], p.code_xor, hi);
+          if constexpr (BITS == 0) {
 #pragma unroll
-            for (int q = 0; q < 4; ++q) d[t][q] = e[t][q] = 0.0f;
+            for (int t = 0; t < NT; ++t)
 #pragma unroll
-          for (int s = 0; s < 4; ++s) {
-            uint32_t a0, a1, b0, b1;
-            few_pairs<BITS>(ca[half][b], s, p.code_xor, a0, a1);
-            few_pairs<BITS>(cb[half][b], s, p.code_xor, b0, b1);
+              for (int s = 0; s < 4; ++s)
+                mma_16x8x16(y[m][t], lo[2 * s], hi[2 * s], lo[2 * s + 1], hi[2 * s + 1], x[t][2 * s], x[t][2 * s + 1]);
+          } else {
+            const uint32_t z0 = sb[half][b][2 * m], z1 = sb[half][b][2 * m + 1];
+            const float s0 = bf16_bits_to_f32(z0 & 0xFFFFu), o0 = bf16_bits_to_f32(z0 >> 16);
+            const float s1 = bf16_bits_to_f32(z1 & 0xFFFFu), o1 = bf16_bits_to_f32(z1 >> 16);
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
-              mma_16x8x16(d[t], a0, b0, a1, b1, x[t][2 * s], x[t][2 * s + 1]);
-              mma_16x8x16(e[t], ones, ones, ones, ones, x[t][2 * s], x[t][2 * s + 1]);
+              float d[4];
+              mma_16x8x16_first(d, lo[0], hi[0], lo[1], hi[1], x[t][0], x[t][1]);
+#pragma unroll
+              for (int s = 1; s < 4; ++s)
+                mma_16x8x16(d, lo[2 * s], hi[2 * s], lo[2 * s + 1], hi[2 * s + 1], x[t][2 * s], x[t][2 * s + 1]);
+#pragma unroll
+              for (int q = 0; q < 4; ++q)
+                y[m][t][q] = fmaf(q < 2 ? s0 : s1, fmaf(-p.zero, sum[t][q], d[q]),
+                                  fmaf(q < 2 ? o0 : o1, sum[t][q], y[m][t][q]));
             }
           }
-          const float s0 = bf16_bits_to_f32(za[half][b] & 0xFFFFu), o0 = bf16_bits_to_f32(za[half][b] >> 16);
-          const float s1 = bf16_bits_to_f32(zb[half][b] & 0xFFFFu), o1 = bf16_bits_to_f32(zb[half][b] >> 16);
-#pragma unroll
-          for (int t = 0; t < NT; ++t)
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-              y[t][q] = fmaf(q < 2 ? s0 : s1, fmaf(-p.zero, e[t][q], d[t][q]), fmaf(q < 2 ? o0 : o1, e[t][q], y[t][q]));
         }
       }
     }
   }
 #pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    part[warp][g][8 * t + 2 * j] = y[t][0];
-    part[warp][g][8 * t + 2 * j + 1] = y[t][1];
-    part[warp][g + 8][8 * t + 2 * j] = y[t][2];
-    part[warp][g + 8][8 * t + 2 * j + 1] = y[t][3];
-  }
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) part[warp][16 * m + g + 8 * (q >> 1)][8 * t + 2 * j + (q & 1)] = y[m][t][q];
   __syncthreads();
   pdl_wait();  // v is complete; y may be written
   pdl_release();
-  const int f = threadIdx.x & 15;
+  const int f = threadIdx.x % kFeat;
   if (f0 + f >= p.n) return;
-  for (int t = threadIdx.x >> 4; t < p.m; t += 32 * kFewWarps / 16) {
+  for (int t = threadIdx.x / kFeat; t < p.m; t += 32 * kFewWarps / kFeat) {
     float sum = part[0][f][t];
 #pragma unroll
     for (int w = 1; w < kFewWarps; ++w) sum += part[w][f][t];
@@ -585,15 +622,24 @@ cudaError_t launch_rank_rows(const RankParams& p, cudaStream_t stream) {
 
 namespace {
 
-template <int BITS>
+template <int BITS, int MT>
 cudaError_t launch_few(const FewParams& p, cudaStream_t stream) {
-  const dim3 grid((p.n + 15) / 16), block(32 * kFewWarps);
+  const dim3 grid((p.n + 16 * MT - 1) / (16 * MT)), block(32 * kFewWarps);
   // it may start beside rank_rows_kernel, never beside what comes before that
   const bool over = p.chunks > 0;
-  if (p.m <= 8) return launch_overlapped(few_rows_kernel<BITS, 1>, grid, block, p, stream, over);
-  if (p.m <= 16) return launch_overlapped(few_rows_kernel<BITS, 2>, grid, block, p, stream, over);
-  if (p.m <= 32) return launch_overlapped(few_rows_kernel<BITS, 4>, grid, block, p, stream, over);
+  if (p.m <= 8) return launch_overlapped(few_rows_kernel<BITS, MT, 1>, grid, block, p, stream, over);
+  if (p.m <= 16) return launch_overlapped(few_rows_kernel<BITS, MT, 2>, grid, block, p, stream, over);
+  if constexpr (MT == 1) {
+    if (p.m <= 32) return launch_overlapped(few_rows_kernel<BITS, MT, 4>, grid, block, p, stream, over);
+  }
   return cudaErrorInvalidValue;
+}
+
+// 32 features a block halve the reads of x and the sums of it; 16 while 32 would
+// leave SMs without a block.
+template <int BITS>
+cudaError_t launch_few(const FewParams& p, cudaStream_t stream) {
+  return p.n >= 32 * 2 * 148 && p.m <= 16 ? launch_few<BITS, 2>(p, stream) : launch_few<BITS, 1>(p, stream);
 }
 
 }  // namespace
