@@ -32,6 +32,7 @@ cudaError_t launch_attention(const AttnParams& p, cudaStream_t stream);
 cudaError_t launch_plan_requests(const PlanParams& p, cudaStream_t stream);
 cudaError_t launch_bank_set(const BankSetParams& p, cudaStream_t stream);
 cudaError_t launch_rank_rows(const RankParams& p, cudaStream_t stream);
+cudaError_t launch_rank_tiles(const RankParams& p, cudaStream_t stream);
 cudaError_t launch_few_rows(const FewParams& p, int bits, cudaStream_t stream);
 cudaError_t launch_adapter_grad(const GradParams& p, cudaStream_t stream);
 cudaError_t launch_checkpoint(const CheckpointParams& p, cudaStream_t stream);
@@ -119,6 +120,8 @@ struct mp_adapters {
   int32_t* bad = nullptr;  // [cap]: a factor held a value that is not finite
   CUtensorMap tm_b;        // [cap * n, rp], box {64, 128}, SW128
   CUtensorMap tm_at;       // [cap * k, rp]
+  CUtensorMap tm_a;        // [cap * rp, k], box {64, rp}, SW128
+  CUtensorMap tm_bt;       // [cap * rp, n]
 };
 
 struct mp_requests {
@@ -742,6 +745,7 @@ struct RequestsLaunch {
   const mp_adapters* bank = nullptr;
   const uint16_t* f = nullptr;  // rank-space factor [cap][rp][fp]
   int fp = 0;
+  const CUtensorMap* tm_f = nullptr;
   const uint16_t* b = nullptr;  // the other factor [cap][n][rp]
   const CUtensorMap* tm_b = nullptr;
   float* v32 = nullptr;         // also kept in f32 (nullable)
@@ -2012,16 +2016,6 @@ extern "C" int mp_linear_lora_static(mp_ctx* c, const mp_weight* w, const void* 
 
 namespace {
 
-// The rank-space rows of a batch of requests: v = s_q (x F_q^T), into `p`'s
-// outputs.
-int launch_ranks(mp_ctx* c, const mp::RankParams& p, cudaStream_t stream) {
-  cudaError_t e = mp::launch_rank_rows(p, stream);
-  if (e != cudaSuccess) return cuda_fail(c, e, "rank_rows_kernel");
-  c->eng.kernels += 1;
-  c->eng.lora_down += 1;
-  return MP_OK;
-}
-
 mp::RankParams rank_params(const mp_ctx* c, const RequestsLaunch& ext, const void* x, int64_t ldx, int k) {
   mp::RankParams r;
   std::memset(&r, 0, sizeof(r));
@@ -2035,9 +2029,36 @@ mp::RankParams rank_params(const mp_ctx* c, const RequestsLaunch& ext, const voi
   r.plan = ext.req->plan;
   r.v32 = ext.v32;
   r.ld32 = ext.ld32;
+  r.lvl = 1;  // 128-row tiles, where no blocks are asked for
   r.wait_limit_ns = c->wait_limit_ns;
   r.err = c->err_word;
   return r;
+}
+
+// The rank-space rows of a batch of requests: v = s_q (x F_q^T), into `r`'s
+// outputs. Requests of 16 rows and more on average go to the tensor core in
+// tiles of 128 rows, shorter ones in runs of 8 rows.
+int launch_ranks(mp_ctx* c, const RequestsLaunch& ext, mp::RankParams* r, cudaStream_t stream) {
+  const mp::RequestPlan& pl = r->plan;
+  const bool tiles = pl.m > mp::kFewRows && pl.m >= 16 * static_cast<int64_t>(pl.n_req);
+  cudaError_t e;
+  if (tiles) {
+    if (!encode_2d(&r->tm_x, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, r->x, r->k, pl.m, static_cast<uint64_t>(r->ldx) * 2, 64,
+                   128, CU_TENSOR_MAP_SWIZZLE_128B))
+      return fail(c, MP_ECUDA, "tensor map encode failed (rank-space rows)");
+    r->tm_f = *ext.tm_f;
+    e = mp::launch_rank_tiles(*r, stream);
+  } else {
+    if (r->vblk != nullptr) {
+      const size_t rows = static_cast<size_t>(mp::plan_blocks(pl.m, pl.n_req, r->lvl)) << (6 + r->lvl);
+      MP_CUDA(c, cudaMemsetAsync(r->vblk, 0, rows * r->ldb * sizeof(uint16_t), stream));
+    }
+    e = mp::launch_rank_rows(*r, stream);
+  }
+  if (e != cudaSuccess) return cuda_fail(c, e, tiles ? "rank_tiles_kernel" : "rank_rows_kernel");
+  c->eng.kernels += 1;
+  c->eng.lora_down += 1;
+  return MP_OK;
 }
 
 // Member 0 of the launch `p` takes its appended K tiles from the plan's lists:
@@ -2056,8 +2077,7 @@ int launch_request_ranks(mp_ctx* c, ProjParams* p, const RequestsLaunch& ext, co
   r.vblk = c->req_blk;
   r.lvl = level;
   r.ldb = ldb;
-  MP_CUDA(c, cudaMemsetAsync(c->req_blk, 0, rows * ldb * sizeof(uint16_t), stream));
-  rc = launch_ranks(c, r, stream);
+  rc = launch_ranks(c, ext, &r, stream);
   if (rc != MP_OK) return rc;
   mp::ProjMember& mb = p->mem[0];
   if (!encode_2d(&mb.tm_t, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, c->req_blk, ldb, rows,
@@ -2082,7 +2102,8 @@ int run_requests(mp_ctx* c, const mp_weight* w, const void* x, int64_t ldx, void
       ext->v32 = c->req_u;
       ext->ld32 = ext->bank->rp;
     }
-    int rc = launch_ranks(c, rank_params(c, *ext, x, ldx, w->d.k), stream);
+    mp::RankParams r = rank_params(c, *ext, x, ldx, w->d.k);
+    int rc = launch_ranks(c, *ext, &r, stream);
     if (rc != MP_OK) return rc;
     mp::FewParams p;
     p.x = static_cast<const uint16_t*>(x);
@@ -2192,7 +2213,11 @@ int mp_adapters_create(mp_ctx* c, int n, int k, int capacity, int max_rank, int 
   if (!encode_2d(&b->tm_b, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, b->b, b->rp, cap * n, pitch, 64, 128,
                  CU_TENSOR_MAP_SWIZZLE_128B) ||
       (training && !encode_2d(&b->tm_at, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, b->at, b->rp, cap * k, pitch, 64, 128,
-                              CU_TENSOR_MAP_SWIZZLE_128B)))
+                              CU_TENSOR_MAP_SWIZZLE_128B)) ||
+      !encode_2d(&b->tm_a, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, b->a, k, cap * b->rp, static_cast<uint64_t>(b->kp) * 2,
+                 64, b->rp, CU_TENSOR_MAP_SWIZZLE_128B) ||
+      (training && !encode_2d(&b->tm_bt, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, b->bt, n, cap * b->rp,
+                              static_cast<uint64_t>(b->np) * 2, 64, b->rp, CU_TENSOR_MAP_SWIZZLE_128B)))
     return cleanup(fail(c, MP_ECUDA, "tensor map encode failed (adapters)"));
   *out = b;
   return MP_OK;
@@ -2350,6 +2375,7 @@ int mp_linear_requests(mp_ctx* c, const mp_weight* w, const void* x, int64_t ldx
   ext.bank = b;
   ext.f = b->a;
   ext.fp = b->kp;
+  ext.tm_f = &b->tm_a;
   ext.b = b->b;
   ext.tm_b = &b->tm_b;
   ext.v32 = ranks;
@@ -2420,6 +2446,7 @@ int mp_linear_requests_grad(mp_ctx* c, const mp_weight* wt, const void* dy, int6
   ext.bank = b;
   ext.f = b->bt;
   ext.fp = b->np;
+  ext.tm_f = &b->tm_bt;
   ext.b = b->at;
   ext.tm_b = &b->tm_at;
   if (da != nullptr) {
@@ -2431,7 +2458,8 @@ int mp_linear_requests_grad(mp_ctx* c, const mp_weight* wt, const void* dy, int6
   if (dx != nullptr) {
     rc = run_requests(c, wt, dy, ldy, dx, lddx, m, &ext, s);
   } else if (da != nullptr) {
-    rc = launch_ranks(c, rank_params(c, ext, dy, ldy, n), s);
+    mp::RankParams rk = rank_params(c, ext, dy, ldy, n);
+    rc = launch_ranks(c, ext, &rk, s);
   }
   if (rc != MP_OK) return rc;
   mp::GradParams g;

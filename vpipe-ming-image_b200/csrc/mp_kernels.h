@@ -201,6 +201,9 @@ struct BankSetParams {
 
 // Rank-space rows of a batch of requests: v = s_q (x F_q^T), F_q [rp][k].
 struct RankParams {
+  CUtensorMap tm_x;   // x (box {64, 128}, SW128), rank_tiles_kernel only
+  CUtensorMap tm_f;   // F as [cap * rp, k] (box {64, rp}, SW128)
+  int32_t splits;     // CTAs that share K (set by the launch)
   const uint16_t* x;  // bf16 [m][ldx]
   int64_t ldx;
   const uint16_t* f;  // bf16 [cap][rp][fp]

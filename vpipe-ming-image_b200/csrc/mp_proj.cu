@@ -378,6 +378,10 @@ __device__ void pair_producer(const ProjParams& p, const PairSmem& sm, bool lead
     const uint32_t sub_bytes = static_cast<uint32_t>(t.half) * 128u;  // one sub-tile, one CTA
     const uint32_t xbytes_pair = 2u * static_cast<uint32_t>(t.n_sub) * sub_bytes;
     const uint32_t codes_bytes = static_cast<uint32_t>(kBlockN * kBlockK * mb.bits / 8);
+    // adapters by request: the next list entry, loaded one entry ahead
+    const bool ext = p.ext_first != nullptr && t.kt_end > base_kt;
+    int2 ext_next = ext ? p.ext_list[t.ext0] : make_int2(0, 0);
+    int2 ext_now = ext_next;
     for (int kt = t.kt_begin; kt < t.kt_end; ++kt, ++it) {
       const int s = static_cast<int>(it % stages);
       const uint32_t ph = (it / stages) & 1u;
@@ -403,12 +407,15 @@ __device__ void pair_producer(const ProjParams& p, const PairSmem& sm, bool lead
       int xk = (lora ? kt - base_kt : kt) * kBlockK;
       int xrow = t.t0;                               // first row of the tile in xmap
       int brow = mb.swiglu ? 2 * t.f0 : t.f0;        // SwiGLU: the interleaved B stack holds 128 rows per 64 features
-      if (lora && p.ext_first != nullptr) {          // adapters by request
-        const int e = (kt - base_kt) / p.ext_chunks;
-        xk = (kt - base_kt - e * p.ext_chunks) * kBlockK;
-        const int2 ent = p.ext_list[t.ext0 + e];
-        xrow = ent.x * p.n_tok;
-        brow = ent.y * mb.N + t.f0;
+      if (lora && ext) {
+        const int e = (kt - base_kt) / p.ext_chunks, chunk = kt - base_kt - e * p.ext_chunks;
+        if (chunk == 0) {
+          ext_now = ext_next;
+          if (kt + p.ext_chunks < t.kt_end) ext_next = p.ext_list[t.ext0 + e + 1];
+        }
+        xk = chunk * kBlockK;
+        xrow = ext_now.x * p.n_tok;
+        brow = ext_now.y * mb.N + t.f0;
       }
       if (!lora && quant) {
         if (leader) mbar_arrive_expect_tx(full_local, xbytes_pair);

@@ -534,13 +534,13 @@ class Context:
         n, k = w.info.n, w.info.k
         ldx = _rows("x", x, m, k)
         if out is None:
-            out = _alloc_out(m, n, x.device)
+            out = x.new_empty((m, n)) if n % 8 == 0 else _alloc_out(m, n, x.device)
         ldy = _rows("out", out, m, n)
         v, vp, ldv = None, None, 0
         if ranks is not False and ranks is not None:
             v = ranks
             if ranks is True:
-                v = torch.empty((m, bank.rank_pad), dtype=torch.float32, device=x.device)
+                v = x.new_empty((m, bank.rank_pad), dtype=torch.float32)
             ldv = _rows("ranks", v, m, bank.rank_pad, torch.float32)
             vp = v.data_ptr()
         rc = self.lib.mp_linear_requests(
@@ -570,7 +570,7 @@ class Context:
         dxp = dap = dbp = xp = qp = sp = vp = None
         lddx = ldx = ldq = ldv = 0
         if need_dx:
-            dx = _alloc_out(m, k, dy.device)
+            dx = dy.new_empty((m, k)) if k % 8 == 0 else _alloc_out(m, k, dy.device)
             lddx = _rows("dx", dx, m, k)
             dxp = dx.data_ptr()
         if need_factors:
@@ -585,10 +585,8 @@ class Context:
                 raise ValueError(f"v must have at least {bank.max_rank} columns")
             ldv = _rows("v", v, m, v.shape[1], torch.float32)
             vp = v.data_ptr()
-            da = torch.empty((plan.capacity, bank.max_rank, k), dtype=torch.float32,
-                             device=dy.device)
-            db = torch.empty((plan.capacity, n, bank.max_rank), dtype=torch.float32,
-                             device=dy.device)
+            da = dy.new_empty((plan.capacity, bank.max_rank, k), dtype=torch.float32)
+            db = dy.new_empty((plan.capacity, n, bank.max_rank), dtype=torch.float32)
             dap, dbp = da.data_ptr(), db.data_ptr()
         rc = self.lib.mp_linear_requests_grad(
             self.h, wt.handle, dy.data_ptr(), ldy, xp, ldx, qp, ldq, sp, vp, ldv, bank.handle,
@@ -603,8 +601,8 @@ class Context:
         m, k = x.shape
         ldx = _rows("x", x, m, k)
         ldq = (k + 15) // 16 * 16
-        q = torch.empty((m, ldq), dtype=torch.int8, device=x.device)
-        scale = torch.empty(((k + 127) // 128, m), dtype=torch.float32, device=x.device)
+        q = x.new_empty((m, ldq), dtype=torch.int8)
+        scale = x.new_empty(((k + 127) // 128, m), dtype=torch.float32)
         rc = self.lib.mp_checkpoint(self.h, x.data_ptr(), ldx, m, k, q.data_ptr(), ldq,
                                     scale.data_ptr(), _stream_handle(stream))
         if rc != MP_OK:
