@@ -2036,11 +2036,14 @@ mp::RankParams rank_params(const mp_ctx* c, const RequestsLaunch& ext, const voi
 }
 
 // The rank-space rows of a batch of requests: v = s_q (x F_q^T), into `r`'s
-// outputs. Requests of 16 rows and more on average go to the tensor core in
-// tiles of 128 rows, shorter ones in runs of 8 rows.
+// outputs. Where there is much to multiply, requests of 16 rows and more on
+// average go to the tensor core in tiles of 128 rows; else runs of 8 rows. At
+// m 4352, k 3840 the runs / the tiles take 12.7 / 14.4 us with 16 ranks (m k rp
+// = 2.7e8), 20.6 / 15.4 us with 32 (5.3e8); at m 16896 with 64, 175 / 37 us.
 int launch_ranks(mp_ctx* c, const RequestsLaunch& ext, mp::RankParams* r, cudaStream_t stream) {
   const mp::RequestPlan& pl = r->plan;
-  const bool tiles = pl.m > mp::kFewRows && pl.m >= 16 * static_cast<int64_t>(pl.n_req);
+  const bool tiles = pl.m >= 16 * static_cast<int64_t>(pl.n_req) &&
+                     static_cast<double>(pl.m) * r->k * r->rp >= 4.0e8;
   cudaError_t e;
   if (tiles) {
     if (!encode_2d(&r->tm_x, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, r->x, r->k, pl.m, static_cast<uint64_t>(r->ldx) * 2, 64,
@@ -2436,8 +2439,10 @@ int mp_linear_requests_grad(mp_ctx* c, const mp_weight* wt, const void* dy, int6
       rc = check_x(c, x, ldx, k, m);
     }
   }
-  if (rc == MP_OK && db != nullptr && (v == nullptr || ldv < b->max_rank))
-    rc = fail(c, MP_EINVAL, "v: f32 rows of at least %d ranks are required", b->max_rank);
+  if (rc == MP_OK && db != nullptr)
+    rc = v == nullptr ? fail(c, MP_EINVAL, "v is required for db") : check_rank_rows(c, v, ldv, b->max_rank);
+  if (rc == MP_OK && (reinterpret_cast<uintptr_t>(da) % 16 != 0 || reinterpret_cast<uintptr_t>(db) % 16 != 0))
+    rc = fail(c, MP_EINVAL, "da and db must be 16-byte aligned");
   if (rc == MP_OK) rc = use_device(c);
   if (rc != MP_OK) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -2473,6 +2478,10 @@ int mp_linear_requests_grad(mp_ctx* c, const mp_weight* wt, const void* dy, int6
     return encode_2d(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, base, width, m, static_cast<uint64_t>(ld) * 2, 64, 64,
                      CU_TENSOR_MAP_SWIZZLE_128B);
   };
+  auto ranks_map = [&](CUtensorMap* map, const float* base, int64_t ld) {
+    return encode_2d(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, base, b->max_rank, m, static_cast<uint64_t>(ld) * 4, b->rp,
+                     64, CU_TENSOR_MAP_SWIZZLE_NONE);
+  };
   bool maps = true;
   if (da != nullptr) {
     mp::GradMember& mb = g.mem[g.n_mem++];
@@ -2483,17 +2492,14 @@ int mp_linear_requests_grad(mp_ctx* c, const mp_weight* wt, const void* dy, int6
     } else {
       maps = rows_map(&mb.tm_x, x, ldx, k);
     }
-    mb.u = c->req_u;
-    mb.ldu = b->rp;
+    maps = maps && ranks_map(&mb.tm_u, c->req_u, b->rp);
     mb.out = da;
     mb.width = k;
     mb.rank_major = 1;
   }
   if (db != nullptr) {
     mp::GradMember& mb = g.mem[g.n_mem++];
-    maps = maps && rows_map(&mb.tm_x, dy, ldy, n);
-    mb.u = v;
-    mb.ldu = ldv;
+    maps = maps && rows_map(&mb.tm_x, dy, ldy, n) && ranks_map(&mb.tm_u, v, ldv);
     mb.out = db;
     mb.width = n;
   }

@@ -7,18 +7,21 @@
 // v = s x A^T. Bound by memory: x and dy are read once, 2 r operations for
 // every byte or two of them.
 //
-// One cluster per adapter and 128 features; its CTAs take the adapter's rows
-// 64 at a time in turn and add their sums through distributed shared memory, in
-// CTA order. Per 64 rows: x by TMA, [64 rows][64 features] boxes that are the
-// MN-major A operand of tcgen05 as they land (M = features, K = rows); u, f32 in
-// memory, is cut by warps 2-9 into three bf16 parts of 8 bits each, side by
-// side in the N of the B operand: the products are then those of the f32
-// values, and cost no second pass over x.
+// An item is one adapter and 128 features. Per 64 of its rows: x by TMA, [64
+// rows][64 features] boxes that are the MN-major A operand of tcgen05 as they land
+// (M = features, K = rows); u, f32, by TMA too, is cut by warps 2-9 into three bf16
+// parts of 8 bits each, side by side in the N of the B operand: the products are
+// then those of the f32 values, and cost no second pass over x.
 //
 // tcgen05 adds to its f32 accumulator without rounding to nearest: over a long
 // run of rows the sums drift towards zero (2e-6 at 1000 rows). So an accumulator
 // takes kChunk stages (256 rows) only; the last warps then add it, the three
 // parts smallest first, to sums in registers, while the MMAs fill the other one.
+//
+// With many items the CTAs are persistent: they walk the items, the loads of the
+// next one running while the last warps write this one's sums. With few, a cluster
+// takes one item, its CTAs the row tiles in turn, and they add their sums through
+// distributed shared memory, in CTA order.
 //
 // A checkpoint's codes are whole numbers of up to 8 bits, exact in bf16: warps
 // 2-9 widen them, and the scale of a (row, 128 features) goes into u, in f32.
@@ -53,7 +56,7 @@ constexpr uint32_t kBoxBytes = kRows * 128;      // [64 rows][64 bf16]
 constexpr uint32_t kXBytes = 2 * kBoxBytes;      // the A operand
 constexpr uint32_t kCodeBytes = kRows * kTileF;  // a stage's codes
 constexpr int kMaxGradStages = 6;
-constexpr uint32_t kGradSmemMost = 220 * 1024;
+constexpr uint32_t kGradSmemMost = 226 * 1024;
 
 constexpr uint32_t kAllBarrier = 1;  // named barrier of the whole CTA
 
@@ -94,18 +97,26 @@ __host__ __device__ inline PartCols part_cols(int rp) {
 // rank fastest, and one more float puts consecutive ranks in different banks.
 __host__ __device__ inline int exchange_ld(bool rank_major) { return rank_major ? kTileF : kTileF + 1; }
 
+// A stage: x as the A operand | u's parts, the B operand | u, f32 | with a
+// checkpoint its codes and the rows' scales.
 struct GradGeo {
   int stages;
-  uint32_t stage_bytes, u_off, code_off;
+  uint32_t parts_off, u_off, code_off, scale_off, stage_bytes;
   uint32_t smem;
 };
 
 __host__ __device__ inline GradGeo grad_geo(int rp, bool codes) {
   GradGeo g;
-  g.u_off = kXBytes;
-  g.code_off = kXBytes + part_cols(rp).boxes * kBoxBytes;
-  g.stage_bytes = g.code_off + (codes ? kCodeBytes : 0);
-  g.stages = static_cast<int>(kGradSmemMost / g.stage_bytes);
+  const PartCols pc = part_cols(rp);
+  g.parts_off = kXBytes;
+  g.u_off = g.parts_off + pc.boxes * kBoxBytes;
+  g.code_off = g.u_off + kRows * rp * 4;
+  g.scale_off = g.code_off + (codes ? kCodeBytes : 0);
+  g.stage_bytes = (g.scale_off + (codes ? kRows * 4 : 0) + 1023) / 1024 * 1024;
+  // two CTAs an SM with up to 32 ranks (their accumulators take half of TMEM each)
+  const uint32_t half = 112 * 1024;
+  const bool two = rp <= 32 && 2 * g.stage_bytes + 1280 <= half;
+  g.stages = static_cast<int>(((two ? half : kGradSmemMost) - 1280) / g.stage_bytes);
   if (g.stages > kMaxGradStages) g.stages = kMaxGradStages;
   const uint32_t tiles = g.stages * g.stage_bytes;
   const uint32_t exchange = rp * (kTileF + 1) * 4;
@@ -171,29 +182,21 @@ __device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
   return v;
 }
 
-// Eight values of row `row` of u from column c: zeros past the valid columns
-// and for rows outside the segment.
-__device__ __forceinline__ void load_u8(const float* u, int64_t ldu, int64_t row, int c, int cols, bool vec, bool ok,
-                                        float (&f)[8]) {
-  const float* at = u + row * ldu + c;
-  if (ok && vec && c + 8 <= cols) {
-    const float4 a = *reinterpret_cast<const float4*>(at), b = *reinterpret_cast<const float4*>(at + 4);
-    f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w;
-    f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = ok && c + i < cols ? at[i] : 0.0f;
-  }
-}
-
-// The next bf16 part of two values, which keep what is left of them. An
-// infinity or NaN is all in its first part (inf - inf would be NaN).
+// The next bf16 part of two values, which keep what is left of them.
 __device__ __forceinline__ uint32_t take_part(float& a, float& b) {
   const uint32_t w = pack_bf16x2(a, b);
-  const float ha = __uint_as_float(w << 16), hb = __uint_as_float(w & 0xFFFF0000u);
-  a = fabsf(ha) <= 3.4e38f ? a - ha : 0.0f;
-  b = fabsf(hb) <= 3.4e38f ? b - hb : 0.0f;
+  a -= __uint_as_float(w << 16);
+  b -= __uint_as_float(w & 0xFFFF0000u);
   return w;
+}
+
+// 4 bytes, asynchronously; and their arrival on an mbarrier whose count has a
+// place for this thread.
+__device__ __forceinline__ void cp_async_4(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
 }
 
 struct GradSmem {
@@ -206,14 +209,29 @@ struct GradSmem {
   volatile uint32_t* abort;
 };
 
-// TASKS: 8-value pieces of a 64-row stage of u per converting thread.
-template <int TASKS, bool CODES>
-__device__ void convert(const GradParams& p, const GradMember& mb, const GradSmem& sm, const GradGeo& geo,
-                        const PartCols& pc, int a, int f_tile, int rank, int count) {
+// An item: its adapter, member and feature tile.
+struct Item {
+  int a, f_tile;
+  const GradMember* mb;
+};
+
+__device__ __forceinline__ Item item_of(const GradParams& p, int i) {
+  Item it;
+  it.a = i / p.tiles;
+  int t = i - it.a * p.tiles;
+  const int first = (p.mem[0].width + kTileF - 1) / kTileF;
+  const bool second = p.n_mem > 1 && t >= first;
+  it.mb = &p.mem[second ? 1 : 0];
+  it.f_tile = second ? t - first : t;
+  return it;
+}
+
+// Warps 2-9. TASKS: 8-value pieces of a 64-row stage of u per thread.
+template <int TASKS>
+__device__ void convert(const GradParams& p, const GradSmem& sm, const GradGeo& geo, const PartCols& pc, int item0,
+                        int step, int rank, int count) {
   const int tid = threadIdx.x - 32 * kConvWarp0, lane = threadIdx.x & 31;
   const int per_row = p.rp / 8, pieces = kRows * per_row;
-  const bool vec = mb.ldu % 4 == 0 && (reinterpret_cast<uintptr_t>(mb.u) & 15) == 0;
-  const float* scale = CODES ? mb.scale + static_cast<int64_t>(f_tile) * p.plan.m : nullptr;
   int row_of[TASKS], col_of[TASKS];
 #pragma unroll
   for (int j = 0; j < TASKS; ++j) {
@@ -221,99 +239,107 @@ __device__ void convert(const GradParams& p, const GradMember& mb, const GradSme
     row_of[j] = e < pieces ? e / per_row : kRows;  // kRows: no piece
     col_of[j] = e < pieces ? e % per_row * 8 : 0;
   }
-  float f[TASKS][8], by[TASKS];
-  auto load = [&](int t0, int rows) {
-#pragma unroll
-    for (int j = 0; j < TASKS; ++j) {
-      const bool ok = row_of[j] < rows;
-      load_u8(mb.u, mb.ldu, t0 + row_of[j], col_of[j], p.r, vec, ok, f[j]);
-      if (CODES) by[j] = ok ? scale[t0 + row_of[j]] : 0.0f;
-    }
-  };
   // one answer for the warp, so that all of its lanes give up together
   auto wait_all = [&](uint32_t bar, uint32_t parity, uint32_t site) {
     return __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity, sm.abort, site, p.wait_limit_ns)) != 0;
   };
-  TileIter it(p.plan, a, rank, count);
-  int t0, rows;
-  bool have = it.next(t0, rows);
-  if (have) load(t0, rows);
-  for (uint32_t n = 0; have; ++n) {
-    const int s = static_cast<int>(n % geo.stages);
-    const uint32_t ph = (n / geo.stages) & 1u;
-    if (n >= static_cast<uint32_t>(geo.stages) &&
-        !wait_all(smem_u32(&sm.empty[s]), ph ^ 1u, kSiteGradEmpty | s))
-      return;
-    const uint32_t xs = sm.tiles + s * geo.stage_bytes, us = xs + geo.u_off;
-#pragma unroll
-    for (int j = 0; j < TASKS; ++j) {
-      if (row_of[j] >= kRows) continue;
-      const uint32_t row = us + row_of[j] * 128u, sw = static_cast<uint32_t>(row_of[j] & 7);
-      if (CODES) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) f[j][i] *= by[j];
-      }
-#pragma unroll
-      for (int part = 0; part < kParts; ++part) {
-        uint32_t w[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = take_part(f[j][2 * i], f[j][2 * i + 1]);
-        const uint32_t col = col_of[j] + (part == 2 ? pc.third : part * p.rp);
-        st_shared_v4(row + (col >> 6) * kBoxBytes + (((col >> 3 & 7u) ^ sw) << 4), w[0], w[1], w[2], w[3]);
-      }
-    }
-    const int rows_now = rows;
-    have = it.next(t0, rows);
-    if (have) load(t0, rows);  // in flight until the next stage
-    if (CODES) {
+  int n = 0;
+  for (int i = item0; i < p.items; i += step) {
+    const Item item = item_of(p, i);
+    const bool codes = item.mb->scale != nullptr;
+    TileIter it(p.plan, item.a, rank, count);
+    int t0, rows;
+    for (; it.next(t0, rows); ++n) {
+      const int s = n % geo.stages;
+      const uint32_t ph = (n / geo.stages) & 1u;
+      // the tile has landed (so the stage's last MMAs are done)
       if (!wait_all(smem_u32(&sm.full[s]), ph, kSiteGradFull | s)) return;
+      const uint32_t xs = sm.tiles + s * geo.stage_bytes, parts = xs + geo.parts_off;
 #pragma unroll
-      for (int j = 0; j < kRows * kTileF / 16 / kConvThreads; ++j) {  // 16 codes of a row at a time
-        const int e = tid + j * kConvThreads, row = e / (kTileF / 16), c = e % (kTileF / 16);
-        uint4 q = ld_shared_v4(xs + geo.code_off + row * kTileF + c * 16);
-        if (row >= rows_now) q = make_uint4(0, 0, 0, 0);
-        const uint32_t qw[4] = {q.x, q.y, q.z, q.w};
-        uint32_t w[8];
+      for (int j = 0; j < TASKS; ++j) {
+        if (row_of[j] >= kRows) continue;
+        // rows past the segment's last are another request's: zeros
+        float f[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+        if (row_of[j] < rows) {
+          const uint32_t at = xs + geo.u_off + (row_of[j] * p.rp + col_of[j]) * 4u;
+          const float4 a = ld_shared_f4(at), b = ld_shared_f4(at + 16);
+          f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w;
+          f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
+          if (codes) {
+            float by;
+            asm volatile("ld.shared.f32 %0, [%1];" : "=f"(by) : "r"(xs + geo.scale_off + row_of[j] * 4u));
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          // byte b + 128 as the float 32768 + (b + 128), less 32896: exact
-          const uint32_t ofs = qw[i] ^ 0x80808080u;
-          const float v0 = __uint_as_float(__byte_perm(ofs, 0x4700u, 0x5404u)) - 32896.0f;
-          const float v1 = __uint_as_float(__byte_perm(ofs, 0x4700u, 0x5414u)) - 32896.0f;
-          const float v2 = __uint_as_float(__byte_perm(ofs, 0x4700u, 0x5424u)) - 32896.0f;
-          const float v3 = __uint_as_float(__byte_perm(ofs, 0x4700u, 0x5434u)) - 32896.0f;
-          w[2 * i] = pack_bf16x2(v0, v1);
-          w[2 * i + 1] = pack_bf16x2(v2, v3);
+            for (int e = 0; e < 8; ++e) f[e] *= by;
+          }
         }
-        const uint32_t at = xs + (c >> 2) * kBoxBytes + row * 128u, ch = static_cast<uint32_t>(2 * (c & 3));
-        const uint32_t sw = static_cast<uint32_t>(row & 7);
-        st_shared_v4(at + ((ch ^ sw) << 4), w[0], w[1], w[2], w[3]);
-        st_shared_v4(at + (((ch + 1) ^ sw) << 4), w[4], w[5], w[6], w[7]);
+        float top = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(f[e]));
+        const uint32_t row = parts + row_of[j] * 128u, sw = static_cast<uint32_t>(row_of[j] & 7);
+#pragma unroll
+        for (int part = 0; part < kParts; ++part) {
+          uint32_t w[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) w[e] = take_part(f[2 * e], f[2 * e + 1]);
+          if (part == 0 && top > 3.38e38f) {
+            // an infinity is all in its first part (inf - inf would be NaN)
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              if ((w[e >> 1] >> (16 * (e & 1)) & 0x7FFFu) == 0x7F80u) f[e] = 0.0f;
+          }
+          const uint32_t col = col_of[j] + (part == 2 ? pc.third : part * p.rp);
+          st_shared_v4(row + (col >> 6) * kBoxBytes + (((col >> 3 & 7u) ^ sw) << 4), w[0], w[1], w[2], w[3]);
+        }
       }
-    } else if (rows_now < kRows) {
-      // the rows after the segment's last are another request's: zeros, since
-      // an infinity or NaN there would come through a product with 0
-      if (!wait_all(smem_u32(&sm.full[s]), ph, kSiteGradFull | s)) return;
-      for (int e = rows_now * 8 + tid; e < kRows * 8; e += kConvThreads) {
-        st_shared_v4(xs + e * 16, 0, 0, 0, 0);
-        st_shared_v4(xs + kBoxBytes + e * 16, 0, 0, 0, 0);
+      if (codes) {
+#pragma unroll
+        for (int j = 0; j < kRows * kTileF / 16 / kConvThreads; ++j) {  // 16 codes of a row at a time
+          const int e = tid + j * kConvThreads, row = e / (kTileF / 16), c = e % (kTileF / 16);
+          uint4 q = ld_shared_v4(xs + geo.code_off + row * kTileF + c * 16);
+          if (row >= rows) q = make_uint4(0, 0, 0, 0);
+          const uint32_t qw[4] = {q.x, q.y, q.z, q.w};
+          const uint64_t less = f32x2(-32896.0f, -32896.0f);
+          uint32_t w[8];
+#pragma unroll
+          for (int h = 0; h < 4; ++h) {
+            // byte b + 128 as the float 32768 + (b + 128), less 32896: exact
+            const uint32_t ofs = qw[h] ^ 0x80808080u;
+            auto code = [&](uint32_t sel) { return __uint_as_float(__byte_perm(ofs, 0x4700u, sel)); };
+            w[2 * h] = f32x2_to_bf16x2(add_f32x2(f32x2(code(0x5404u), code(0x5414u)), less));
+            w[2 * h + 1] = f32x2_to_bf16x2(add_f32x2(f32x2(code(0x5424u), code(0x5434u)), less));
+          }
+          const uint32_t at = xs + (c >> 2) * kBoxBytes + row * 128u, ch = static_cast<uint32_t>(2 * (c & 3));
+          const uint32_t sw = static_cast<uint32_t>(row & 7);
+          st_shared_v4(at + ((ch ^ sw) << 4), w[0], w[1], w[2], w[3]);
+          st_shared_v4(at + (((ch + 1) ^ sw) << 4), w[4], w[5], w[6], w[7]);
+        }
+      } else if (rows < kRows) {
+        // an infinity or NaN in the rows after the segment's last would come
+        // through a product with 0
+        for (int e = rows * 8 + tid; e < kRows * 8; e += kConvThreads) {
+          st_shared_v4(xs + e * 16, 0, 0, 0, 0);
+          st_shared_v4(xs + kBoxBytes + e * 16, 0, 0, 0, 0);
+        }
       }
+      fence_proxy_async_shared();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&sm.conv[s]));
     }
-    fence_proxy_async_shared();
-    __syncwarp();
-    if (lane == 0) mbar_arrive(smem_u32(&sm.conv[s]));
   }
 }
 
-template <int TASKS, bool CODES>
-__device__ void grad_tile(const GradParams& p, const GradMember& mb, int a, int f_tile, uint8_t* raw) {
+template <int TASKS>
+__global__ void __launch_bounds__(kGradThreads<TASKS>, TASKS == 1 ? 2 : 1)
+    adapter_grad_kernel(const __grid_constant__ GradParams p) {
+  extern __shared__ uint8_t grad_raw[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int rank = static_cast<int>(cluster_ctarank()), count = p.splits;
+  const int count = p.splits, rank = count > 1 ? static_cast<int>(cluster_ctarank()) : 0;
+  const int item0 = static_cast<int>(blockIdx.x) / count, step = static_cast<int>(gridDim.x) / count;
   const int col0 = warp >= kSumWarp0 + 4 ? kSumCols<TASKS> : 0;  // the adding warp's first rank
   const PartCols pc = part_cols(p.rp);
-  const GradGeo geo = grad_geo(p.rp, CODES);
+  const GradGeo geo = grad_geo(p.rp, p.codes != 0);
   GradSmem sm;
-  uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023u) & ~uintptr_t(1023u));
+  uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(grad_raw) + 1023u) & ~uintptr_t(1023u));
   sm.tiles = smem_u32(base);
   sm.exchange = reinterpret_cast<float*>(base);
   uint64_t* bars = reinterpret_cast<uint64_t*>(base + geo.smem - 1024 - 256);
@@ -327,7 +353,7 @@ __device__ void grad_tile(const GradParams& p, const GradMember& mb, int a, int 
   sm.abort = sm.tmem_slot + 1;
   if (threadIdx.x == 0) {
     for (int s = 0; s < geo.stages; ++s) {
-      mbar_init(smem_u32(&sm.full[s]), 1);
+      mbar_init(smem_u32(&sm.full[s]), 33);  // the producer's lane 0 with the copies' bytes, and every lane
       mbar_init(smem_u32(&sm.conv[s]), kConvThreads / 32);
       mbar_init(smem_u32(&sm.empty[s]), 1);
     }
@@ -338,7 +364,10 @@ __device__ void grad_tile(const GradParams& p, const GradMember& mb, int a, int 
     mbar_init(smem_u32(sm.done), 1);
     *sm.abort = 0u;
     fence_mbar_init();
-    tma_prefetch_map(&mb.tm_x);
+    for (int i = 0; i < p.n_mem; ++i) {
+      tma_prefetch_map(&p.mem[i].tm_x);
+      tma_prefetch_map(&p.mem[i].tm_u);
+    }
   }
   if (warp == 1) {
     tmem_alloc(smem_u32(sm.tmem_slot), pc.cols * pc.bufs);
@@ -351,62 +380,79 @@ __device__ void grad_tile(const GradParams& p, const GradMember& mb, int a, int 
   pdl_wait();
   pdl_release();
 
-  const int tiles = TileIter(p.plan, a, rank, count).total();
-  const int ld = exchange_ld(mb.rank_major != 0);
   if (warp == 0) {
-    if (lane == 0) {
-      TileIter it(p.plan, a, rank, count);
+    int n = 0;
+    bool ok = true;
+    for (int i = item0; i < p.items && ok; i += step) {
+      const Item item = item_of(p, i);
+      const GradMember& mb = *item.mb;
+      const bool codes = mb.scale != nullptr;
+      TileIter it(p.plan, item.a, rank, count);
       int t0, rows;
-      uint32_t n = 0, pend = 0;
-      for (; it.next(t0, rows); ++n) {
-        const int s = static_cast<int>(n % geo.stages);
-        if (n >= static_cast<uint32_t>(geo.stages) &&
-            !mbar_wait(smem_u32(&sm.empty[s]), ((n / geo.stages) & 1u) ^ 1u, sm.abort, kSiteGradEmpty | s,
-                       p.wait_limit_ns))
-          break;
+      for (; ok && it.next(t0, rows); ++n) {
+        const int s = n % geo.stages;
+        if (n >= geo.stages)
+          ok = __all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&sm.empty[s]), ((n / geo.stages) & 1u) ^ 1u, sm.abort,
+                                                 kSiteGradEmpty | s, p.wait_limit_ns)) != 0;
+        if (!ok) break;
         const uint32_t bar = smem_u32(&sm.full[s]), xs = sm.tiles + s * geo.stage_bytes;
-        if (CODES) {
-          mbar_arrive_expect_tx(bar, kCodeBytes);
-          tma_load_2d(xs + geo.code_off, &mb.tm_x, bar, f_tile * kTileF, t0);
-        } else {
-          mbar_arrive_expect_tx(bar, kXBytes);
-          tma_load_2d(xs, &mb.tm_x, bar, f_tile * kTileF, t0);
-          tma_load_2d(xs + kBoxBytes, &mb.tm_x, bar, f_tile * kTileF + 64, t0);
+        if (lane == 0) {
+          mbar_arrive_expect_tx(bar, kRows * p.rp * 4 + (codes ? kCodeBytes : kXBytes));
+          tma_load_2d(xs + geo.u_off, &mb.tm_u, bar, 0, t0);
+          if (codes) {
+            tma_load_2d(xs + geo.code_off, &mb.tm_x, bar, item.f_tile * kTileF, t0);
+          } else {
+            tma_load_2d(xs, &mb.tm_x, bar, item.f_tile * kTileF, t0);
+            tma_load_2d(xs + kBoxBytes, &mb.tm_x, bar, item.f_tile * kTileF + 64, t0);
+          }
         }
-        pend = n + 1;
-      }
-      if (*sm.abort != 0u) {
-        // copies in flight land (bounded) before the CTA leaves
-        const uint64_t since = global_timer_ns();
-        for (uint32_t j = pend > static_cast<uint32_t>(geo.stages) ? pend - geo.stages : 0; j < pend; ++j)
-          while (!mbar_try_wait(smem_u32(&sm.full[j % geo.stages]), (j / geo.stages) & 1u))
-            if (global_timer_ns() - since > p.wait_limit_ns) break;
+        if (codes) {
+          const float* scale = mb.scale + static_cast<int64_t>(item.f_tile) * p.plan.m + t0;
+          for (int r = lane; r < rows; r += 32) cp_async_4(xs + geo.scale_off + r * 4u, scale + r);
+        }
+        cp_async_arrive(bar);
       }
     }
+    if (*sm.abort != 0u && lane == 0) {
+      // copies in flight land (bounded) before the CTA leaves
+      const uint64_t since = global_timer_ns();
+      for (int j = max(0, n - geo.stages); j < n; ++j)
+        while (!mbar_try_wait(smem_u32(&sm.full[j % geo.stages]), (j / geo.stages) & 1u))
+          if (global_timer_ns() - since > p.wait_limit_ns) break;
+    }
   } else if (warp == 1) {
-    if (lane == 0 && tiles > 0) {
+    if (lane == 0) {
       const uint32_t mn = (1u << 15) | (1u << 16);  // both operands MN-major
       const uint32_t id1 = make_idesc_bf16(kTileF, pc.n1) | mn, id2 = make_idesc_bf16(kTileF, pc.n2) | mn;
-      for (int n = 0; n < tiles; ++n) {
-        const int s = n % geo.stages, chunk = n / kChunk, b = chunk % pc.bufs, use = chunk / pc.bufs;
-        const uint32_t ph = (n / geo.stages) & 1u;
-        if (n % kChunk == 0 && use > 0 &&
-            !mbar_wait(smem_u32(&sm.taken[b]), (use - 1) & 1u, sm.abort, kSiteGradTaken | b, p.wait_limit_ns))
-          break;
-        if (!mbar_wait(smem_u32(&sm.full[s]), ph, sm.abort, kSiteGradFull | s, p.wait_limit_ns) ||
-            !mbar_wait(smem_u32(&sm.conv[s]), ph, sm.abort, kSiteGradConv | s, p.wait_limit_ns))
-          break;
-        tc_fence_after();
-        const uint32_t xs = sm.tiles + s * geo.stage_bytes, us = xs + geo.u_off, d = tmem + b * pc.cols;
+      int n = 0, chunk = 0;  // stages and accumulators filled
+      bool ok = true;
+      for (int i = item0; i < p.items && ok; i += step) {
+        const int tiles = TileIter(p.plan, item_of(p, i).a, rank, count).total();
+        for (int k = 0; k < tiles; ++k, ++n) {
+          const int s = n % geo.stages, b = chunk % pc.bufs, use = chunk / pc.bufs;
+          const uint32_t ph = (n / geo.stages) & 1u;
+          const bool first = k % kChunk == 0, last = k % kChunk == kChunk - 1 || k == tiles - 1;
+          if (first && use > 0)
+            ok = mbar_wait(smem_u32(&sm.taken[b]), (use - 1) & 1u, sm.abort, kSiteGradTaken | b, p.wait_limit_ns);
+          // the converting warps arrive after the tile has landed
+          ok = ok && mbar_wait(smem_u32(&sm.full[s]), ph, sm.abort, kSiteGradFull | s, p.wait_limit_ns) &&
+               mbar_wait(smem_u32(&sm.conv[s]), ph, sm.abort, kSiteGradConv | s, p.wait_limit_ns);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t xs = sm.tiles + s * geo.stage_bytes, us = xs + geo.parts_off, d = tmem + b * pc.cols;
 #pragma unroll
-        for (int kk = 0; kk < kRows / 16; ++kk) {
-          const uint32_t acc = n % kChunk != 0 || kk > 0 ? 1u : 0u;
-          umma_ss(d, mn_desc(xs, kk), mn_desc(us, kk), id1, acc);
-          if (pc.n2 > 0)
-            umma_ss(d + pc.third, mn_desc(xs, kk), mn_desc(us + (pc.third >> 6) * kBoxBytes, kk), id2, acc);
+          for (int kk = 0; kk < kRows / 16; ++kk) {
+            const uint32_t acc = !first || kk > 0 ? 1u : 0u;
+            umma_ss(d, mn_desc(xs, kk), mn_desc(us, kk), id1, acc);
+            if (pc.n2 > 0)
+              umma_ss(d + pc.third, mn_desc(xs, kk), mn_desc(us + (pc.third >> 6) * kBoxBytes, kk), id2, acc);
+          }
+          umma_commit(smem_u32(&sm.empty[s]));
+          if (last) {
+            umma_commit(smem_u32(&sm.sum[b]));
+            ++chunk;
+          }
         }
-        umma_commit(smem_u32(&sm.empty[s]));
-        if (n % kChunk == kChunk - 1 || n == tiles - 1) umma_commit(smem_u32(&sm.sum[b]));
       }
       umma_commit(smem_u32(sm.done));
       const uint64_t since = global_timer_ns();
@@ -417,103 +463,123 @@ __device__ void grad_tile(const GradParams& p, const GradMember& mb, int a, int 
         }
     }
   } else if (warp < kSumWarp0) {
-    convert<TASKS, CODES>(p, mb, sm, geo, pc, a, f_tile, rank, count);
+    convert<TASKS>(p, sm, geo, pc, item0, step, rank, count);
   } else {
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const int f = (warp & 3) * 32 + lane;
     float sums[kSumCols<TASKS>];  // one feature, consecutive ranks
+    int chunk = 0;
+    bool ok = true;
+    for (int i = item0; i < p.items && ok; i += step) {
+      const Item item = item_of(p, i);
+      const int tiles = TileIter(p.plan, item.a, rank, count).total();
 #pragma unroll
-    for (int c = 0; c < kSumCols<TASKS>; ++c) sums[c] = 0.0f;
-    for (int chunk = 0; chunk * kChunk < tiles; ++chunk) {
-      const int b = chunk % pc.bufs;
-      if (!__all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&sm.sum[b]), (chunk / pc.bufs) & 1u, sm.abort,
-                                             kSiteGradSum | b, p.wait_limit_ns)))
-        break;
-      tc_fence_after();
+      for (int c = 0; c < kSumCols<TASKS>; ++c) sums[c] = 0.0f;
+      for (int k = 0; k < tiles; k += kChunk, ++chunk) {
+        const int b = chunk % pc.bufs;
+        ok = __all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&sm.sum[b]), (chunk / pc.bufs) & 1u, sm.abort,
+                                               kSiteGradSum | b, p.wait_limit_ns)) != 0;
+        if (!ok) break;
+        tc_fence_after();
 #pragma unroll
-      for (int c = 0; c < kSumCols<TASKS>; c += 16) {
-        if (col0 + c >= p.rp) break;
-        uint32_t v[16], w[16];
-        const uint32_t at = tmem + lanes + b * pc.cols + col0 + c;
-        MP_TMEM_LD_32X32B_X16(at + p.rp, v);
-        MP_TMEM_LD_32X32B_X16(at + pc.third, w);
-        MP_TMEM_WAIT_LD_REGS16(v);
-        MP_TMEM_WAIT_LD_REGS16(w);
+        for (int c = 0; c < kSumCols<TASKS>; c += 16) {
+          if (col0 + c >= p.rp) break;
+          uint32_t v[16], w[16];
+          const uint32_t at = tmem + lanes + b * pc.cols + col0 + c;
+          MP_TMEM_LD_32X32B_X16(at + p.rp, v);
+          MP_TMEM_LD_32X32B_X16(at + pc.third, w);
+          MP_TMEM_WAIT_LD_REGS16(v);
+          MP_TMEM_WAIT_LD_REGS16(w);
 #pragma unroll
-        for (int j = 0; j < 16; ++j) w[j] = __float_as_uint(__uint_as_float(v[j]) + __uint_as_float(w[j]));
-        MP_TMEM_LD_32X32B_X16(at, v);
-        MP_TMEM_WAIT_LD_REGS16(v);
+          for (int j = 0; j < 16; ++j) w[j] = __float_as_uint(__uint_as_float(v[j]) + __uint_as_float(w[j]));
+          MP_TMEM_LD_32X32B_X16(at, v);
+          MP_TMEM_WAIT_LD_REGS16(v);
 #pragma unroll
-        for (int j = 0; j < 16; ++j) sums[c + j] += __uint_as_float(v[j]) + __uint_as_float(w[j]);
+          for (int j = 0; j < 16; ++j) sums[c + j] += __uint_as_float(v[j]) + __uint_as_float(w[j]);
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&sm.taken[b]));
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&sm.taken[b]));
+      if (count > 1 || !ok) break;  // a cluster has one item
+      const int ff = item.f_tile * kTileF + f;
+      if (ff < item.mb->width) {
+        float* out = item.mb->out + static_cast<int64_t>(item.a) * p.r * item.mb->width;
+        if (item.mb->rank_major) {
+#pragma unroll
+          for (int c = 0; c < kSumCols<TASKS>; ++c)
+            if (col0 + c < p.r) out[static_cast<int64_t>(col0 + c) * item.mb->width + ff] = sums[c];
+        } else {
+          float* row = out + static_cast<int64_t>(ff) * p.r + col0;
+          if (p.r % 4 == 0) {  // whole 16-byte pieces (the output is 16-byte aligned)
+#pragma unroll
+            for (int c = 0; c < kSumCols<TASKS>; c += 4)
+              if (col0 + c < p.r)
+                *reinterpret_cast<float4*>(row + c) = make_float4(sums[c], sums[c + 1], sums[c + 2], sums[c + 3]);
+          } else {
+#pragma unroll
+            for (int c = 0; c < kSumCols<TASKS>; ++c)
+              if (col0 + c < p.r) row[c] = sums[c];
+          }
+        }
+      }
     }
     // every copy has landed and every MMA is done (or the CTA gave up): the
-    // stages' memory takes the sums
+    // stages' memory takes a cluster's sums
     named_barrier(kAllBarrier, kGradThreads<TASKS>);
-    const int f = (warp & 3) * 32 + lane;
+    if (count > 1) {
+      const int ld = exchange_ld(item_of(p, item0).mb->rank_major != 0);
 #pragma unroll
-    for (int c = 0; c < kSumCols<TASKS>; ++c)
-      if (col0 + c < p.rp) sm.exchange[(col0 + c) * ld + f] = sums[c];
+      for (int c = 0; c < kSumCols<TASKS>; ++c)
+        if (col0 + c < p.rp) sm.exchange[(col0 + c) * ld + f] = sums[c];
+    }
   }
   __syncwarp();
   if (warp < kSumWarp0) named_barrier(kAllBarrier, kGradThreads<TASKS>);
   const bool aborted = *sm.abort != 0u;
-  cluster_sync();
-  // the CTAs share the adding up: each takes some ranks (dA) or features (dB)
-  const int f0 = f_tile * kTileF, width = min(kTileF, mb.width - f0);
-  float* out = mb.out + static_cast<int64_t>(a) * p.r * mb.width;
-  const uint32_t ex = smem_u32(sm.exchange);
-  auto sum_at = [&](int r, int f) {
-    const uint32_t at = ex + static_cast<uint32_t>(r * ld + f) * 4u;
-    float s = ld_cluster_f32(mapa_shared(at, 0));
-    for (int z = 1; z < count; ++z) s += ld_cluster_f32(mapa_shared(at, z));
-    return s;
-  };
-  if (!aborted) {
-    if (mb.rank_major) {
-      for (int e = threadIdx.x; e < p.r * kTileF; e += kGradThreads<TASKS>) {
-        const int r = e / kTileF, f = e % kTileF;
-        if (r % count == rank && f < width) out[static_cast<int64_t>(r) * mb.width + f0 + f] = sum_at(r, f);
+  if (count > 1) {
+    cluster_sync();
+    if (!aborted) {
+      // the CTAs share the adding up: each takes some ranks (dA) or features (dB)
+      const Item item = item_of(p, item0);
+      const GradMember& mb = *item.mb;
+      const int ld = exchange_ld(mb.rank_major != 0);
+      const int f0 = item.f_tile * kTileF, width = min(kTileF, mb.width - f0);
+      float* out = mb.out + static_cast<int64_t>(item.a) * p.r * mb.width;
+      const uint32_t ex = smem_u32(sm.exchange);
+      auto sum_at = [&](int r, int f) {
+        const uint32_t at = ex + static_cast<uint32_t>(r * ld + f) * 4u;
+        float s = ld_cluster_f32(mapa_shared(at, 0));
+        for (int z = 1; z < count; ++z) s += ld_cluster_f32(mapa_shared(at, z));
+        return s;
+      };
+      if (mb.rank_major) {
+        for (int e = threadIdx.x; e < p.r * kTileF; e += kGradThreads<TASKS>) {
+          const int r = e / kTileF, f = e % kTileF;
+          if (r % count == rank && f < width) out[static_cast<int64_t>(r) * mb.width + f0 + f] = sum_at(r, f);
+        }
+      } else {
+        const int per = kTileF / count, lo = rank * per, hi = min(lo + per, width);
+        for (int e = lo * p.r + threadIdx.x; e < hi * p.r; e += kGradThreads<TASKS>)
+          out[static_cast<int64_t>(f0) * p.r + e] = sum_at(e % p.r, e / p.r);
       }
-    } else {
-      const int per = kTileF / count, lo = rank * per, hi = min(lo + per, width);
-      for (int e = lo * p.r + threadIdx.x; e < hi * p.r; e += kGradThreads<TASKS>)
-        out[static_cast<int64_t>(f0) * p.r + e] = sum_at(e % p.r, e / p.r);
     }
+    cluster_sync();  // no CTA leaves while another reads its sums
+  } else {
+    __syncthreads();
   }
-  cluster_sync();  // no CTA leaves while another reads its sums
   tc_fence_after();
   if (warp == 1) tmem_dealloc(tmem, pc.cols * pc.bufs);
   if (threadIdx.x == 0 && aborted) atomicOr(p.err, kErrTimeout);
 }
 
 template <int TASKS>
-__global__ void __launch_bounds__(kGradThreads<TASKS>, 1) adapter_grad_kernel(const __grid_constant__ GradParams p) {
-  extern __shared__ uint8_t grad_raw[];
-  int tile = static_cast<int>(blockIdx.x) / p.splits, mi = 0;
-  if (p.n_mem > 1) {
-    const int first = (p.mem[0].width + kTileF - 1) / kTileF;
-    if (tile >= first) {
-      mi = 1;
-      tile -= first;
-    }
-  }
-  const int a = blockIdx.y;
-  if (p.mem[mi].scale != nullptr)
-    grad_tile<TASKS, true>(p, p.mem[mi], a, tile, grad_raw);
-  else
-    grad_tile<TASKS, false>(p, p.mem[mi], a, tile, grad_raw);
-}
-
-template <int TASKS>
-cudaError_t launch_tasks(const GradParams& p, uint32_t smem, dim3 grid, cudaStream_t stream) {
+cudaError_t launch_tasks(const GradParams& p, uint32_t smem, unsigned grid, cudaStream_t stream) {
   cudaError_t e = cudaFuncSetAttribute(adapter_grad_kernel<TASKS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                        static_cast<int>(smem));
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
+  cfg.gridDim = dim3(grid);
   cfg.blockDim = dim3(kGradThreads<TASKS>);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
@@ -533,28 +599,29 @@ cudaError_t launch_tasks(const GradParams& p, uint32_t smem, dim3 grid, cudaStre
 
 cudaError_t launch_adapter_grad(const GradParams& p, cudaStream_t stream) {
   GradParams q = p;
-  int tiles = 0;
-  bool codes = false;
+  q.tiles = 0;
+  q.codes = 0;
   for (int i = 0; i < p.n_mem; ++i) {
-    tiles += (p.mem[i].width + kTileF - 1) / kTileF;
-    codes = codes || p.mem[i].scale != nullptr;
+    q.tiles += (p.mem[i].width + kTileF - 1) / kTileF;
+    if (p.mem[i].scale != nullptr) q.codes = 1;
   }
+  const long long items = static_cast<long long>(q.tiles) * p.plan.cap;
+  if (items > (1 << 30)) return cudaErrorInvalidValue;
+  q.items = static_cast<int>(items);
+  const GradGeo geo = grad_geo(p.rp, q.codes != 0);
   // Row splits: while the CTAs of the adapters in use are fewer than the SMs
   // hold at once and each split keeps two stages of rows.
   const int used = p.plan.cap < p.plan.n_req ? p.plan.cap : (p.plan.n_req > 0 ? p.plan.n_req : 1);
   const int rows = (p.plan.m + used - 1) / used;
+  const int room = 148 * (geo.smem <= 113 * 1024 ? 2 : 1);
   q.splits = 1;
-  while (q.splits < 8 && static_cast<long long>(tiles) * used * q.splits < 148 && rows > 2 * kRows * q.splits * 2)
+  while (q.splits < 8 && static_cast<long long>(q.tiles) * used * q.splits < room && rows > 4 * kRows * q.splits)
     q.splits *= 2;
-  uint32_t smem = grad_geo(p.rp, false).smem;
-  if (codes) {
-    const uint32_t s = grad_geo(p.rp, true).smem;
-    smem = s > smem ? s : smem;
-  }
-  const dim3 grid(tiles * q.splits, p.plan.cap);
-  if (p.rp <= 32) return launch_tasks<1>(q, smem, grid, stream);
-  if (p.rp <= 64) return launch_tasks<2>(q, smem, grid, stream);
-  return launch_tasks<4>(q, smem, grid, stream);
+  const unsigned grid = q.splits > 1 ? static_cast<unsigned>(q.items) * q.splits
+                                     : static_cast<unsigned>(q.items < room ? q.items : room);
+  if (p.rp <= 32) return launch_tasks<1>(q, geo.smem, grid, stream);
+  if (p.rp <= 64) return launch_tasks<2>(q, geo.smem, grid, stream);
+  return launch_tasks<4>(q, geo.smem, grid, stream);
 }
 
 }  // namespace mp

@@ -339,9 +339,8 @@ struct CheckpointParams {
 struct GradMember {
   CUtensorMap tm_x;    // bf16 [m, width] (box {64, 64}, SW128), or with `scale`
                        // codes u8 [m, width] (box {128, 64}, no swizzle)
+  CUtensorMap tm_u;    // u: f32 [m, r] (box {rp, 64}, no swizzle)
   const float* scale;  // null, or the checkpoint's scales [groups][m]
-  const float* u;      // f32 [m][ldu]
-  int64_t ldu;
   float* out;
   int32_t width;       // features
   int32_t rank_major;  // 1: out [cap][r][width]; 0: out [cap][width][r]
@@ -351,7 +350,9 @@ struct GradParams {
   GradMember mem[2];
   int32_t n_mem;
   int32_t r, rp;    // ranks written, and rounded up to 16
-  int32_t splits;   // CTAs that share an adapter's rows (set by the launch)
+  // set by the launch: feature tiles of both products, tiles * cap items, CTAs
+  // that share an adapter's rows, whether a member reads a checkpoint
+  int32_t tiles, items, splits, codes;
   RequestPlan plan;
   uint64_t wait_limit_ns;
   uint32_t* err;
