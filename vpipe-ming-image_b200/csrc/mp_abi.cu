@@ -2092,6 +2092,7 @@ int launch_request_ranks(mp_ctx* c, ProjParams* p, const RequestsLaunch& ext, co
   p->ext_live = pl.live[level];
   p->ext_list = pl.list[level];
   p->ext_chunks = chunks;
+  p->late_wait = pl.n_req > 0 ? 1 : 0;  // without requests there may be no rank-space launch
   return MP_OK;
 }
 

@@ -370,6 +370,7 @@ __device__ void pair_producer(const ProjParams& p, const PairSmem& sm, bool lead
   uint32_t pend_full = 0;      // slots whose pair copies this thread has not seen consumed
   uint32_t pend_full_par = 0;
   bool aborted = false;
+  bool waited = false;
   UnitIter units = units_begin(p);
   for (int unit = units_next(p, units); unit != kNoUnit && !aborted; unit = units_next(p, units)) {
     const Tile t = decode_unit(p, unit, rank, base_kt);
@@ -408,6 +409,11 @@ __device__ void pair_producer(const ProjParams& p, const PairSmem& sm, bool lead
       int xrow = t.t0;                               // first row of the tile in xmap
       int brow = mb.swiglu ? 2 * t.f0 : t.f0;        // SwiGLU: the interleaved B stack holds 128 rows per 64 features
       if (lora && ext) {
+        if (p.late_wait && !waited) {  // the rank-space blocks are complete
+          pdl_wait();
+          fence_proxy_async_global();
+          waited = true;
+        }
         const int e = (kt - base_kt) / p.ext_chunks, chunk = kt - base_kt - e * p.ext_chunks;
         if (chunk == 0) {
           ext_now = ext_next;
@@ -1276,7 +1282,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
   tc_fence_after();
   const uint32_t tmem = *sm.tmem_slot;
   // set-up done (shared memory, TMEM, tensor maps): global memory from here on
-  pdl_wait();
+  if (!p.late_wait) pdl_wait();
   pdl_release();
 
   if (warp == 0) {
@@ -1291,6 +1297,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     else
       pair_epilogue_cols(p, sm, tmem, rank, base_kt);
   }
+
+  // whoever waits for this launch waits for the one it ran beside, too
+  if (p.late_wait) pdl_wait();
 
   if (*sm.abort != 0u) {
     // Error path only: let copies issued before the abort land (their
