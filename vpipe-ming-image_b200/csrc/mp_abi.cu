@@ -2043,7 +2043,7 @@ mp::RankParams rank_params(const mp_ctx* c, const RequestsLaunch& ext, const voi
 int launch_ranks(mp_ctx* c, const RequestsLaunch& ext, mp::RankParams* r, cudaStream_t stream) {
   const mp::RequestPlan& pl = r->plan;
   const bool tiles = pl.m >= 16 * static_cast<int64_t>(pl.n_req) &&
-                     static_cast<double>(pl.m) * r->k * r->rp >= 4.0e8;
+                     static_cast<double>(pl.m) * r->k * r->rp >= 1.0e8;
   cudaError_t e;
   if (tiles) {
     if (!encode_2d(&r->tm_x, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, r->x, r->k, pl.m, static_cast<uint64_t>(r->ldx) * 2, 64,

@@ -118,6 +118,22 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
   }
 }
 
+// Place in a ring of `slots` mbarrier-guarded slots whose count is known at run
+// time only: slot and phase are stepped, not divided out of a running index (two
+// integer divisions a stage were a quarter of a one-thread role's loop).
+struct RingPos {
+  int slot = 0;
+  uint32_t phase = 0;  // parity of the slot's current use
+  int uses = 0;        // whole rounds before this one
+  __device__ __forceinline__ void next(int slots) {
+    if (++slot == slots) {
+      slot = 0;
+      phase ^= 1u;
+      ++uses;
+    }
+  }
+};
+
 // ---- TMA -------------------------------------------------------------------
 
 __device__ __forceinline__ void tma_prefetch_map(const CUtensorMap* map) {

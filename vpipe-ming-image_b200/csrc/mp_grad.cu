@@ -56,6 +56,7 @@ constexpr uint32_t kBoxBytes = kRows * 128;      // [64 rows][64 bf16]
 constexpr uint32_t kXBytes = 2 * kBoxBytes;      // the A operand
 constexpr uint32_t kCodeBytes = kRows * kTileF;  // a stage's codes
 constexpr int kMaxGradStages = 6;
+constexpr int kMaxGradSplits = 8;
 constexpr uint32_t kGradSmemMost = 226 * 1024;
 
 constexpr uint32_t kAllBarrier = 1;  // named barrier of the whole CTA
@@ -241,17 +242,17 @@ __device__ void convert(const GradParams& p, const GradSmem& sm, const GradGeo& 
   }
   // one answer for the warp, so that all of its lanes give up together
   auto wait_all = [&](uint32_t bar, uint32_t parity, uint32_t site) {
-    return __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity, sm.abort, site, p.wait_limit_ns)) != 0;
+    return __all_sync(0xFFFFFFFFu, mbar_wait<true>(bar, parity, sm.abort, site, p.wait_limit_ns)) != 0;
   };
-  int n = 0;
+  RingPos at_stage;
   for (int i = item0; i < p.items; i += step) {
     const Item item = item_of(p, i);
     const bool codes = item.mb->scale != nullptr;
     TileIter it(p.plan, item.a, rank, count);
     int t0, rows;
-    for (; it.next(t0, rows); ++n) {
-      const int s = n % geo.stages;
-      const uint32_t ph = (n / geo.stages) & 1u;
+    for (; it.next(t0, rows); at_stage.next(geo.stages)) {
+      const int s = at_stage.slot;
+      const uint32_t ph = at_stage.phase;
       // the tile has landed (so the stage's last MMAs are done)
       if (!wait_all(smem_u32(&sm.full[s]), ph, kSiteGradFull | s)) return;
       const uint32_t xs = sm.tiles + s * geo.stage_bytes, parts = xs + geo.parts_off;
@@ -381,7 +382,8 @@ __global__ void __launch_bounds__(kGradThreads<TASKS>, TASKS == 1 ? 2 : 1)
   pdl_release();
 
   if (warp == 0) {
-    int n = 0;
+    RingPos at_stage;
+    int sent = 0;
     bool ok = true;
     for (int i = item0; i < p.items && ok; i += step) {
       const Item item = item_of(p, i);
@@ -389,11 +391,11 @@ __global__ void __launch_bounds__(kGradThreads<TASKS>, TASKS == 1 ? 2 : 1)
       const bool codes = mb.scale != nullptr;
       TileIter it(p.plan, item.a, rank, count);
       int t0, rows;
-      for (; ok && it.next(t0, rows); ++n) {
-        const int s = n % geo.stages;
-        if (n >= geo.stages)
-          ok = __all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&sm.empty[s]), ((n / geo.stages) & 1u) ^ 1u, sm.abort,
-                                                 kSiteGradEmpty | s, p.wait_limit_ns)) != 0;
+      for (; ok && it.next(t0, rows); at_stage.next(geo.stages), ++sent) {
+        const int s = at_stage.slot;
+        if (at_stage.uses > 0)
+          ok = __all_sync(0xFFFFFFFFu, mbar_wait<true>(smem_u32(&sm.empty[s]), at_stage.phase ^ 1u, sm.abort,
+                                                       kSiteGradEmpty | s, p.wait_limit_ns)) != 0;
         if (!ok) break;
         const uint32_t bar = smem_u32(&sm.full[s]), xs = sm.tiles + s * geo.stage_bytes;
         if (lane == 0) {
@@ -416,7 +418,7 @@ __global__ void __launch_bounds__(kGradThreads<TASKS>, TASKS == 1 ? 2 : 1)
     if (*sm.abort != 0u && lane == 0) {
       // copies in flight land (bounded) before the CTA leaves
       const uint64_t since = global_timer_ns();
-      for (int j = max(0, n - geo.stages); j < n; ++j)
+      for (int j = max(0, sent - geo.stages); j < sent; ++j)
         while (!mbar_try_wait(smem_u32(&sm.full[j % geo.stages]), (j / geo.stages) & 1u))
           if (global_timer_ns() - since > p.wait_limit_ns) break;
     }
@@ -424,19 +426,19 @@ __global__ void __launch_bounds__(kGradThreads<TASKS>, TASKS == 1 ? 2 : 1)
     if (lane == 0) {
       const uint32_t mn = (1u << 15) | (1u << 16);  // both operands MN-major
       const uint32_t id1 = make_idesc_bf16(kTileF, pc.n1) | mn, id2 = make_idesc_bf16(kTileF, pc.n2) | mn;
-      int n = 0, chunk = 0;  // stages and accumulators filled
+      RingPos at_stage, at_acc;  // stages and accumulators filled
       bool ok = true;
       for (int i = item0; i < p.items && ok; i += step) {
         const int tiles = TileIter(p.plan, item_of(p, i).a, rank, count).total();
-        for (int k = 0; k < tiles; ++k, ++n) {
-          const int s = n % geo.stages, b = chunk % pc.bufs, use = chunk / pc.bufs;
-          const uint32_t ph = (n / geo.stages) & 1u;
+        for (int k = 0; k < tiles; ++k, at_stage.next(geo.stages)) {
+          const int s = at_stage.slot, b = at_acc.slot;
+          const uint32_t ph = at_stage.phase;
           const bool first = k % kChunk == 0, last = k % kChunk == kChunk - 1 || k == tiles - 1;
-          if (first && use > 0)
-            ok = mbar_wait(smem_u32(&sm.taken[b]), (use - 1) & 1u, sm.abort, kSiteGradTaken | b, p.wait_limit_ns);
+          if (first && at_acc.uses > 0)
+            ok = mbar_wait<true>(smem_u32(&sm.taken[b]), at_acc.phase ^ 1u, sm.abort, kSiteGradTaken | b, p.wait_limit_ns);
           // the converting warps arrive after the tile has landed
-          ok = ok && mbar_wait(smem_u32(&sm.full[s]), ph, sm.abort, kSiteGradFull | s, p.wait_limit_ns) &&
-               mbar_wait(smem_u32(&sm.conv[s]), ph, sm.abort, kSiteGradConv | s, p.wait_limit_ns);
+          ok = ok && mbar_wait<true>(smem_u32(&sm.full[s]), ph, sm.abort, kSiteGradFull | s, p.wait_limit_ns) &&
+               mbar_wait<true>(smem_u32(&sm.conv[s]), ph, sm.abort, kSiteGradConv | s, p.wait_limit_ns);
           if (!ok) break;
           tc_fence_after();
           const uint32_t xs = sm.tiles + s * geo.stage_bytes, us = xs + geo.parts_off, d = tmem + b * pc.cols;
@@ -450,7 +452,7 @@ __global__ void __launch_bounds__(kGradThreads<TASKS>, TASKS == 1 ? 2 : 1)
           umma_commit(smem_u32(&sm.empty[s]));
           if (last) {
             umma_commit(smem_u32(&sm.sum[b]));
-            ++chunk;
+            at_acc.next(pc.bufs);
           }
         }
       }
@@ -468,17 +470,17 @@ __global__ void __launch_bounds__(kGradThreads<TASKS>, TASKS == 1 ? 2 : 1)
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const int f = (warp & 3) * 32 + lane;
     float sums[kSumCols<TASKS>];  // one feature, consecutive ranks
-    int chunk = 0;
+    RingPos at_acc;
     bool ok = true;
     for (int i = item0; i < p.items && ok; i += step) {
       const Item item = item_of(p, i);
       const int tiles = TileIter(p.plan, item.a, rank, count).total();
 #pragma unroll
       for (int c = 0; c < kSumCols<TASKS>; ++c) sums[c] = 0.0f;
-      for (int k = 0; k < tiles; k += kChunk, ++chunk) {
-        const int b = chunk % pc.bufs;
-        ok = __all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&sm.sum[b]), (chunk / pc.bufs) & 1u, sm.abort,
-                                               kSiteGradSum | b, p.wait_limit_ns)) != 0;
+      for (int k = 0; k < tiles; k += kChunk, at_acc.next(pc.bufs)) {
+        const int b = at_acc.slot;
+        ok = __all_sync(0xFFFFFFFFu, mbar_wait<true>(smem_u32(&sm.sum[b]), at_acc.phase, sm.abort, kSiteGradSum | b,
+                                                     p.wait_limit_ns)) != 0;
         if (!ok) break;
         tc_fence_after();
 #pragma unroll
@@ -549,8 +551,14 @@ __global__ void __launch_bounds__(kGradThreads<TASKS>, TASKS == 1 ? 2 : 1)
       const uint32_t ex = smem_u32(sm.exchange);
       auto sum_at = [&](int r, int f) {
         const uint32_t at = ex + static_cast<uint32_t>(r * ld + f) * 4u;
-        float s = ld_cluster_f32(mapa_shared(at, 0));
-        for (int z = 1; z < count; ++z) s += ld_cluster_f32(mapa_shared(at, z));
+        float o[kMaxGradSplits];  // all in flight, then added in CTA order
+#pragma unroll
+        for (int z = 0; z < kMaxGradSplits; ++z)
+          if (z < count) o[z] = ld_cluster_f32(mapa_shared(at, z));
+        float s = o[0];
+#pragma unroll
+        for (int z = 1; z < kMaxGradSplits; ++z)
+          if (z < count) s += o[z];
         return s;
       };
       if (mb.rank_major) {
@@ -615,7 +623,7 @@ cudaError_t launch_adapter_grad(const GradParams& p, cudaStream_t stream) {
   const int rows = (p.plan.m + used - 1) / used;
   const int room = 148 * (geo.smem <= 113 * 1024 ? 2 : 1);
   q.splits = 1;
-  while (q.splits < 8 && static_cast<long long>(q.tiles) * used * q.splits < room && rows > 4 * kRows * q.splits)
+  while (q.splits < kMaxGradSplits && static_cast<long long>(q.tiles) * used * q.splits < room && rows > 4 * kRows * q.splits)
     q.splits *= 2;
   const unsigned grid = q.splits > 1 ? static_cast<unsigned>(q.items) * q.splits
                                      : static_cast<unsigned>(q.items < room ? q.items : room);

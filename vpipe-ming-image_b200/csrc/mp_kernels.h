@@ -207,7 +207,7 @@ struct BankSetParams {
 struct RankParams {
   CUtensorMap tm_x;   // x (box {64, 128}, SW128), rank_tiles_kernel only
   CUtensorMap tm_f;   // F as [cap * rp, k] (box {64, rp}, SW128)
-  int32_t splits;     // CTAs that share K (set by the launch)
+  int32_t splits, units;  // CTAs that share K, and 128-row units (set by the launch)
   const uint16_t* x;  // bf16 [m][ldx]
   int64_t ldx;
   const uint16_t* f;  // bf16 [cap][rp][fp]

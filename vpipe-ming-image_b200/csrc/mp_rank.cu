@@ -5,12 +5,18 @@
 // (A in the forward pass, B^T in the backward pass). Bound by reading x once: 2 r
 // operations for every two bytes.
 //
-// A cluster takes up to 128 rows of one block of the plan (the rows of one
-// request in one token tile); its CTAs share K and add their sums through
-// distributed shared memory, in CTA order. D[row][rank] = x F^T, both operands by
-// TMA with the 128-byte swizzle, rows past the request's included: D's rows are
-// independent, theirs are not used. As in mp_grad.cu an accumulator takes kChunk
-// stages and is then added, in f32 with rounding to nearest, to sums in registers.
+// A unit is up to 128 rows of one block of the plan (the rows of one request in
+// one token tile). D[row][rank] = x F^T, both operands by TMA with the 128-byte
+// swizzle, rows past the request's included: D's rows are independent, theirs are
+// not used. As in mp_grad.cu an accumulator takes kChunk stages and is then added,
+// in f32 with rounding to nearest, to sums in registers.
+//
+// With few units a cluster takes one, its CTAs share K and add their sums through
+// distributed shared memory, in CTA order; with many, persistent CTAs walk them.
+// (A few CTAs on the SMs that the projection beside them leaves idle would hide
+// the whole launch, but one CTA needs 0.35 us a 64-wide stage, 65 cycles an MMA
+// with 64 ranks, and the projection then waits for it: 4352 rows took 158 us, not
+// 127.)
 //
 // The block is written whole (zeros in the rows of other requests and past rp):
 // the projection kernel takes it as the appended K tiles' operand.
@@ -26,7 +32,8 @@ namespace {
 constexpr int kTileRows = 128;  // MMA M
 constexpr int kChunk = 4;       // 64-wide stages of an accumulator
 constexpr uint32_t kXBytes = kTileRows * 128;
-constexpr int kMaxStages = 8;
+constexpr int kMaxStages = 10;
+constexpr int kMaxRankSplits = 8;
 constexpr int kSumWarp0 = 2;
 constexpr int kRankThreads = 32 * (kSumWarp0 + 4);
 constexpr uint32_t kAllBarrier = 1;
@@ -48,7 +55,7 @@ struct RankGeo {
 __host__ __device__ inline RankGeo rank_geo(int rp) {
   RankGeo g;
   g.stage_bytes = kXBytes + (static_cast<uint32_t>(rp) * 128u + 1023u) / 1024u * 1024u;
-  const uint32_t room = rp <= 64 ? 104 * 1024 : 200 * 1024;
+  const uint32_t room = (rp <= 64 ? 104 : 224) * 1024;
   g.stages = static_cast<int>(room / g.stage_bytes);
   if (g.stages > kMaxStages) g.stages = kMaxStages;
   const uint32_t tiles = g.stages * g.stage_bytes, exchange = kTileRows * (rp + 4) * 4;
@@ -65,12 +72,43 @@ __device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
   return v;
 }
 
+struct RankUnit {
+  int blk, sub;   // block of the plan, 128-row part of it
+  int row0;       // first row of x
+  int lo, hi;     // the request's rows in the part
+  int adapter;
+  bool used, work;
+};
+
+__device__ __forceinline__ RankUnit rank_unit(const RankParams& p, int unit) {
+  const int tile_rows = 64 << p.lvl, subs = tile_rows > kTileRows ? tile_rows / kTileRows : 1;
+  RankUnit u;
+  u.blk = unit / subs;
+  u.sub = unit - u.blk * subs;
+  const int4 ent = p.plan.block[p.lvl][u.blk];  // {tile, first row, row past the last, adapter}
+  u.adapter = ent.w;
+  u.used = ent.w >= 0;
+  u.row0 = ent.x * tile_rows + u.sub * kTileRows;
+  u.lo = max(ent.y, u.row0) - u.row0;
+  u.hi = min(ent.z, u.row0 + min(kTileRows, tile_rows)) - u.row0;
+  u.work = u.used && u.lo < u.hi;
+  return u;
+}
+
+// The request's strength; NaN with a factor that is not finite (it is stored as
+// zeros, and its request's rows are NaN).
+__device__ __forceinline__ float unit_scale(const RankParams& p, const RankUnit& u) {
+  return p.bad[u.adapter] != 0 ? __int_as_float(0x7FC00000) : p.plan.block_s[p.lvl][u.blk];
+}
+
 // COLS: rp rounded up to 32, 64 or 128, the sums a thread holds (one row each).
 template <int COLS>
 __global__ void __launch_bounds__(kRankThreads, COLS <= 64 ? 2 : 1) rank_tiles_kernel(const __grid_constant__ RankParams p) {
   extern __shared__ uint8_t rank_raw[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int rank = static_cast<int>(cluster_ctarank()), count = p.splits;
+  const int count = p.splits, rank = count > 1 ? static_cast<int>(cluster_ctarank()) : 0;
+  const int unit0 = static_cast<int>(blockIdx.x) / count, step = static_cast<int>(gridDim.x) / count;
+  const int rows = min(kTileRows, 64 << p.lvl);  // of a unit
   const RankGeo geo = rank_geo(p.rp);
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(rank_raw) + 1023u) & ~uintptr_t(1023u));
   const uint32_t tiles = smem_u32(base);
@@ -79,6 +117,26 @@ __global__ void __launch_bounds__(kRankThreads, COLS <= 64 ? 2 : 1) rank_tiles_k
            *done = sum + 4;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
   volatile uint32_t* abort = tmem_slot + 1;
+  pdl_wait();
+  pdl_release();
+
+  // first row of unit u's part of its block
+  auto block_row = [&](const RankUnit& u) {
+    return p.vblk + ((static_cast<int64_t>(u.blk) << (6 + p.lvl)) + u.sub * kTileRows) * p.ldb;
+  };
+  if (count > 1) {
+    // Whole clusters leave here, before any set-up: most of the grid's units have
+    // nothing of the block's request, or the block is not used at all.
+    const RankUnit u = rank_unit(p, unit0);
+    if (!u.work) {
+      if (u.used && p.vblk != nullptr) {
+        uint4* at = reinterpret_cast<uint4*>(block_row(u));
+        for (int e = rank * kRankThreads + threadIdx.x; e < rows * p.ldb / 8; e += count * kRankThreads)
+          at[e] = make_uint4(0, 0, 0, 0);
+      }
+      return;
+    }
+  }
   if (threadIdx.x == 0) {
     for (int s = 0; s < geo.stages; ++s) {
       mbar_init(smem_u32(&full[s]), 1);
@@ -102,60 +160,65 @@ __global__ void __launch_bounds__(kRankThreads, COLS <= 64 ? 2 : 1) rank_tiles_k
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  pdl_wait();
-  pdl_release();
 
-  // this cluster's rows: part `sub` of a block of 64 << lvl rows
-  const int tile_rows = 64 << p.lvl, subs = tile_rows > kTileRows ? tile_rows / kTileRows : 1;
-  const int unit = static_cast<int>(blockIdx.x) / count, blk = unit / subs, sub = unit % subs;
-  const int4 ent = p.plan.block[p.lvl][blk];  // {tile, first row, row past the last, adapter}
-  const bool used = ent.w >= 0;
-  const int row0 = ent.x * tile_rows + sub * kTileRows, rows = min(kTileRows, tile_rows);
-  const int lo = max(ent.y, row0) - row0, hi = min(ent.z, row0 + rows) - row0;  // the request's rows here
-  const bool work = used && lo < hi;
   // K stages of this CTA
   const int all = (p.k + 63) / 64, per = (all + count - 1) / count;
-  const int kt0 = min(rank * per, all), n_kt = work ? min(kt0 + per, all) - kt0 : 0;
+  const int kt0 = min(rank * per, all), n_kt = min(kt0 + per, all) - kt0;
 
   if (warp == 0) {
     if (lane == 0) {
+      RingPos at_stage;
       int sent = 0;
-      for (int n = 0; n < n_kt; ++n) {
-        const int s = n % geo.stages;
-        if (n >= geo.stages && !mbar_wait(smem_u32(&empty[s]), ((n / geo.stages) & 1u) ^ 1u, abort,
-                                          kSiteRankEmpty | s, p.wait_limit_ns))
-          break;
-        const uint32_t bar = smem_u32(&full[s]), at = tiles + s * geo.stage_bytes;
-        mbar_arrive_expect_tx(bar, kXBytes + static_cast<uint32_t>(p.rp) * 128u);
-        tma_load_2d(at, &p.tm_x, bar, (kt0 + n) * 64, row0);
-        tma_load_2d(at + kXBytes, &p.tm_f, bar, (kt0 + n) * 64, ent.w * p.rp);
-        sent = n + 1;
+      bool ok = true;
+      for (int unit = unit0; unit < p.units && ok; unit += step) {
+        const RankUnit u = rank_unit(p, unit);
+        if (!u.work) continue;
+        for (int k = 0; k < n_kt; ++k, at_stage.next(geo.stages), ++sent) {
+          const int s = at_stage.slot;
+          if (at_stage.uses > 0)
+            ok = mbar_wait<true>(smem_u32(&empty[s]), at_stage.phase ^ 1u, abort, kSiteRankEmpty | s, p.wait_limit_ns);
+          if (!ok) break;
+          const uint32_t bar = smem_u32(&full[s]), at = tiles + s * geo.stage_bytes;
+          mbar_arrive_expect_tx(bar, kXBytes + static_cast<uint32_t>(p.rp) * 128u);
+          tma_load_2d(at, &p.tm_x, bar, (kt0 + k) * 64, u.row0);
+          tma_load_2d(at + kXBytes, &p.tm_f, bar, (kt0 + k) * 64, u.adapter * p.rp);
+        }
       }
       if (*abort != 0u) {
         // copies in flight land (bounded) before the CTA leaves
         const uint64_t since = global_timer_ns();
-        for (int n = max(0, sent - geo.stages); n < sent; ++n)
-          while (!mbar_try_wait(smem_u32(&full[n % geo.stages]), (n / geo.stages) & 1u))
+        for (int j = max(0, sent - geo.stages); j < sent; ++j)
+          while (!mbar_try_wait(smem_u32(&full[j % geo.stages]), (j / geo.stages) & 1u))
             if (global_timer_ns() - since > p.wait_limit_ns) break;
       }
     }
   } else if (warp == 1) {
-    if (lane == 0 && n_kt > 0) {
+    if (lane == 0) {
       const uint32_t idesc = make_idesc_bf16(kTileRows, p.rp);
-      for (int n = 0; n < n_kt; ++n) {
-        const int s = n % geo.stages, chunk = n / kChunk, b = chunk & 1;
-        if (n % kChunk == 0 && chunk >= 2 &&
-            !mbar_wait(smem_u32(&taken[b]), ((chunk >> 1) - 1) & 1u, abort, kSiteRankTaken | b, p.wait_limit_ns))
-          break;
-        if (!mbar_wait(smem_u32(&full[s]), (n / geo.stages) & 1u, abort, kSiteRankFull | s, p.wait_limit_ns)) break;
-        tc_fence_after();
-        const uint32_t xs = tiles + s * geo.stage_bytes, fs = xs + kXBytes;
+      RingPos at_stage;
+      int chunk = 0;
+      bool ok = true;
+      for (int unit = unit0; unit < p.units && ok; unit += step) {
+        if (!rank_unit(p, unit).work) continue;
+        for (int k = 0; k < n_kt; ++k, at_stage.next(geo.stages)) {
+          const int s = at_stage.slot, b = chunk & 1;
+          const bool first = k % kChunk == 0, last = k % kChunk == kChunk - 1 || k == n_kt - 1;
+          if (first && chunk >= 2)
+            ok = mbar_wait<true>(smem_u32(&taken[b]), ((chunk >> 1) - 1) & 1u, abort, kSiteRankTaken | b, p.wait_limit_ns);
+          ok = ok && mbar_wait<true>(smem_u32(&full[s]), at_stage.phase, abort, kSiteRankFull | s, p.wait_limit_ns);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t xs = tiles + s * geo.stage_bytes, fs = xs + kXBytes;
 #pragma unroll
-        for (int kk = 0; kk < 4; ++kk)
-          umma_ss(tmem + b * COLS, make_sdesc_sw128(xs + kk * 32), make_sdesc_sw128(fs + kk * 32), idesc,
-                  n % kChunk != 0 || kk > 0 ? 1u : 0u);
-        umma_commit(smem_u32(&empty[s]));
-        if (n % kChunk == kChunk - 1 || n == n_kt - 1) umma_commit(smem_u32(&sum[b]));
+          for (int kk = 0; kk < 4; ++kk)
+            umma_ss(tmem + b * COLS, make_sdesc_sw128(xs + kk * 32), make_sdesc_sw128(fs + kk * 32), idesc,
+                    !first || kk > 0 ? 1u : 0u);
+          umma_commit(smem_u32(&empty[s]));
+          if (last) {
+            umma_commit(smem_u32(&sum[b]));
+            ++chunk;
+          }
+        }
       }
       umma_commit(smem_u32(done));
       const uint64_t since = global_timer_ns();
@@ -166,32 +229,59 @@ __global__ void __launch_bounds__(kRankThreads, COLS <= 64 ? 2 : 1) rank_tiles_k
         }
     }
   } else {
-    const int q = warp & 3;
+    const int q = warp & 3, r = q * 32 + lane;  // this thread's row of a unit
     float sums[COLS];
+    int chunk = 0;
+    bool ok = true;
+    for (int unit = unit0; unit < p.units && ok; unit += step) {
+      const RankUnit u = rank_unit(p, unit);
+      if (!u.used) continue;
 #pragma unroll
-    for (int c = 0; c < COLS; ++c) sums[c] = 0.0f;
-    for (int chunk = 0; chunk * kChunk < n_kt; ++chunk) {
-      const int b = chunk & 1;
-      if (!__all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&sum[b]), (chunk >> 1) & 1u, abort, kSiteRankSum | b,
-                                             p.wait_limit_ns)))
-        break;
-      tc_fence_after();
+      for (int c = 0; c < COLS; ++c) sums[c] = 0.0f;
+      for (int k = 0; u.work && k < n_kt; k += kChunk, ++chunk) {
+        const int b = chunk & 1;
+        ok = __all_sync(0xFFFFFFFFu, mbar_wait<true>(smem_u32(&sum[b]), (chunk >> 1) & 1u, abort, kSiteRankSum | b,
+                                               p.wait_limit_ns)) != 0;
+        if (!ok) break;
+        tc_fence_after();
 #pragma unroll
-      for (int c = 0; c < COLS; c += 16) {
-        if (c >= p.rp) break;
-        uint32_t v[16];
-        MP_TMEM_LD_32X32B_X16(tmem + (static_cast<uint32_t>(q * 32) << 16) + b * COLS + c, v);
-        MP_TMEM_WAIT_LD_REGS16(v);
+        for (int c = 0; c < COLS; c += 16) {
+          if (c >= p.rp) break;
+          uint32_t v[16];
+          MP_TMEM_LD_32X32B_X16(tmem + (static_cast<uint32_t>(q * 32) << 16) + b * COLS + c, v);
+          MP_TMEM_WAIT_LD_REGS16(v);
 #pragma unroll
-        for (int j = 0; j < 16; ++j) sums[c + j] += __uint_as_float(v[j]);
+          for (int j = 0; j < 16; ++j) sums[c + j] += __uint_as_float(v[j]);
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&taken[b]));
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&taken[b]));
+      if (count > 1 || !ok) break;  // a cluster has one unit
+      if (r >= rows) continue;
+      const bool mine = r >= u.lo && r < u.hi;
+      const float scale = unit_scale(p, u);
+#pragma unroll
+      for (int c = 0; c < COLS; ++c) sums[c] = mine ? sums[c] * scale : 0.0f;
+      if (mine && p.v32 != nullptr) {
+        float* at = p.v32 + static_cast<int64_t>(u.row0 + r) * p.ld32;
+#pragma unroll
+        for (int c = 0; c < COLS; c += 4)
+          if (c < p.rp) *reinterpret_cast<float4*>(at + c) = make_float4(sums[c], sums[c + 1], sums[c + 2], sums[c + 3]);
+      }
+      if (p.vblk != nullptr) {
+        uint16_t* at = block_row(u) + static_cast<int64_t>(r) * p.ldb;
+#pragma unroll
+        for (int c = 0; c < COLS; c += 8)
+          *reinterpret_cast<uint4*>(at + c) =
+              make_uint4(pack_bf16x2(sums[c], sums[c + 1]), pack_bf16x2(sums[c + 2], sums[c + 3]),
+                         pack_bf16x2(sums[c + 4], sums[c + 5]), pack_bf16x2(sums[c + 6], sums[c + 7]));
+        for (int c = COLS; c < p.ldb; c += 8) *reinterpret_cast<uint4*>(at + c) = make_uint4(0, 0, 0, 0);
+      }
     }
     named_barrier(kAllBarrier, kRankThreads);  // copies landed, MMAs done: the stages' memory is free
-    if (work) {
-      float* row = reinterpret_cast<float*>(base) + (q * 32 + lane) * (p.rp + 4);
+    if (count > 1) {
+      float* row = reinterpret_cast<float*>(base) + r * (p.rp + 4);
 #pragma unroll
       for (int c = 0; c < COLS; c += 4)
         if (c < p.rp) *reinterpret_cast<float4*>(row + c) = make_float4(sums[c], sums[c + 1], sums[c + 2], sums[c + 3]);
@@ -200,50 +290,53 @@ __global__ void __launch_bounds__(kRankThreads, COLS <= 64 ? 2 : 1) rank_tiles_k
   __syncwarp();
   if (warp < kSumWarp0) named_barrier(kAllBarrier, kRankThreads);
   const bool aborted = *abort != 0u;
-  cluster_sync();
-  if (used && !aborted) {
-    // each CTA adds up and writes its share of the rows
-    float scale = p.plan.block_s[p.lvl][blk];
-    // a factor that is not finite is stored as zeros; its request's rows are NaN
-    if (p.bad[ent.w] != 0) scale = __int_as_float(0x7FC00000);
-    const int share = (rows + count - 1) / count, first = rank * share, last = min(first + share, rows);
-    const int quads = (p.vblk != nullptr ? p.ldb : p.rp) / 4;
-    const uint32_t ld = static_cast<uint32_t>(p.rp + 4) * 4u;
-    for (int e = first * quads + threadIdx.x; e < last * quads; e += kRankThreads) {
-      const int r = e / quads, c = e % quads * 4;
-      float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      const bool mine = work && r >= lo && r < hi && c < p.rp;
-      if (mine) {
-        const uint32_t at = tiles + r * ld + c * 4u;
-        s = ld_cluster_f4(mapa_shared(at, 0));
-        for (int z = 1; z < count; ++z) {
-          const float4 o = ld_cluster_f4(mapa_shared(at, z));
-          s.x += o.x, s.y += o.y, s.z += o.z, s.w += o.w;
+  if (count > 1) {
+    cluster_sync();
+    if (!aborted) {
+      // each CTA adds up and writes its share of the rows
+      const RankUnit u = rank_unit(p, unit0);
+      const float scale = unit_scale(p, u);
+      const int share = (rows + count - 1) / count, first = rank * share, last = min(first + share, rows);
+      const int quads = (p.vblk != nullptr ? p.ldb : p.rp) / 4;
+      const uint32_t ld = static_cast<uint32_t>(p.rp + 4) * 4u;
+      for (int e = first * quads + threadIdx.x; e < last * quads; e += kRankThreads) {
+        const int r = e / quads, c = e % quads * 4;
+        float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (r >= u.lo && r < u.hi && c < p.rp) {
+          const uint32_t at = tiles + r * ld + c * 4u;
+          float4 o[kMaxRankSplits];  // all in flight, then added in CTA order
+#pragma unroll
+          for (int z = 0; z < kMaxRankSplits; ++z)
+            if (z < count) o[z] = ld_cluster_f4(mapa_shared(at, z));
+          s = o[0];
+#pragma unroll
+          for (int z = 1; z < kMaxRankSplits; ++z)
+            if (z < count) s.x += o[z].x, s.y += o[z].y, s.z += o[z].z, s.w += o[z].w;
+          s.x *= scale, s.y *= scale, s.z *= scale, s.w *= scale;
+          if (p.v32 != nullptr) *reinterpret_cast<float4*>(p.v32 + static_cast<int64_t>(u.row0 + r) * p.ld32 + c) = s;
         }
-        s.x *= scale, s.y *= scale, s.z *= scale, s.w *= scale;
-        if (p.v32 != nullptr) *reinterpret_cast<float4*>(p.v32 + static_cast<int64_t>(row0 + r) * p.ld32 + c) = s;
-      }
-      if (p.vblk != nullptr) {
-        const int64_t at = static_cast<int64_t>(blk) * tile_rows + sub * kTileRows + r;
-        *reinterpret_cast<uint2*>(p.vblk + at * p.ldb + c) =
-            make_uint2(pack_bf16x2(s.x, s.y), pack_bf16x2(s.z, s.w));
+        if (p.vblk != nullptr)
+          *reinterpret_cast<uint2*>(block_row(u) + static_cast<int64_t>(r) * p.ldb + c) =
+              make_uint2(pack_bf16x2(s.x, s.y), pack_bf16x2(s.z, s.w));
       }
     }
+    cluster_sync();  // no CTA leaves while another reads its sums
+  } else {
+    __syncthreads();
   }
-  cluster_sync();  // no CTA leaves while another reads its sums
   tc_fence_after();
   if (warp == 1) tmem_dealloc(tmem, 2 * COLS);
   if (threadIdx.x == 0 && aborted) atomicOr(p.err, kErrTimeout);
 }
 
 template <int COLS>
-cudaError_t launch_cols(const RankParams& p, unsigned clusters, cudaStream_t stream) {
+cudaError_t launch_cols(const RankParams& p, unsigned ctas, cudaStream_t stream) {
   const uint32_t smem = rank_geo(p.rp).smem;
   cudaError_t e = cudaFuncSetAttribute(rank_tiles_kernel<COLS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                        static_cast<int>(smem));
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(clusters * p.splits);
+  cfg.gridDim = dim3(ctas);
   cfg.blockDim = dim3(kRankThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
@@ -263,18 +356,21 @@ cudaError_t launch_cols(const RankParams& p, unsigned clusters, cudaStream_t str
 
 cudaError_t launch_rank_tiles(const RankParams& p, cudaStream_t stream) {
   RankParams q = p;
-  const int blocks = plan_blocks(p.plan.m, p.plan.n_req, p.lvl), tile_rows = 64 << p.lvl;
-  const int subs = tile_rows > kTileRows ? tile_rows / kTileRows : 1;
-  if (blocks == 0) return cudaSuccess;
-  // K splits: until the row parts with work (about one per 128 rows and one
-  // more per request) times the splits fill the SMs, each with four stages
+  const int tile_rows = 64 << p.lvl, subs = tile_rows > kTileRows ? tile_rows / kTileRows : 1;
+  q.units = plan_blocks(p.plan.m, p.plan.n_req, p.lvl) * subs;
+  // K splits: until the units with work (about one per 128 rows and one more per
+  // request) times the splits take most SMs, each with four stages. More cost more
+  // than they bring: m 4352, k 3840 in one request takes 21.8 us with 8 splits,
+  // 16.1 with 4.
   const int parts = (p.plan.m + kTileRows - 1) / kTileRows + p.plan.n_req, stages = (p.k + 63) / 64;
   q.splits = 1;
-  while (q.splits < 8 && parts * q.splits < 148 && stages >= 8 * q.splits) q.splits *= 2;
-  const unsigned clusters = static_cast<unsigned>(blocks) * subs;
-  if (p.rp <= 32) return launch_cols<32>(q, clusters, stream);
-  if (p.rp <= 64) return launch_cols<64>(q, clusters, stream);
-  return launch_cols<128>(q, clusters, stream);
+  while (q.splits < kMaxRankSplits && parts * q.splits < 100 && stages >= 8 * q.splits) q.splits *= 2;
+  const int room = 148 * (p.rp <= 64 ? 2 : 1);  // CTAs resident at once
+  const unsigned ctas = q.splits > 1 ? static_cast<unsigned>(q.units) * q.splits
+                                     : static_cast<unsigned>(q.units < room ? q.units : room);
+  if (p.rp <= 32) return launch_cols<32>(q, ctas, stream);
+  if (p.rp <= 64) return launch_cols<64>(q, ctas, stream);
+  return launch_cols<128>(q, ctas, stream);
 }
 
 }  // namespace mp
