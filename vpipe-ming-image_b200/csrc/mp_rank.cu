@@ -5,8 +5,8 @@
 // (A in the forward pass, B^T in the backward pass). Bound by reading x once: 2 r
 // operations for every two bytes.
 //
-// A unit is up to 128 rows of one block of the plan (the rows of one request in
-// one token tile). D[row][rank] = x F^T, both operands by TMA with the 128-byte
+// A unit is the rows of one request in one tile of 128 rows (64 where the blocks
+// are that high). D[row][rank] = x F^T, both operands by TMA with the 128-byte
 // swizzle, rows past the request's included: D's rows are independent, theirs are
 // not used. As in mp_grad.cu an accumulator takes kChunk stages and is then added,
 // in f32 with rounding to nearest, to sums in registers.
@@ -73,32 +73,58 @@ __device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
 }
 
 struct RankUnit {
-  int blk, sub;   // block of the plan, 128-row part of it
+  int unit;       // block of the plan at the units' level
   int row0;       // first row of x
-  int lo, hi;     // the request's rows in the part
+  int lo, hi;     // the request's rows, from row0
   int adapter;
-  bool used, work;
+  bool work;
+  int64_t out;    // row of vblk for row0
+  int zero0, zero1, zero2, zero3;  // rows of vblk to clear besides: [zero0, zero1) and [zero2, zero3), from `out`
 };
 
-__device__ __forceinline__ RankUnit rank_unit(const RankParams& p, int unit) {
-  const int tile_rows = 64 << p.lvl, subs = tile_rows > kTileRows ? tile_rows / kTileRows : 1;
+__device__ __forceinline__ int unit_level(const RankParams& p) { return p.lvl > 0 ? 1 : 0; }
+
+// Unit i is block i of level 0 or 1 of the plan. The unit with the request's
+// first (last) row in a block of 64 << lvl rows clears the block's rows before
+// (after) its own 128, too.
+__device__ __forceinline__ RankUnit rank_unit(const RankParams& p, int i) {
+  const int ul = unit_level(p);
   RankUnit u;
-  u.blk = unit / subs;
-  u.sub = unit - u.blk * subs;
-  const int4 ent = p.plan.block[p.lvl][u.blk];  // {tile, first row, row past the last, adapter}
+  u.unit = i;
+  const int4 ent = p.plan.block[ul][i];  // {tile, first row, row past the last, adapter}
   u.adapter = ent.w;
-  u.used = ent.w >= 0;
-  u.row0 = ent.x * tile_rows + u.sub * kTileRows;
-  u.lo = max(ent.y, u.row0) - u.row0;
-  u.hi = min(ent.z, u.row0 + min(kTileRows, tile_rows)) - u.row0;
-  u.work = u.used && u.lo < u.hi;
+  u.work = ent.w >= 0;
+  u.row0 = ent.x << (6 + ul);
+  u.lo = ent.y - u.row0;
+  u.hi = ent.z - u.row0;
+  u.zero0 = u.zero1 = u.zero2 = u.zero3 = 0;
+  u.out = 0;
+  if (u.work && p.vblk != nullptr) {
+    const int tile = u.row0 >> (6 + p.lvl), blk = tile + (i - ent.x);  // i - ent.x: the request
+    const int in = u.row0 - (tile << (6 + p.lvl));                     // the unit's place in the block
+    u.out = (static_cast<int64_t>(blk) << (6 + p.lvl)) + in;
+    if (p.lvl > 1) {
+      const int4 whole = p.plan.block[p.lvl][blk];
+      if (whole.y == ent.y) u.zero0 = -in;
+      if (whole.z == ent.z) u.zero2 = kTileRows, u.zero3 = (64 << p.lvl) - in;
+    }
+  }
   return u;
 }
 
 // The request's strength; NaN with a factor that is not finite (it is stored as
 // zeros, and its request's rows are NaN).
 __device__ __forceinline__ float unit_scale(const RankParams& p, const RankUnit& u) {
-  return p.bad[u.adapter] != 0 ? __int_as_float(0x7FC00000) : p.plan.block_s[p.lvl][u.blk];
+  return p.bad[u.adapter] != 0 ? __int_as_float(0x7FC00000) : p.plan.block_s[unit_level(p)][u.unit];
+}
+
+// The unit's rows of vblk outside its 128, by threads `tid` of `threads`.
+__device__ __forceinline__ void clear_rows(const RankParams& p, const RankUnit& u, int tid, int threads) {
+  if (p.vblk == nullptr) return;
+  const int per_row = p.ldb / 8;
+  uint4* at = reinterpret_cast<uint4*>(p.vblk + u.out * p.ldb);
+  for (int e = u.zero0 * per_row + tid; e < u.zero1 * per_row; e += threads) at[e] = make_uint4(0, 0, 0, 0);
+  for (int e = u.zero2 * per_row + tid; e < u.zero3 * per_row; e += threads) at[e] = make_uint4(0, 0, 0, 0);
 }
 
 // COLS: rp rounded up to 32, 64 or 128, the sums a thread holds (one row each).
@@ -108,7 +134,7 @@ __global__ void __launch_bounds__(kRankThreads, COLS <= 64 ? 2 : 1) rank_tiles_k
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int count = p.splits, rank = count > 1 ? static_cast<int>(cluster_ctarank()) : 0;
   const int unit0 = static_cast<int>(blockIdx.x) / count, step = static_cast<int>(gridDim.x) / count;
-  const int rows = min(kTileRows, 64 << p.lvl);  // of a unit
+  const int rows = 64 << unit_level(p);  // of a unit
   const RankGeo geo = rank_geo(p.rp);
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(rank_raw) + 1023u) & ~uintptr_t(1023u));
   const uint32_t tiles = smem_u32(base);
@@ -117,26 +143,6 @@ __global__ void __launch_bounds__(kRankThreads, COLS <= 64 ? 2 : 1) rank_tiles_k
            *done = sum + 4;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
   volatile uint32_t* abort = tmem_slot + 1;
-  pdl_wait();
-  pdl_release();
-
-  // first row of unit u's part of its block
-  auto block_row = [&](const RankUnit& u) {
-    return p.vblk + ((static_cast<int64_t>(u.blk) << (6 + p.lvl)) + u.sub * kTileRows) * p.ldb;
-  };
-  if (count > 1) {
-    // Whole clusters leave here, before any set-up: most of the grid's units have
-    // nothing of the block's request, or the block is not used at all.
-    const RankUnit u = rank_unit(p, unit0);
-    if (!u.work) {
-      if (u.used && p.vblk != nullptr) {
-        uint4* at = reinterpret_cast<uint4*>(block_row(u));
-        for (int e = rank * kRankThreads + threadIdx.x; e < rows * p.ldb / 8; e += count * kRankThreads)
-          at[e] = make_uint4(0, 0, 0, 0);
-      }
-      return;
-    }
-  }
   if (threadIdx.x == 0) {
     for (int s = 0; s < geo.stages; ++s) {
       mbar_init(smem_u32(&full[s]), 1);
@@ -160,6 +166,8 @@ __global__ void __launch_bounds__(kRankThreads, COLS <= 64 ? 2 : 1) rank_tiles_k
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  pdl_wait();
+  pdl_release();
 
   // K stages of this CTA
   const int all = (p.k + 63) / 64, per = (all + count - 1) / count;
@@ -235,10 +243,10 @@ __global__ void __launch_bounds__(kRankThreads, COLS <= 64 ? 2 : 1) rank_tiles_k
     bool ok = true;
     for (int unit = unit0; unit < p.units && ok; unit += step) {
       const RankUnit u = rank_unit(p, unit);
-      if (!u.used) continue;
+      if (!u.work) continue;
 #pragma unroll
       for (int c = 0; c < COLS; ++c) sums[c] = 0.0f;
-      for (int k = 0; u.work && k < n_kt; k += kChunk, ++chunk) {
+      for (int k = 0; k < n_kt; k += kChunk, ++chunk) {
         const int b = chunk & 1;
         ok = __all_sync(0xFFFFFFFFu, mbar_wait<true>(smem_u32(&sum[b]), (chunk >> 1) & 1u, abort, kSiteRankSum | b,
                                                p.wait_limit_ns)) != 0;
@@ -258,6 +266,7 @@ __global__ void __launch_bounds__(kRankThreads, COLS <= 64 ? 2 : 1) rank_tiles_k
         if (lane == 0) mbar_arrive(smem_u32(&taken[b]));
       }
       if (count > 1 || !ok) break;  // a cluster has one unit
+      clear_rows(p, u, threadIdx.x - 32 * kSumWarp0, 32 * 4);
       if (r >= rows) continue;
       const bool mine = r >= u.lo && r < u.hi;
       const float scale = unit_scale(p, u);
@@ -270,7 +279,7 @@ __global__ void __launch_bounds__(kRankThreads, COLS <= 64 ? 2 : 1) rank_tiles_k
           if (c < p.rp) *reinterpret_cast<float4*>(at + c) = make_float4(sums[c], sums[c + 1], sums[c + 2], sums[c + 3]);
       }
       if (p.vblk != nullptr) {
-        uint16_t* at = block_row(u) + static_cast<int64_t>(r) * p.ldb;
+        uint16_t* at = p.vblk + (u.out + r) * p.ldb;
 #pragma unroll
         for (int c = 0; c < COLS; c += 8)
           *reinterpret_cast<uint4*>(at + c) =
@@ -295,11 +304,12 @@ __global__ void __launch_bounds__(kRankThreads, COLS <= 64 ? 2 : 1) rank_tiles_k
     if (!aborted) {
       // each CTA adds up and writes its share of the rows
       const RankUnit u = rank_unit(p, unit0);
-      const float scale = unit_scale(p, u);
+      const float scale = u.work ? unit_scale(p, u) : 0.0f;
+      clear_rows(p, u, rank * kRankThreads + threadIdx.x, count * kRankThreads);
       const int share = (rows + count - 1) / count, first = rank * share, last = min(first + share, rows);
       const int quads = (p.vblk != nullptr ? p.ldb : p.rp) / 4;
       const uint32_t ld = static_cast<uint32_t>(p.rp + 4) * 4u;
-      for (int e = first * quads + threadIdx.x; e < last * quads; e += kRankThreads) {
+      for (int e = first * quads + threadIdx.x; u.work && e < last * quads; e += kRankThreads) {
         const int r = e / quads, c = e % quads * 4;
         float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         if (r >= u.lo && r < u.hi && c < p.rp) {
@@ -316,7 +326,7 @@ __global__ void __launch_bounds__(kRankThreads, COLS <= 64 ? 2 : 1) rank_tiles_k
           if (p.v32 != nullptr) *reinterpret_cast<float4*>(p.v32 + static_cast<int64_t>(u.row0 + r) * p.ld32 + c) = s;
         }
         if (p.vblk != nullptr)
-          *reinterpret_cast<uint2*>(block_row(u) + static_cast<int64_t>(r) * p.ldb + c) =
+          *reinterpret_cast<uint2*>(p.vblk + (u.out + r) * p.ldb + c) =
               make_uint2(pack_bf16x2(s.x, s.y), pack_bf16x2(s.z, s.w));
       }
     }
@@ -356,15 +366,13 @@ cudaError_t launch_cols(const RankParams& p, unsigned ctas, cudaStream_t stream)
 
 cudaError_t launch_rank_tiles(const RankParams& p, cudaStream_t stream) {
   RankParams q = p;
-  const int tile_rows = 64 << p.lvl, subs = tile_rows > kTileRows ? tile_rows / kTileRows : 1;
-  q.units = plan_blocks(p.plan.m, p.plan.n_req, p.lvl) * subs;
-  // K splits: until the units with work (about one per 128 rows and one more per
-  // request) times the splits take most SMs, each with four stages. More cost more
+  q.units = plan_blocks(p.plan.m, p.plan.n_req, p.lvl > 0 ? 1 : 0);
+  // K splits: until the units times the splits take most SMs, each with four stages. More cost more
   // than they bring: m 4352, k 3840 in one request takes 21.8 us with 8 splits,
   // 16.1 with 4.
-  const int parts = (p.plan.m + kTileRows - 1) / kTileRows + p.plan.n_req, stages = (p.k + 63) / 64;
+  const int stages = (p.k + 63) / 64;
   q.splits = 1;
-  while (q.splits < kMaxRankSplits && parts * q.splits < 100 && stages >= 8 * q.splits) q.splits *= 2;
+  while (q.splits < kMaxRankSplits && q.units * q.splits < 100 && stages >= 8 * q.splits) q.splits *= 2;
   const int room = 148 * (p.rp <= 64 ? 2 : 1);  // CTAs resident at once
   const unsigned ctas = q.splits > 1 ? static_cast<unsigned>(q.units) * q.splits
                                      : static_cast<unsigned>(q.units < room ? q.units : room);
