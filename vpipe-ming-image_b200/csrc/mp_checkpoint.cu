@@ -8,8 +8,8 @@
 // Both kernels are one pass, bound by memory: 3 bytes a value. Each of 16
 // lanes holds 8 consecutive features of a group (one 16-byte load), the group's
 // maximum goes round them by shuffles. A thread takes the same features of
-// kCkRows rows: four loads in flight each, and the four scales of a group land
-// in one 32-byte sector. The bf16 rows are read and written with a streaming
+// kCkRows rows: four loads in flight each, one reciprocal for four rows, and the
+// four scales of a group land in one 32-byte sector. The bf16 rows are read and written with a streaming
 // hint, which leaves L2 to the codes: the restore that follows finds some there.
 #include <cuda_runtime.h>
 
@@ -25,6 +25,12 @@ constexpr int kPerLane = 8;                         // features of a lane
 constexpr int kGroupLanes = kCkGroup / kPerLane;    // 16
 
 constexpr int kCkRows = 4;
+
+__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("max.u16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
 
 // Block (x, y): rows [4 x, 4 x + 4), groups [16 y, 16 y + 16), one per half-warp.
 __global__ void __launch_bounds__(kCkThreads) checkpoint_kernel(const __grid_constant__ CheckpointParams p) {
@@ -49,21 +55,38 @@ __global__ void __launch_bounds__(kCkThreads) checkpoint_kernel(const __grid_con
       raw[r] = make_uint4(w[0], w[1], w[2], w[3]);
     }
   }
+  // max|x| on the bf16 patterns, two at a time: without the sign they order like
+  // the values, infinities and NaNs last
+  uint32_t top2[kCkRows];
+#pragma unroll
+  for (int r = 0; r < kCkRows; ++r)
+    top2[r] = max_u16x2(max_u16x2(raw[r].x & 0x7FFF7FFFu, raw[r].y & 0x7FFF7FFFu),
+                        max_u16x2(raw[r].z & 0x7FFF7FFFu, raw[r].w & 0x7FFF7FFFu));
+  // The group's lanes share the four rows' maxima out as they reduce them: after
+  // two exchanges lane (8 b3 + 4 b2 + ..) holds row 2 b3 + b2 alone, so that the
+  // reciprocal and the division are done once a lane, not once a row.
+  const int lane = threadIdx.x % kGroupLanes;
+  const bool b3 = (lane & 8) != 0, b2 = (lane & 4) != 0;
+  const uint32_t s0 = __shfl_xor_sync(0xFFFFFFFFu, b3 ? top2[0] : top2[2], 8);
+  const uint32_t s1 = __shfl_xor_sync(0xFFFFFFFFu, b3 ? top2[1] : top2[3], 8);
+  const uint32_t k0 = max_u16x2(b3 ? top2[2] : top2[0], s0), k1 = max_u16x2(b3 ? top2[3] : top2[1], s1);
+  uint32_t mine = max_u16x2(b2 ? k1 : k0, __shfl_xor_sync(0xFFFFFFFFu, b2 ? k0 : k1, 4));
+  mine = max_u16x2(mine, __shfl_xor_sync(0xFFFFFFFFu, mine, 2));
+  mine = max_u16x2(mine, __shfl_xor_sync(0xFFFFFFFFu, mine, 1));
+  const uint32_t top_bits = max(mine & 0xFFFFu, mine >> 16);
+  const float top = bf16_bits_to_f32(top_bits);
+  const bool finite = top_bits < 0x7F80u, live = finite && top >= kCkTiny;
+  const float my_inv = live ? __fmul_rn(127.0f, __frcp_rn(top)) : 0.0f;
+  const int my_row = row0 + (lane >> 2);
+  if ((lane & 3) == 0 && group * kCkGroup < p.k && my_row < p.m) {
+    // a group with an infinity or a NaN is NaN throughout
+    p.scale[static_cast<int64_t>(group) * p.m + my_row] =
+        live ? __fdiv_rn(top, 127.0f) : finite ? 0.0f : __int_as_float(0x7FC00000);
+  }
 #pragma unroll
   for (int r = 0; r < kCkRows; ++r) {
-    // max|x| on the bf16 patterns, two at a time: without the sign they order
-    // like the values, infinities and NaNs last
-    const uint32_t v[4] = {raw[r].x, raw[r].y, raw[r].z, raw[r].w};
-    uint32_t top2 = __vmaxu2(__vmaxu2(v[0] & 0x7FFF7FFFu, v[1] & 0x7FFF7FFFu),
-                             __vmaxu2(v[2] & 0x7FFF7FFFu, v[3] & 0x7FFF7FFFu));
-#pragma unroll
-    for (int d = 1; d < kGroupLanes; d <<= 1) top2 = __vmaxu2(top2, __shfl_xor_sync(0xFFFFFFFFu, top2, d));
-    const uint32_t top_bits = max(top2 & 0xFFFFu, top2 >> 16);
-    const float top = bf16_bits_to_f32(top_bits);
-    const bool finite = top_bits < 0x7F80u;
+    const float inv = __shfl_sync(0xFFFFFFFFu, my_inv, 4 * r, kGroupLanes);
     if (c >= p.k || row0 + r >= p.m) continue;
-    const bool live = finite && top >= kCkTiny;
-    const float inv = live ? __fmul_rn(127.0f, __frcp_rn(top)) : 0.0f;
     // x inv, then the nearest whole number (ties to even) in the low mantissa
     // bits of 1.5 2^23; |x| inv <= 127 (1 + 2^-24)^3 rounds to 127 at most. The
     // two roundings are the definition's, so never one FMA (packed f32x2 products
@@ -71,21 +94,17 @@ __global__ void __launch_bounds__(kCkThreads) checkpoint_kernel(const __grid_con
     auto code = [&](uint32_t pattern) {
       return __float_as_uint(__fadd_rn(__fmul_rn(__uint_as_float(pattern), inv), 12582912.0f));
     };
+    const uint32_t v[4] = {raw[r].x, raw[r].y, raw[r].z, raw[r].w};
     uint32_t w[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const uint32_t a = v[2 * h], b = v[2 * h + 1];
       const uint32_t lo = __byte_perm(code(a << 16), code(a & 0xFFFF0000u), 0x0040);
       const uint32_t hi = __byte_perm(code(b << 16), code(b & 0xFFFF0000u), 0x0040);
-      w[h] = live ? __byte_perm(lo, hi, 0x5410) : 0u;
+      w[h] = inv != 0.0f ? __byte_perm(lo, hi, 0x5410) : 0u;
     }
     int8_t* out = p.q + static_cast<int64_t>(row0 + r) * p.ldq + c;  // the pitch is a multiple of 16
     *reinterpret_cast<uint2*>(out) = make_uint2(w[0], w[1]);
-    if (threadIdx.x % kGroupLanes == 0) {
-      // a group with an infinity or a NaN is NaN throughout
-      const float s = finite ? (live ? __fdiv_rn(top, 127.0f) : 0.0f) : __int_as_float(0x7FC00000);
-      p.scale[static_cast<int64_t>(group) * p.m + row0 + r] = s;
-    }
   }
 }
 
