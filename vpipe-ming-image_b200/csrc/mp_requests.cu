@@ -343,8 +343,6 @@ __global__ void __launch_bounds__(32 * kRankWarps) rank_rows_kernel(const __grid
 
 // ---- the whole projection, few rows ------------------------------------------------
 
-constexpr int kFewWarps = 8;
-
 // The 16 weights of one row that a lane holds of a 64-wide K group, as loaded.
 template <int BITS>
 struct FewCodes {
@@ -352,15 +350,19 @@ struct FewCodes {
   uint32_t w[kWords];
 };
 
+// Bytes of a 64-wide group of a row, and of a lane's share of it.
 template <int BITS>
-__device__ __forceinline__ void few_load(const uint8_t* row, int group, int j, int k, bool ok, FewCodes<BITS>& c) {
-  if constexpr (BITS == 0) {
-    load16(reinterpret_cast<const uint16_t*>(row), 64 * group + 16 * j, k, ok, c.w);
+constexpr int kGroupBytes = BITS == 0 ? 128 : 8 * BITS;
+
+template <int BITS>
+__device__ __forceinline__ void few_load(const uint8_t* at, int col, int k, FewCodes<BITS>& c) {
+  if constexpr (BITS == 0) {  // `at`: the lane's column `col`; zeros from column k on
+    load16(reinterpret_cast<const uint16_t*>(at) - col, col, k, true, c.w);
   } else if constexpr (BITS == 8) {
-    const uint4 v = ok ? ld_global_nc_v4(row + 64 * group + 16 * j) : make_uint4(0, 0, 0, 0);
+    const uint4 v = ld_global_nc_v4(at);
     c.w[0] = v.x, c.w[1] = v.y, c.w[2] = v.z, c.w[3] = v.w;
   } else {
-    const uint2 v = ok ? __ldg(reinterpret_cast<const uint2*>(row + 32 * group + 8 * j)) : make_uint2(0, 0);
+    const uint2 v = __ldg(reinterpret_cast<const uint2*>(at));
     c.w[0] = v.x, c.w[1] = v.y;
   }
 }
@@ -391,12 +393,11 @@ __device__ __forceinline__ void few_pairs(const FewCodes<BITS>& c, uint32_t code
 
 // The lane's 16 values of x in the same order.
 template <int BITS>
-__device__ __forceinline__ void few_x(const uint16_t* row, int group, int j, int k, uint32_t (&x)[8]) {
+__device__ __forceinline__ void few_x(const uint16_t* at, int col, int k, uint32_t (&x)[8]) {
   if constexpr (BITS == 0) {
-    load16(row, 64 * group + 16 * j, k, true, x);
+    load16(at - col, col, k, true, x);
   } else {
-    const uint4* at = reinterpret_cast<const uint4*>(row + 64 * group + 16 * j);
-    const uint4 a = __ldg(at), b = __ldg(at + 1);
+    const uint4 a = __ldg(reinterpret_cast<const uint4*>(at)), b = __ldg(reinterpret_cast<const uint4*>(at) + 1);
     if constexpr (BITS == 8) {
       x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w;
       x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
@@ -410,53 +411,61 @@ __device__ __forceinline__ void few_x(const uint16_t* row, int group, int j, int
 }
 
 // y[t] = W x[t] + B_a v[t] for up to 8 NT rows: bound by reading W once. A
-// block takes 16 MT features, its warps the 64-wide K groups in turn, lanes as in
+// block takes 16 features, its WARPS warps the 64-wide K groups in turn, lanes as in
 // rank_rows_kernel. Packed weights are not dequantized: a group's MMAs run on
 // the codes, and with the sum of the group's x (one more MMA, against ones)
-//   sum_k W x = scale (sum_k q x - zero sum_k x) + bias sum_k x
+//   sum_k W x = scale sum_k q x + (bias - scale zero) sum_k x
 // in f32, exact codes and one scale per group. The kernel starts beside
 // rank_rows_kernel (it reads x and W, which are complete when that one runs) and
 // waits for it before the adapters' part. Rows past m repeat the last one: the
 // MMA's columns are independent, theirs are not stored.
-template <int BITS, int MT, int NT>
-__global__ void __launch_bounds__(32 * kFewWarps, NT <= 2 ? 2 : 1)
+template <int BITS, int NT, int WARPS>
+__global__ void __launch_bounds__(32 * WARPS, NT > 2 ? 1 : 16 / WARPS)
     few_rows_kernel(const __grid_constant__ FewParams p) {
-  constexpr int kBatch = (BITS == 0 ? 2 : 4) / MT;  // K groups a warp has in flight, twice
-  constexpr int kFeat = 16 * MT;
-  __shared__ float part[kFewWarps][kFeat][8 * NT + 1];
+  // K groups a warp loads at a time, one batch ahead: 128 bytes a lane in flight
+  constexpr int kBatch = BITS == 4 ? 4 : BITS == 8 ? 2 : 1;
+  __shared__ float part[WARPS][16][8 * NT + 1];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, j = lane & 3;
-  const int f0 = blockIdx.x * kFeat;
-  const uint8_t* wrow[2 * MT];
-  const uint32_t* srow[2 * MT];
+  const int f0 = blockIdx.x * 16;
+  // The lane's place in the warp's first group, stepped from batch to batch: the
+  // groups of a batch are constant offsets from it.
+  constexpr int kGroup = kGroupBytes<BITS>, kStep = WARPS * kBatch;
+  const uint8_t* wp[2];
+  const uint32_t* sp[2];
 #pragma unroll
-  for (int h = 0; h < 2 * MT; ++h) {
+  for (int h = 0; h < 2; ++h) {
     const int n = min(f0 + 8 * h + g, p.n - 1);  // rows past n repeat the last
-    wrow[h] = p.w + static_cast<size_t>(n) * p.w_pitch;
-    srow[h] = p.sb + static_cast<size_t>(n) * p.sb_stride;
+    wp[h] = p.w + static_cast<size_t>(n) * p.w_pitch + warp * kGroup + j * (kGroup / 4);
+    sp[h] = p.sb + static_cast<size_t>(n) * p.sb_stride + warp;
   }
-  const uint16_t* xrow[NT];
+  const uint16_t* xp[NT];
 #pragma unroll
-  for (int t = 0; t < NT; ++t) xrow[t] = p.x + static_cast<int64_t>(min(8 * t + g, p.m - 1)) * p.ldx;
+  for (int t = 0; t < NT; ++t) xp[t] = p.x + static_cast<int64_t>(min(8 * t + g, p.m - 1)) * p.ldx + 64 * warp + 16 * j;
   const int groups = (p.k + 63) / 64;
-  constexpr int kStep = kFewWarps * kBatch;
 
-  FewCodes<BITS> codes[2][kBatch][2 * MT];
-  uint32_t sb[2][kBatch][2 * MT];
-  auto load = [&](int i0, int buf) {
+  FewCodes<BITS> codes[2][kBatch][2];
+  uint32_t sb[2][kBatch][2];
+  auto load = [&](int i0, int buf) {  // and steps on
 #pragma unroll
     for (int b = 0; b < kBatch; ++b) {
-      const int i = i0 + b * kFewWarps;
+      if (i0 + b * WARPS < groups) {
 #pragma unroll
-      for (int h = 0; h < 2 * MT; ++h) {
-        few_load<BITS>(wrow[h], i, j, p.k, i < groups, codes[buf][b][h]);
-        if constexpr (BITS != 0) sb[buf][b][h] = i < groups ? __ldg(srow[h] + i) : 0u;
+        for (int h = 0; h < 2; ++h) {
+          few_load<BITS>(wp[h] + b * WARPS * kGroup, 64 * (i0 + b * WARPS) + 16 * j, p.k, codes[buf][b][h]);
+          if constexpr (BITS != 0) sb[buf][b][h] = __ldg(sp[h] + b * WARPS);
+        }
       }
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      wp[h] += kStep * kGroup;
+      sp[h] += kStep;
     }
   };
   load(warp, 0);
-  float y[MT][NT][4];
+  float y[NT][4];
 #pragma unroll
-  for (int e = 0; e < MT * NT * 4; ++e) y[e / (4 * NT)][e / 4 % NT][e % 4] = 0.0f;
+  for (int e = 0; e < 4 * NT; ++e) y[e / 4][e % 4] = 0.0f;
   const uint32_t ones = 0x3F803F80u;
   // whole pairs of batches, so that the buffers' indices are constants
   for (int i0 = warp; i0 < groups; i0 += 2 * kStep) {
@@ -467,67 +476,60 @@ __global__ void __launch_bounds__(32 * kFewWarps, NT <= 2 ? 2 : 1)
       load(ih + kStep, half ^ 1);
 #pragma unroll
       for (int b = 0; b < kBatch; ++b) {
-        const int i = ih + b * kFewWarps;
+        const int i = ih + b * WARPS;
         if (i >= groups) break;
         uint32_t x[NT][8];
 #pragma unroll
-        for (int t = 0; t < NT; ++t) few_x<BITS>(xrow[t], i, j, p.k, x[t]);
-        float sum[NT][4];  // of the group's x: a column each, the same in every row
-        if constexpr (BITS != 0) {
+        for (int t = 0; t < NT; ++t) few_x<BITS>(xp[t] + b * WARPS * 64, 64 * i + 16 * j, p.k, x[t]);
+        uint32_t lo[8], hi[8];
+        few_pairs<BITS>(codes[half][b][0], p.code_xor, lo);
+        few_pairs<BITS>(codes[half][b][1], p.code_xor, hi);
+        if constexpr (BITS == 0) {
+#pragma unroll
+          for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int s = 0; s < 4; ++s)
+              mma_16x8x16(y[t], lo[2 * s], hi[2 * s], lo[2 * s + 1], hi[2 * s + 1], x[t][2 * s], x[t][2 * s + 1]);
+        } else {
+          // scale, and bias less scale * zero, of rows g and g + 8
+          const uint32_t z0 = sb[half][b][0], z1 = sb[half][b][1];
+          const float s0 = bf16_bits_to_f32(z0 & 0xFFFFu), s1 = bf16_bits_to_f32(z1 & 0xFFFFu);
+          const float o0 = fmaf(-p.zero, s0, bf16_bits_to_f32(z0 >> 16));
+          const float o1 = fmaf(-p.zero, s1, bf16_bits_to_f32(z1 >> 16));
 #pragma unroll
           for (int t = 0; t < NT; ++t) {
-            mma_16x8x16_first(sum[t], ones, ones, ones, ones, x[t][0], x[t][1]);
+            float d[4], e[4];  // e: the sums of x, the same in every row
+            mma_16x8x16_first(e, ones, ones, ones, ones, x[t][0], x[t][1]);
+            mma_16x8x16_first(d, lo[0], hi[0], lo[1], hi[1], x[t][0], x[t][1]);
 #pragma unroll
-            for (int s = 1; s < 4; ++s) mma_16x8x16(sum[t], ones, ones, ones, ones, x[t][2 * s], x[t][2 * s + 1]);
-          }
-        }
-#pragma unroll
-        for (int m = 0; m < MT; ++m) {
-          uint32_t lo[8], hi[8];
-          few_pairs<BITS>(codes[half][b][2 * m], p.code_xor, lo);
-          few_pairs<BITS>(codes[half][b][2 * m + 1], p.code_xor, hi);
-          if constexpr (BITS == 0) {
-#pragma unroll
-            for (int t = 0; t < NT; ++t)
-#pragma unroll
-              for (int s = 0; s < 4; ++s)
-                mma_16x8x16(y[m][t], lo[2 * s], hi[2 * s], lo[2 * s + 1], hi[2 * s + 1], x[t][2 * s], x[t][2 * s + 1]);
-          } else {
-            const uint32_t z0 = sb[half][b][2 * m], z1 = sb[half][b][2 * m + 1];
-            const float s0 = bf16_bits_to_f32(z0 & 0xFFFFu), o0 = bf16_bits_to_f32(z0 >> 16);
-            const float s1 = bf16_bits_to_f32(z1 & 0xFFFFu), o1 = bf16_bits_to_f32(z1 >> 16);
-#pragma unroll
-            for (int t = 0; t < NT; ++t) {
-              float d[4];
-              mma_16x8x16_first(d, lo[0], hi[0], lo[1], hi[1], x[t][0], x[t][1]);
-#pragma unroll
-              for (int s = 1; s < 4; ++s)
-                mma_16x8x16(d, lo[2 * s], hi[2 * s], lo[2 * s + 1], hi[2 * s + 1], x[t][2 * s], x[t][2 * s + 1]);
-#pragma unroll
-              for (int q = 0; q < 4; ++q)
-                y[m][t][q] = fmaf(q < 2 ? s0 : s1, fmaf(-p.zero, sum[t][q], d[q]),
-                                  fmaf(q < 2 ? o0 : o1, sum[t][q], y[m][t][q]));
+            for (int s = 1; s < 4; ++s) {
+              mma_16x8x16(e, ones, ones, ones, ones, x[t][2 * s], x[t][2 * s + 1]);
+              mma_16x8x16(d, lo[2 * s], hi[2 * s], lo[2 * s + 1], hi[2 * s + 1], x[t][2 * s], x[t][2 * s + 1]);
             }
+            y[t][0] = fmaf(s0, d[0], fmaf(o0, e[0], y[t][0]));
+            y[t][1] = fmaf(s0, d[1], fmaf(o0, e[1], y[t][1]));
+            y[t][2] = fmaf(s1, d[2], fmaf(o1, e[0], y[t][2]));
+            y[t][3] = fmaf(s1, d[3], fmaf(o1, e[1], y[t][3]));
           }
         }
       }
+#pragma unroll
+      for (int t = 0; t < NT; ++t) xp[t] += kStep * 64;
     }
   }
 #pragma unroll
-  for (int m = 0; m < MT; ++m)
+  for (int t = 0; t < NT; ++t)
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-      for (int q = 0; q < 4; ++q) part[warp][16 * m + g + 8 * (q >> 1)][8 * t + 2 * j + (q & 1)] = y[m][t][q];
+    for (int q = 0; q < 4; ++q) part[warp][g + 8 * (q >> 1)][8 * t + 2 * j + (q & 1)] = y[t][q];
   __syncthreads();
   pdl_wait();  // v is complete; y may be written
   pdl_release();
-  const int f = threadIdx.x % kFeat;
+  const int f = threadIdx.x & 15;
   if (f0 + f >= p.n) return;
-  for (int t = threadIdx.x / kFeat; t < p.m; t += 32 * kFewWarps / kFeat) {
+  for (int t = threadIdx.x >> 4; t < p.m; t += 2 * WARPS) {
     float sum = part[0][f][t];
 #pragma unroll
-    for (int w = 1; w < kFewWarps; ++w) sum += part[w][f][t];
+    for (int w = 1; w < WARPS; ++w) sum += part[w][f][t];
     const int a = p.row_adapter[t];
     if (a >= 0) {
       const uint16_t* br = p.b + (static_cast<size_t>(a) * p.n + f0 + f) * p.rp;
@@ -622,24 +624,27 @@ cudaError_t launch_rank_rows(const RankParams& p, cudaStream_t stream) {
 
 namespace {
 
-template <int BITS, int MT>
+template <int BITS, int WARPS>
 cudaError_t launch_few(const FewParams& p, cudaStream_t stream) {
-  const dim3 grid((p.n + 16 * MT - 1) / (16 * MT)), block(32 * kFewWarps);
+  const dim3 grid((p.n + 15) / 16), block(32 * WARPS);
   // it may start beside rank_rows_kernel, never beside what comes before that
   const bool over = p.chunks > 0;
-  if (p.m <= 8) return launch_overlapped(few_rows_kernel<BITS, MT, 1>, grid, block, p, stream, over);
-  if (p.m <= 16) return launch_overlapped(few_rows_kernel<BITS, MT, 2>, grid, block, p, stream, over);
-  if constexpr (MT == 1) {
-    if (p.m <= 32) return launch_overlapped(few_rows_kernel<BITS, MT, 4>, grid, block, p, stream, over);
-  }
+  if (p.m <= 8) return launch_overlapped(few_rows_kernel<BITS, 1, WARPS>, grid, block, p, stream, over);
+  if (p.m <= 16) return launch_overlapped(few_rows_kernel<BITS, 2, WARPS>, grid, block, p, stream, over);
+  if (p.m <= 32) return launch_overlapped(few_rows_kernel<BITS, 4, WARPS>, grid, block, p, stream, over);
   return cudaErrorInvalidValue;
 }
 
-// 32 features a block halve the reads of x and the sums of it; 16 while 32 would
-// leave SMs without a block.
+// Blocks of 8 warps; of 4 for a bf16 weight with many features, whose rows are
+// long enough to keep them busy: 10240x3840 takes 23.7 us with 4 and 30.8 with 8
+// at 16 rows, 3840x10240 39.2 and 29.9. Packed weights are faster with 8 at every
+// shape tried (w4 10240x3840, 16 rows: 23.8 and 21.9 us).
 template <int BITS>
 cudaError_t launch_few(const FewParams& p, cudaStream_t stream) {
-  return p.n >= 32 * 2 * 148 && p.m <= 16 ? launch_few<BITS, 2>(p, stream) : launch_few<BITS, 1>(p, stream);
+  if constexpr (BITS == 0) {
+    if (p.n >= 16 * 3 * 148) return launch_few<BITS, 4>(p, stream);
+  }
+  return launch_few<BITS, 8>(p, stream);
 }
 
 }  // namespace
