@@ -113,7 +113,7 @@ struct mp_adapters {
   int n = 0, k = 0, cap = 0, max_rank = 0;
   int rp = 0;              // max_rank rounded up to 16
   int kp = 0, np = 0;      // k, n rounded up to 8
-  uint16_t* a = nullptr;   // [cap][rp][kp]
+  uint16_t* a = nullptr;   // [cap][rp][kp]; the start of the one allocation
   uint16_t* b = nullptr;   // [cap][n][rp]
   uint16_t* at = nullptr;  // [cap][k][rp] (training)
   uint16_t* bt = nullptr;  // [cap][rp][np] (training)
@@ -2191,28 +2191,23 @@ int mp_adapters_create(mp_ctx* c, int n, int k, int capacity, int max_rank, int 
   b->rp = (max_rank + 15) / 16 * 16;
   b->kp = (k + 7) / 8 * 8;
   b->np = (n + 7) / 8 * 8;
+  // one allocation, zeroed: an adapter that was never set adds nothing
+  const size_t cr = static_cast<size_t>(capacity) * b->rp;  // a multiple of 16: every part is 16-byte aligned
+  const size_t ea = cr * b->kp, eb = cr * n, eat = training ? cr * k : 0, ebt = training ? cr * b->np : 0;
+  const size_t bytes = (ea + eb + eat + ebt) * sizeof(uint16_t) + static_cast<size_t>(capacity) * sizeof(int32_t);
+  cudaError_t e = cudaMalloc(&b->a, bytes);
+  if (e == cudaSuccess) e = cudaMemset(b->a, 0, bytes);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(nullptr);  // a call on any stream may follow
   auto cleanup = [&](int code) {
     cudaFree(b->a);
-    cudaFree(b->b);
-    cudaFree(b->at);
-    cudaFree(b->bt);
-    cudaFree(b->bad);
     delete b;
     return code;
   };
-  // zeroed: an adapter that was never set adds nothing
-  auto zeros = [&](auto** p, size_t elems) {
-    cudaError_t e = cudaMalloc(p, elems * sizeof(**p));
-    return e == cudaSuccess ? cudaMemset(*p, 0, elems * sizeof(**p)) : e;
-  };
-  const size_t cr = static_cast<size_t>(capacity) * b->rp;
-  cudaError_t e = zeros(&b->a, cr * b->kp);
-  if (e == cudaSuccess) e = zeros(&b->b, cr * n);
-  if (e == cudaSuccess && training) e = zeros(&b->at, cr * k);
-  if (e == cudaSuccess && training) e = zeros(&b->bt, cr * b->np);
-  if (e == cudaSuccess) e = zeros(&b->bad, capacity);
-  if (e == cudaSuccess) e = cudaStreamSynchronize(nullptr);  // set on any stream may follow
   if (e != cudaSuccess) return cleanup(cuda_fail(c, e, "cudaMalloc(adapters)"));
+  b->b = b->a + ea;
+  b->at = training ? b->b + eb : nullptr;
+  b->bt = training ? b->at + eat : nullptr;
+  b->bad = reinterpret_cast<int32_t*>(b->b + eb + eat + ebt);
   const uint64_t pitch = static_cast<uint64_t>(b->rp) * 2, cap = static_cast<uint64_t>(capacity);
   if (!encode_2d(&b->tm_b, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, b->b, b->rp, cap * n, pitch, 64, 128,
                  CU_TENSOR_MAP_SWIZZLE_128B) ||
@@ -2232,10 +2227,6 @@ int mp_adapters_free(mp_ctx* c, mp_adapters* b) {
   cudaSetDevice(c->device);
   cudaDeviceSynchronize();
   cudaFree(b->a);
-  cudaFree(b->b);
-  cudaFree(b->at);
-  cudaFree(b->bt);
-  cudaFree(b->bad);
   delete b;
   return MP_OK;
 }
@@ -2309,7 +2300,8 @@ int mp_requests_create(mp_ctx* c, int max_requests, int max_rows, int capacity, 
     at_live[l] = take(tiles);
   }
   const size_t at_chunk = take(4 * static_cast<size_t>(mp::plan_chunks(max_rows, max_requests)));
-  const size_t at_seg = take(2 * q), at_begin = take(capacity + 1), at_row = take(max_rows);
+  const size_t at_seg = take(2 * q), at_begin = take(capacity + 1), at_by = take(capacity),
+               at_row = take(mp::kFewRows);
   cudaError_t e = cudaMalloc(&r->buf, words * sizeof(int32_t));
   if (e != cudaSuccess) {
     delete r;
@@ -2325,6 +2317,7 @@ int mp_requests_create(mp_ctx* c, int max_requests, int max_rows, int capacity, 
   r->plan.chunk = reinterpret_cast<int4*>(r->buf + at_chunk);
   r->plan.seg = reinterpret_cast<int2*>(r->buf + at_seg);
   r->plan.begin = r->buf + at_begin;
+  r->plan.by_rows = r->buf + at_by;
   r->plan.row_adapter = r->buf + at_row;
   *out = r;
   return MP_OK;

@@ -43,6 +43,8 @@ constexpr int kChunk = 4;     // stages of an accumulator
 
 constexpr int kConvWarp0 = 2;
 constexpr int kConvThreads = 256;
+constexpr int kConvGroups = 2;  // of four warps, which take the stages in turn
+constexpr int kConvGroup = kConvThreads / kConvGroups;
 constexpr int kSumWarp0 = kConvWarp0 + kConvThreads / 32;
 // Warps that add up the accumulators: 4 hold a feature row of up to 64 ranks a
 // thread, 8 one of up to 128 in two halves (TASKS 4).
@@ -210,7 +212,8 @@ struct GradSmem {
   volatile uint32_t* abort;
 };
 
-// An item: its adapter, member and feature tile.
+// An item: its adapter, member and feature tile. The adapters with the most rows
+// come first.
 struct Item {
   int a, f_tile;
   const GradMember* mb;
@@ -218,8 +221,9 @@ struct Item {
 
 __device__ __forceinline__ Item item_of(const GradParams& p, int i) {
   Item it;
-  it.a = i / p.tiles;
-  int t = i - it.a * p.tiles;
+  const int place = i / p.tiles;
+  it.a = p.plan.by_rows[place];
+  int t = i - place * p.tiles;
   const int first = (p.mem[0].width + kTileF - 1) / kTileF;
   const bool second = p.n_mem > 1 && t >= first;
   it.mb = &p.mem[second ? 1 : 0];
@@ -227,16 +231,35 @@ __device__ __forceinline__ Item item_of(const GradParams& p, int i) {
   return it;
 }
 
-// Warps 2-9. TASKS: 8-value pieces of a 64-row stage of u per thread.
+// The items of worker `w` of `workers`: one of each round, the rounds to and fro,
+// so that whoever has the larger one of a round has the smaller one of the next
+// (the rounds descend in rows). At 24 requests on 16 adapters the busiest of 148
+// then has 8 % more rows than the average, 35 % more without.
+struct ItemIter {
+  int round, w, workers, items;
+  __device__ ItemIter(const GradParams& p, int w_, int workers_) : round(0), w(w_), workers(workers_), items(p.items) {}
+  // The next item, or -1.
+  __device__ __forceinline__ int next() {
+    const int first = round * workers, i = first + (round & 1 ? workers - 1 - w : w);
+    ++round;
+    return first < items && i < items ? i : -1;  // only the last round can be short
+  }
+};
+
+// Warps 2-9, in two groups: a stage's work is a chain of latencies (its copies'
+// arrival, shared memory, the conversions, the fence), so two stages are worked on
+// at once. TASKS: 16-value pieces of a 64-row stage of u per thread.
 template <int TASKS>
 __device__ void convert(const GradParams& p, const GradSmem& sm, const GradGeo& geo, const PartCols& pc, int item0,
                         int step, int rank, int count) {
-  const int tid = threadIdx.x - 32 * kConvWarp0, lane = threadIdx.x & 31;
+  const int tid = (threadIdx.x - 32 * kConvWarp0) % kConvGroup, lane = threadIdx.x & 31;
+  const int group = (threadIdx.x - 32 * kConvWarp0) / kConvGroup;
   const int per_row = p.rp / 8, pieces = kRows * per_row;
-  int row_of[TASKS], col_of[TASKS];
+  constexpr int kPieces = TASKS * kConvGroups;
+  int row_of[kPieces], col_of[kPieces];
 #pragma unroll
-  for (int j = 0; j < TASKS; ++j) {
-    const int e = tid + j * kConvThreads;
+  for (int j = 0; j < kPieces; ++j) {
+    const int e = tid + j * kConvGroup;
     row_of[j] = e < pieces ? e / per_row : kRows;  // kRows: no piece
     col_of[j] = e < pieces ? e % per_row * 8 : 0;
   }
@@ -245,19 +268,24 @@ __device__ void convert(const GradParams& p, const GradSmem& sm, const GradGeo& 
     return __all_sync(0xFFFFFFFFu, mbar_wait<true>(bar, parity, sm.abort, site, p.wait_limit_ns)) != 0;
   };
   RingPos at_stage;
-  for (int i = item0; i < p.items; i += step) {
+  int turn = 0;  // the group of the next stage
+  ItemIter items(p, item0, step);
+  for (int i = items.next(); i >= 0; i = items.next()) {
     const Item item = item_of(p, i);
     const bool codes = item.mb->scale != nullptr;
     TileIter it(p.plan, item.a, rank, count);
     int t0, rows;
     for (; it.next(t0, rows); at_stage.next(geo.stages)) {
+      const bool ours = turn == group;
+      turn ^= 1;
+      if (!ours) continue;
       const int s = at_stage.slot;
       const uint32_t ph = at_stage.phase;
       // the tile has landed (so the stage's last MMAs are done)
       if (!wait_all(smem_u32(&sm.full[s]), ph, kSiteGradFull | s)) return;
       const uint32_t xs = sm.tiles + s * geo.stage_bytes, parts = xs + geo.parts_off;
 #pragma unroll
-      for (int j = 0; j < TASKS; ++j) {
+      for (int j = 0; j < kPieces; ++j) {
         if (row_of[j] >= kRows) continue;
         // rows past the segment's last are another request's: zeros
         float f[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
@@ -294,8 +322,8 @@ __device__ void convert(const GradParams& p, const GradSmem& sm, const GradGeo& 
       }
       if (codes) {
 #pragma unroll
-        for (int j = 0; j < kRows * kTileF / 16 / kConvThreads; ++j) {  // 16 codes of a row at a time
-          const int e = tid + j * kConvThreads, row = e / (kTileF / 16), c = e % (kTileF / 16);
+        for (int j = 0; j < kRows * kTileF / 16 / kConvGroup; ++j) {  // 16 codes of a row at a time
+          const int e = tid + j * kConvGroup, row = e / (kTileF / 16), c = e % (kTileF / 16);
           uint4 q = ld_shared_v4(xs + geo.code_off + row * kTileF + c * 16);
           if (row >= rows) q = make_uint4(0, 0, 0, 0);
           const uint32_t qw[4] = {q.x, q.y, q.z, q.w};
@@ -317,7 +345,7 @@ __device__ void convert(const GradParams& p, const GradSmem& sm, const GradGeo& 
       } else if (rows < kRows) {
         // an infinity or NaN in the rows after the segment's last would come
         // through a product with 0
-        for (int e = rows * 8 + tid; e < kRows * 8; e += kConvThreads) {
+        for (int e = rows * 8 + tid; e < kRows * 8; e += kConvGroup) {
           st_shared_v4(xs + e * 16, 0, 0, 0, 0);
           st_shared_v4(xs + kBoxBytes + e * 16, 0, 0, 0, 0);
         }
@@ -355,7 +383,7 @@ __global__ void __launch_bounds__(kGradThreads<TASKS>, TASKS == 1 ? 2 : 1)
   if (threadIdx.x == 0) {
     for (int s = 0; s < geo.stages; ++s) {
       mbar_init(smem_u32(&sm.full[s]), 33);  // the producer's lane 0 with the copies' bytes, and every lane
-      mbar_init(smem_u32(&sm.conv[s]), kConvThreads / 32);
+      mbar_init(smem_u32(&sm.conv[s]), kConvGroup / 32);
       mbar_init(smem_u32(&sm.empty[s]), 1);
     }
     for (int b = 0; b < 2; ++b) {
@@ -385,7 +413,8 @@ __global__ void __launch_bounds__(kGradThreads<TASKS>, TASKS == 1 ? 2 : 1)
     RingPos at_stage;
     int sent = 0;
     bool ok = true;
-    for (int i = item0; i < p.items && ok; i += step) {
+    ItemIter items(p, item0, step);
+    for (int i = items.next(); i >= 0 && ok; i = items.next()) {
       const Item item = item_of(p, i);
       const GradMember& mb = *item.mb;
       const bool codes = mb.scale != nullptr;
@@ -428,7 +457,8 @@ __global__ void __launch_bounds__(kGradThreads<TASKS>, TASKS == 1 ? 2 : 1)
       const uint32_t id1 = make_idesc_bf16(kTileF, pc.n1) | mn, id2 = make_idesc_bf16(kTileF, pc.n2) | mn;
       RingPos at_stage, at_acc;  // stages and accumulators filled
       bool ok = true;
-      for (int i = item0; i < p.items && ok; i += step) {
+      ItemIter items(p, item0, step);
+      for (int i = items.next(); i >= 0 && ok; i = items.next()) {
         const int tiles = TileIter(p.plan, item_of(p, i).a, rank, count).total();
         for (int k = 0; k < tiles; ++k, at_stage.next(geo.stages)) {
           const int s = at_stage.slot, b = at_acc.slot;
@@ -472,7 +502,8 @@ __global__ void __launch_bounds__(kGradThreads<TASKS>, TASKS == 1 ? 2 : 1)
     float sums[kSumCols<TASKS>];  // one feature, consecutive ranks
     RingPos at_acc;
     bool ok = true;
-    for (int i = item0; i < p.items && ok; i += step) {
+    ItemIter items(p, item0, step);
+    for (int i = items.next(); i >= 0 && ok; i = items.next()) {
       const Item item = item_of(p, i);
       const int tiles = TileIter(p.plan, item.a, rank, count).total();
 #pragma unroll

@@ -159,12 +159,14 @@ struct ProjParams {
 // chunk[i]: the live requests' rows in runs of at most kChunkRows, as {first
 //   row, rows | q << 8, adapter, strength bits}; unused: 0 rows.
 // seg[begin[a]] .. seg[begin[a + 1] - 1]: the row ranges of adapter a.
-// row_adapter[row]: the adapter of the row's live request, else -1.
+// by_rows[0 .. cap): the adapters, those with the most tiles of 64 rows first.
+// row_adapter[row], row < kFewRows: the adapter of the row's live request, else -1.
 constexpr int kPlanLevels = 4;      // token tiles of 64, 128, 256 and 512 rows
 constexpr int kChunkRows = 8;
 constexpr int kMaxRequests = 4096;
 constexpr int kMaxAdapters = 4096;
 constexpr int kMaxAdapterRank = 128;
+constexpr int kFewRows = 32;        // rows that few_rows_kernel takes, at most
 
 struct RequestPlan {
   int32_t n_req, m, cap;
@@ -176,6 +178,7 @@ struct RequestPlan {
   int4* chunk;
   int2* seg;
   int32_t* begin;
+  int32_t* by_rows;
   int32_t* row_adapter;
 };
 
@@ -224,8 +227,6 @@ struct RankParams {
 };
 
 // y = x W^T + v B^T of at most kFewRows rows (few_rows_kernel).
-constexpr int kFewRows = 32;
-
 struct FewParams {
   const uint16_t* x;  // bf16 [m][ldx]
   int64_t ldx;

@@ -75,6 +75,7 @@ __device__ __forceinline__ int last_at(const int* start, int n, int row) {
 __global__ void __launch_bounds__(kPlanThreads) plan_requests_kernel(const __grid_constant__ PlanParams p) {
   __shared__ int start[kMaxRequests + 1];
   __shared__ int adapter[kMaxRequests];
+  __shared__ uint16_t tiles_of[kMaxAdapters];  // tiles of 64 rows (at most 2^13 + kMaxRequests)
   __shared__ int warp_sums[32];
   const RequestPlan& pl = p.plan;
   const int n = pl.n_req, tid = threadIdx.x;
@@ -157,12 +158,23 @@ __global__ void __launch_bounds__(kPlanThreads) plan_requests_kernel(const __gri
     pl.seg[place] = make_int2(start[q], start[q + 1]);
   }
   for (int a = tid; a <= pl.cap; a += kPlanThreads) {
-    int below = 0;
-    for (int j = 0; j < n; ++j) below += (adapter[j] >= 0 && adapter[j] < a) ? 1 : 0;
+    int below = 0, tiles = 0;
+    for (int j = 0; j < n; ++j) {
+      below += (adapter[j] >= 0 && adapter[j] < a) ? 1 : 0;
+      if (adapter[j] == a) tiles += (start[j + 1] - start[j] + 63) / 64;
+    }
     pl.begin[a] = below;
+    if (a < pl.cap) tiles_of[a] = static_cast<uint16_t>(tiles);
+  }
+  __syncthreads();
+  for (int a = tid; a < pl.cap; a += kPlanThreads) {
+    const int mine = tiles_of[a];
+    int place = 0;
+    for (int b = 0; b < pl.cap; ++b) place += (tiles_of[b] > mine || (tiles_of[b] == mine && b < a)) ? 1 : 0;
+    pl.by_rows[place] = a;
   }
 
-  for (int r = tid; r < pl.m; r += kPlanThreads)
+  for (int r = tid; r < min(pl.m, kFewRows); r += kPlanThreads)
     pl.row_adapter[r] = r < start[n] ? adapter[last_at(start, n, r)] : -1;
 
   // blocks and lists of every level's token tiles
