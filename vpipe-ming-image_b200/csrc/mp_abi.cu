@@ -641,6 +641,37 @@ SplitChoice choose_ksplit(int m, int pairs, int base_kt, int r, int max_split = 
   return best;
 }
 
+// Token tile and K splits of a projection whose requests bring their adapters, the
+// least of: rounds of 74 pairs x (64-wide stages x cycles + 6000) at 1900 cycles a
+// us, and for a split launch 14 us (partial sums written row by row, the second
+// launch, the appended tiles in one split) plus the partial sums' traffic at 4
+// TB/s. The cycles are what such calls take over 64 to 1024 rows, w4 and w8: the
+// pace of the dequantizing warps more than of the tile's size. Against
+// choose_ksplit and pick_ntok_pair, which stay with the calls that had them, at 8
+// requests: w4 10240x3840 300 rows 88 -> 56 us, 1024 rows 125 -> 101; bf16 648x640
+// 333 rows 23 -> 16; w8 3840x3840 517 rows 57 -> 50.
+SplitChoice choose_requests_tile(int m, int pairs, int base_kt, int n, int max_split) {
+  SplitChoice best{kMaxTileTok, 1, 0.0};
+  double best_us = 1e300;
+  const int tiles[4] = {512, 256, 128, 64};
+  const double stage[4] = {1370.0, 1230.0, 1130.0, 1050.0};
+  for (int i = 0; i < 4; ++i) {
+    const long long units = pairs * static_cast<long long>((m + tiles[i] - 1) / tiles[i]);
+    for (int s = 1; s <= max_split && s <= base_kt; ++s) {
+      const int kps = (base_kt + s - 1) / s;
+      if ((base_kt + kps - 1) / kps != s) continue;  // every split gets at least one tile
+      const long long waves = (units * s + 73) / 74;
+      double us = static_cast<double>(waves) * (kps * stage[i] + 6000.0) / 1900.0;
+      if (s > 1) us += 14.0 + (static_cast<double>(s) * 4.0 + 2.0) * m * n / 4.0e6;
+      if (us < best_us * 0.999) {  // ties go to the wider tile and fewer splits
+        best_us = us;
+        best = SplitChoice{tiles[i], s, us};
+      }
+    }
+  }
+  return best;
+}
+
 }  // namespace mp
 
 namespace {
@@ -789,8 +820,11 @@ int launch_projections(mp_ctx* c, const mp_weight* const* ws, void* const* ys,
     const size_t per_split = static_cast<size_t>(mi) * ns[0] * sizeof(float);
     const int most = static_cast<int>(
         std::min<size_t>(mp::kMaxSplits, std::max<size_t>(1, kSplitBytes / per_split)));
-    msplit = mp::choose_ksplit(mi, pairs_of(ns[0]), base_kt, ns[0], most);
-    if (msplit.ksplit > 1) n_tok = msplit.n_tok;
+    msplit = ext != nullptr ? mp::choose_requests_tile(mi, pairs_of(ns[0]), base_kt, ns[0], most)
+                            : mp::choose_ksplit(mi, pairs_of(ns[0]), base_kt, ns[0], most);
+    if (msplit.ksplit > 1 || ext != nullptr) n_tok = msplit.n_tok;
+  } else if (ext != nullptr) {
+    n_tok = mp::choose_requests_tile(mi, pairs_of(ns[0]), (ws[0]->d.k + mp::kBlockK - 1) / mp::kBlockK, ns[0], 1).n_tok;
   }
   // With `sep` (live slots whose rank-space pre-GEMM has not run yet), a
   // split-K launch runs the pre-GEMM, its reduce and the LoRA K tiles (as a
