@@ -105,6 +105,7 @@ CASES = [
     (33, 264, 192, 2, 40, [0, 33, 0], [0, 1, 0], [1.0, 0.3, 1.0]),
     (64, 128, 320, 5, 64, [8] * 8, [0, 1, 2, 3, 4, 0, -1, 2], [1.0] * 8),
     (130, 136, 192, 3, 17, [63, 1, 64], [2, 0, 1], [1.0, 2.0, -1.0]),  # ends inside and on a tile
+    (200, 192, 128, 7, 16, [1] * 200, [(3 * i) % 8 - 1 for i in range(200)], [1.0] * 200),  # a token each
     (300, 256, 256, 4, 128, [129, 5, 100], [3, 0, 3], [0.2, 1.0, 1.0]),  # one adapter twice, rows left over
     (517, 648, 640, 6, 24, [50, 51, 0, 200, 3, 1, 212], [5, 4, 3, 2, 1, -1, 0], [1, 1, 1, 0.0, 1, 1, 1.5]),
     (1100, 512, 512, 2, 80, [600, 500], [1, 0], [1.0, 1.0]),
@@ -132,6 +133,51 @@ def test_linear_requests(ctx, bits, mode, case):
     _within("v", v, rv, bv)
     assert torch.equal(y, again), "the same call twice"
     for h in (w, bank, plan):
+        h.free()
+
+
+LONG = [
+    # enough to multiply for the tensor-core kernels, K split in clusters and not;
+    # long runs of rows for one adapter (the sums of dA and dB)
+    (2100, 384, 640, 3, 128, [1500, 1, 0, 590], [1, 0, 2, 1], [1.0, 1.0, 1.0, -0.5]),
+    (5000, 264, 1032, 2, 20, [4990], [1], [0.7]),
+    (4100, 1024, 768, 12, 64, [300, 257, 511, 64, 1, 900, 128, 640, 777, 33, 400], list(range(11)), [1.0] * 11),
+    (700, 256, 3328, 5, 48, [100, 128, 130, 12, 330], [0, 1, 4, 2, 3], [1.0, -1.0, 0.25, 1.0, 0.0]),
+]
+
+
+@pytest.mark.parametrize("case", LONG, ids=[f"m{c[0]}_n{c[1]}_k{c[2]}_r{c[4]}" for c in LONG])
+@pytest.mark.parametrize("saved", [16, 8])
+def test_long_requests(ctx, case, saved):
+    m, n, k, cap, max_rank, lengths, adapters, strengths = case
+    rng = np.random.default_rng(3 * m + n + saved)
+    w, w64, wround = _weight(ctx, rng, n, k, 0)
+    bank, fac = _bank(ctx, rng, n, k, cap, max_rank, [max(1, max_rank - 3 * i) for i in range(cap)], training=True)
+    plan = ctx.requests(len(lengths), m, cap)
+    plan.plan(lengths, adapters, strengths, m)
+    x, dy = _bf16(rng, m, k), _bf16(rng, m, n, scale=0.1)
+    segs = list(_segments(m, lengths, adapters, strengths))
+    y, v = ctx.linear_requests(w, x, bank, plan, ranks=True)
+    wt = ctx.transposed(w)
+    x_in = ctx.checkpoint(x) if saved == 8 else x
+    kept = x if saved == 16 else x_in.codes.double() * x_in.scales.double().repeat_interleave(128, 1)[:, :k]
+    dx, da, db = ctx.linear_requests_grad(wt, dy, x_in, v, bank, plan)
+    again = ctx.linear_requests_grad(wt, dy, x_in, v, bank, plan)
+    ctx.sync_check()
+    ry, by, rv, bv = _forward_ref(x, w64, wround, fac, segs, bank.rank_pad)
+    _within("y", y, ry, by)
+    _within("v", v, rv, bv)
+    rx, ra, rb = _grad_ref(kept, dy, w64, wround, fac, segs, v, cap, max_rank)
+    _within("dx", dx, *rx)
+    _within("da", da, *ra)
+    _within("db", db, *rb)
+    for name, got, ref in (("v", v, rv), ("da", da, ra[0]), ("db", db, rb[0])):
+        # as near as sums in f32 with rounding to nearest come at these lengths:
+        # 2^-24 of the result a term, added at random, and 2^-17 of a factor
+        off = ((got.double() - ref).norm() / ref.norm()).item()
+        assert off <= 2.0 ** -24 * math.sqrt(m + n + k) + 2.0 ** -17, f"{name}: {off:.3g}"
+    assert all(torch.equal(a, b) for a, b in zip((dx, da, db), again)), "the same call twice"
+    for h in (w, wt, bank, plan):
         h.free()
 
 

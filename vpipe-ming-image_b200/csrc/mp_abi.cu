@@ -2212,8 +2212,8 @@ int mp_adapters_create(mp_ctx* c, int n, int k, int capacity, int max_rank, int 
     return fail(c, MP_EINVAL, "capacity %d outside [1, %d]", capacity, mp::kMaxAdapters);
   if (max_rank <= 0 || max_rank > mp::kMaxAdapterRank)
     return fail(c, MP_EINVAL, "max_rank %d outside [1, %d]", max_rank, mp::kMaxAdapterRank);
-  if (static_cast<int64_t>(capacity) * std::max(n, k) > INT_MAX)
-    return fail(c, MP_EINVAL, "capacity * max(n, k) exceeds 2^31 rows");
+  if (static_cast<int64_t>(capacity) * std::max(n, k) > INT_MAX - 1024)  // rows of the factors' tensor maps
+    return fail(c, MP_EINVAL, "capacity * max(n, k) exceeds 2^31 - 1024 rows");
   int rc = use_device(c);
   if (rc != MP_OK) return rc;
   mp_adapters* b = new (std::nothrow) mp_adapters();
