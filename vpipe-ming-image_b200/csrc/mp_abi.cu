@@ -781,6 +781,7 @@ struct RequestsLaunch {
   const CUtensorMap* tm_b = nullptr;
   float* v32 = nullptr;         // also kept in f32 (nullable)
   int64_t ld32 = 0;
+  bool clear = false;           // zeros there for the rows without an adapter
 };
 
 int launch_request_ranks(mp_ctx* c, ProjParams* p, const RequestsLaunch& ext, const void* x, int64_t ldx,
@@ -2063,6 +2064,7 @@ mp::RankParams rank_params(const mp_ctx* c, const RequestsLaunch& ext, const voi
   r.plan = ext.req->plan;
   r.v32 = ext.v32;
   r.ld32 = ext.ld32;
+  r.clear_v32 = ext.clear ? 1 : 0;
   r.lvl = 1;  // 128-row tiles, where no blocks are asked for
   r.wait_limit_ns = c->wait_limit_ns;
   r.err = c->err_word;
@@ -2086,10 +2088,6 @@ int launch_ranks(mp_ctx* c, const RequestsLaunch& ext, mp::RankParams* r, cudaSt
     r->tm_f = *ext.tm_f;
     e = mp::launch_rank_tiles(*r, stream);
   } else {
-    if (r->vblk != nullptr) {
-      const size_t rows = static_cast<size_t>(mp::plan_blocks(pl.m, pl.n_req, r->lvl)) << (6 + r->lvl);
-      MP_CUDA(c, cudaMemsetAsync(r->vblk, 0, rows * r->ldb * sizeof(uint16_t), stream));
-    }
     e = mp::launch_rank_rows(*r, stream);
   }
   if (e != cudaSuccess) return cuda_fail(c, e, tiles ? "rank_tiles_kernel" : "rank_rows_kernel");
@@ -2126,7 +2124,7 @@ int launch_request_ranks(mp_ctx* c, ProjParams* p, const RequestsLaunch& ext, co
   p->ext_live = pl.live[level];
   p->ext_list = pl.list[level];
   p->ext_chunks = chunks;
-  p->late_wait = pl.n_req > 0 ? 1 : 0;  // without requests there may be no rank-space launch
+  p->late_wait = 1;
   return MP_OK;
 }
 
@@ -2163,7 +2161,7 @@ int run_requests(mp_ctx* c, const mp_weight* w, const void* x, int64_t ldx, void
     p.row_adapter = ext->req->plan.row_adapter;
     p.y = static_cast<uint16_t*>(y);
     p.ldy = ldy;
-    p.chunks = mp::plan_chunks(m, ext->req->plan.n_req);
+    p.chunks = mp::plan_chunks(m, ext->req->plan.n_req) + (ext->clear ? 1 : 0);
     cudaError_t e = mp::launch_few_rows(p, w->d.bits, stream);
     if (e != cudaSuccess) return cuda_fail(c, e, "few_rows_kernel");
     c->eng.kernels += 1;
@@ -2326,7 +2324,7 @@ int mp_requests_create(mp_ctx* c, int max_requests, int max_rows, int capacity, 
     return at;
   };
   for (int l = 0; l < mp::kPlanLevels; ++l) {
-    const size_t tiles = mp::plan_tiles(max_rows, l), blocks = tiles + q;
+    const size_t tiles = mp::plan_tiles(max_rows, l), blocks = mp::plan_blocks(max_rows, max_requests, l);
     at_block[l] = take(4 * blocks);
     at_s[l] = take(blocks);
     at_list[l] = take(2 * blocks);
@@ -2411,8 +2409,7 @@ int mp_linear_requests(mp_ctx* c, const mp_weight* w, const void* x, int64_t ldx
   ext.tm_b = &b->tm_b;
   ext.v32 = ranks;
   ext.ld32 = ldr;
-  if (ranks != nullptr)  // rows without an adapter
-    MP_CUDA(c, cudaMemset2DAsync(ranks, static_cast<size_t>(ldr) * 4, 0, static_cast<size_t>(b->rp) * 4, m, s));
+  ext.clear = ranks != nullptr;
   return run_requests(c, w, x, ldx, y, ldy, m, &ext, s);
 }
 

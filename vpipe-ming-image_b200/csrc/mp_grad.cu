@@ -29,6 +29,7 @@
 
 #include "mp_device.cuh"
 #include "mp_kernels.h"
+#include "mp_launch.h"
 
 namespace mp {
 
@@ -614,8 +615,8 @@ __global__ void __launch_bounds__(kGradThreads<TASKS>, TASKS == 1 ? 2 : 1)
 
 template <int TASKS>
 cudaError_t launch_tasks(const GradParams& p, uint32_t smem, unsigned grid, cudaStream_t stream) {
-  cudaError_t e = cudaFuncSetAttribute(adapter_grad_kernel<TASKS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       static_cast<int>(smem));
+  static SmemOptIn opted;
+  cudaError_t e = opted.allow(reinterpret_cast<const void*>(adapter_grad_kernel<TASKS>));
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid);

@@ -153,8 +153,9 @@ struct ProjParams {
 // request is LIVE when it has rows, an adapter and a strength that is not 0.
 // Per level l, for token tiles of T = 64 << l rows:
 //   block[l][t + q] = {t, first row, row past the last, adapter} for the rows
-//     of live request q in tile t, block_s its strength; adapter -1 where
-//     there are none. (Rows are in request order, so t + q is one pair's only.)
+//     of request q in tile t (q = n_req: the rows after the last request),
+//     block_s its strength; adapter -1 where it is not live, and no rows where
+//     it has none in t. (Rows are in request order, so t + q is one pair's only.)
 //   list[l][first[l][t] + i], i < live[l][t]: tile t's {block, adapter}.
 // chunk[i]: the live requests' rows in runs of at most kChunkRows, as {first
 //   row, rows | q << 8, adapter, strength bits}; unused: 0 rows.
@@ -183,7 +184,7 @@ struct RequestPlan {
 };
 
 inline __host__ __device__ int plan_tiles(int m, int level) { return (m + (64 << level) - 1) / (64 << level); }
-inline __host__ __device__ int plan_blocks(int m, int n_req, int level) { return plan_tiles(m, level) + n_req; }
+inline __host__ __device__ int plan_blocks(int m, int n_req, int level) { return plan_tiles(m, level) + n_req + 1; }
 inline __host__ __device__ int plan_chunks(int m, int n_req) { return m / kChunkRows + n_req; }
 
 struct PlanParams {
@@ -218,7 +219,8 @@ struct RankParams {
   const int32_t* bad;
   RequestPlan plan;
   // outputs (either may be null)
-  float* v32;         // f32 [m][ld32], columns < rp; live rows only
+  float* v32;         // f32 [m][ld32], columns < rp; with clear_v32 zeros in the
+  int32_t clear_v32;  // rows of requests that are not live, which else keep theirs
   int64_t ld32;
   uint16_t* vblk;     // bf16 blocks of 64 << lvl rows by plan block, width ldb
   int32_t lvl, ldb;

@@ -24,6 +24,7 @@
 
 #include "mp_device.cuh"
 #include "mp_kernels.h"
+#include "mp_launch.h"
 
 namespace mp {
 
@@ -77,7 +78,8 @@ struct RankUnit {
   int row0;       // first row of x
   int lo, hi;     // the request's rows, from row0
   int adapter;
-  bool work;
+  bool work;      // of a live request
+  bool clear;     // rows of v32 to clear: not of a live request
   int64_t out;    // row of vblk for row0
   int zero0, zero1, zero2, zero3;  // rows of vblk to clear besides: [zero0, zero1) and [zero2, zero3), from `out`
 };
@@ -94,6 +96,7 @@ __device__ __forceinline__ RankUnit rank_unit(const RankParams& p, int i) {
   const int4 ent = p.plan.block[ul][i];  // {tile, first row, row past the last, adapter}
   u.adapter = ent.w;
   u.work = ent.w >= 0;
+  u.clear = ent.w < 0 && p.clear_v32 && ent.y < ent.z;
   u.row0 = ent.x << (6 + ul);
   u.lo = ent.y - u.row0;
   u.hi = ent.z - u.row0;
@@ -118,9 +121,16 @@ __device__ __forceinline__ float unit_scale(const RankParams& p, const RankUnit&
   return p.bad[u.adapter] != 0 ? __int_as_float(0x7FC00000) : p.plan.block_s[unit_level(p)][u.unit];
 }
 
-// The unit's rows of vblk outside its 128, by threads `tid` of `threads`.
+// The unit's rows of vblk outside its 128, or its rows of v32 if its request is
+// not live, by threads `tid` of `threads`.
 __device__ __forceinline__ void clear_rows(const RankParams& p, const RankUnit& u, int tid, int threads) {
-  if (p.vblk == nullptr) return;
+  if (u.clear) {
+    for (int e = tid; e < (u.hi - u.lo) * p.rp / 4; e += threads) {
+      const int r = u.row0 + u.lo + e / (p.rp / 4), c = e % (p.rp / 4) * 4;
+      *reinterpret_cast<float4*>(p.v32 + static_cast<int64_t>(r) * p.ld32 + c) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    }
+  }
+  if (!u.work || p.vblk == nullptr) return;
   const int per_row = p.ldb / 8;
   uint4* at = reinterpret_cast<uint4*>(p.vblk + u.out * p.ldb);
   for (int e = u.zero0 * per_row + tid; e < u.zero1 * per_row; e += threads) at[e] = make_uint4(0, 0, 0, 0);
@@ -243,7 +253,10 @@ __global__ void __launch_bounds__(kRankThreads, COLS <= 64 ? 2 : 1) rank_tiles_k
     bool ok = true;
     for (int unit = unit0; unit < p.units && ok; unit += step) {
       const RankUnit u = rank_unit(p, unit);
-      if (!u.work) continue;
+      if (!u.work) {
+        if (count == 1) clear_rows(p, u, threadIdx.x - 32 * kSumWarp0, 32 * 4);
+        continue;
+      }
 #pragma unroll
       for (int c = 0; c < COLS; ++c) sums[c] = 0.0f;
       for (int k = 0; k < n_kt; k += kChunk, ++chunk) {
@@ -342,8 +355,8 @@ __global__ void __launch_bounds__(kRankThreads, COLS <= 64 ? 2 : 1) rank_tiles_k
 template <int COLS>
 cudaError_t launch_cols(const RankParams& p, unsigned ctas, cudaStream_t stream) {
   const uint32_t smem = rank_geo(p.rp).smem;
-  cudaError_t e = cudaFuncSetAttribute(rank_tiles_kernel<COLS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       static_cast<int>(smem));
+  static SmemOptIn opted;
+  cudaError_t e = opted.allow(reinterpret_cast<const void*>(rank_tiles_kernel<COLS>));
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(ctas);

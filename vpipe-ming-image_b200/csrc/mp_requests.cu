@@ -185,19 +185,20 @@ __global__ void __launch_bounds__(kPlanThreads) plan_requests_kernel(const __gri
     for (int t = tid; t < tiles; t += kPlanThreads) {
       const int row0 = t * tile, row1 = min(row0 + tile, pl.m);
       int live = 0, first = 0;
-      if (n > 0 && row0 < start[n]) {
+      if (row0 < start[n]) {
         const int q0 = last_at(start, n, row0);
         first = t + q0;
         for (int q = q0; q < n && start[q] < row1; ++q) {
-          if (adapter[q] < 0) continue;
           const int lo = max(start[q], row0), hi = min(start[q + 1], row1);
           if (lo >= hi) continue;
           pl.block[l][t + q] = make_int4(t, lo, hi, adapter[q]);
+          if (adapter[q] < 0) continue;
           pl.block_s[l][t + q] = p.strengths != nullptr ? p.strengths[q] : 1.0f;
           pl.list[l][first + live] = make_int2(t + q, adapter[q]);
           ++live;
         }
       }
+      if (row1 > start[n]) pl.block[l][t + n] = make_int4(t, max(start[n], row0), row1, -1);
       pl.first[l][t] = first;
       pl.live[l][t] = live;
     }
@@ -293,8 +294,28 @@ __device__ __forceinline__ void load16(const uint16_t* row, int c, int k, bool o
 constexpr int kRankWarps = 16;
 constexpr int kRankBatch = 4;  // K groups a warp has in flight
 
+// What no chunk writes of the plan's block `blk`: for a live request its block of
+// vblk but for the request's rows and ranks, otherwise the rows of v32.
+__device__ void clear_block(const RankParams& p, int blk, int tid, int threads) {
+  const int4 ent = p.plan.block[p.lvl][blk];
+  if (ent.w >= 0 && p.vblk != nullptr) {
+    const int rows = 64 << p.lvl, row0 = ent.x << (6 + p.lvl), quads = p.ldb / 8, own = p.rp / 8;
+    uint4* at = reinterpret_cast<uint4*>(p.vblk + (static_cast<int64_t>(blk) << (6 + p.lvl)) * p.ldb);
+    for (int e = tid; e < rows * quads; e += threads) {
+      const int r = row0 + e / quads;
+      if (r < ent.y || r >= ent.z || e % quads >= own) at[e] = make_uint4(0, 0, 0, 0);
+    }
+  } else if (ent.w < 0 && p.clear_v32) {
+    for (int e = tid; e < (ent.z - ent.y) * p.rp / 4; e += threads) {
+      const int r = ent.y + e / (p.rp / 4), c = e % (p.rp / 4) * 4;
+      *reinterpret_cast<float4*>(p.v32 + static_cast<int64_t>(r) * p.ld32 + c) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    }
+  }
+}
+
 // One block: 16 ranks of one chunk (at most 8 rows of one request); its warps
-// take the 64-wide K groups in turn and their sums are added in warp order.
+// take the 64-wide K groups in turn and their sums are added in warp order. The
+// blocks after the chunks' clear what no chunk writes.
 // Within a group lane (g, j) (g = lane / 4, j = lane % 4) holds columns
 // 16 j .. 16 j + 15 of ranks g and g + 8 and of row g: both operands of the
 // four MMAs of a group then come from two 16-byte loads each, the K columns
@@ -305,6 +326,11 @@ __global__ void __launch_bounds__(32 * kRankWarps) rank_rows_kernel(const __grid
   __shared__ float part[kRankWarps][16][kChunkRows];
   pdl_wait();
   pdl_release();
+  const int chunks = plan_chunks(p.plan.m, p.plan.n_req);
+  if (static_cast<int>(blockIdx.x) >= chunks) {
+    if (blockIdx.y == 0) clear_block(p, static_cast<int>(blockIdx.x) - chunks, threadIdx.x, 32 * kRankWarps);
+    return;
+  }
   const int4 ch = p.plan.chunk[blockIdx.x];
   const int rows = ch.y & 0xFF;
   if (rows == 0) return;
@@ -629,7 +655,9 @@ cudaError_t launch_bank_set(const BankSetParams& p, cudaStream_t stream) {
 }
 
 cudaError_t launch_rank_rows(const RankParams& p, cudaStream_t stream) {
-  const dim3 grid(plan_chunks(p.plan.m, p.plan.n_req), p.rp / 16);
+  const bool clear = p.vblk != nullptr || p.clear_v32;
+  const int blocks = clear ? plan_blocks(p.plan.m, p.plan.n_req, p.lvl) : 0;
+  const dim3 grid(plan_chunks(p.plan.m, p.plan.n_req) + blocks, p.rp / 16);
   if (grid.x == 0) return cudaSuccess;  // no request
   return launch_overlapped(rank_rows_kernel, grid, dim3(32 * kRankWarps), p, stream);
 }

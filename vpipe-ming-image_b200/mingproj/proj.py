@@ -248,6 +248,13 @@ def _rows(name: str, t: torch.Tensor, m: int, k: int, dtype=torch.bfloat16) -> i
     return _bad_rows(name, t, m, k, dtype)
 
 
+def _new_rows(like: torch.Tensor, m: int, n: int) -> tuple[torch.Tensor, int]:
+    """bf16 rows [m, n] beside `like`, and their pitch (a multiple of 8)."""
+    ld = (n + 7) // 8 * 8
+    out = like.new_empty((m, ld), dtype=torch.bfloat16)
+    return (out if ld == n else out[:, :n]), ld
+
+
 def _check_scales(t: torch.Tensor, m: int, k: int) -> None:
     groups = (k + 127) // 128
     if not (t.dtype is torch.float32 and t.shape == (m, groups) and t.is_cuda
@@ -534,14 +541,17 @@ class Context:
         n, k = w.info.n, w.info.k
         ldx = _rows("x", x, m, k)
         if out is None:
-            out = x.new_empty((m, n)) if n % 8 == 0 else _alloc_out(m, n, x.device)
-        ldy = _rows("out", out, m, n)
+            out, ldy = _new_rows(x, m, n)
+        else:
+            ldy = _rows("out", out, m, n)
         v, vp, ldv = None, None, 0
         if ranks is not False and ranks is not None:
             v = ranks
             if ranks is True:
                 v = x.new_empty((m, bank.rank_pad), dtype=torch.float32)
-            ldv = _rows("ranks", v, m, bank.rank_pad, torch.float32)
+                ldv = bank.rank_pad
+            else:
+                ldv = _rows("ranks", v, m, bank.rank_pad, torch.float32)
             vp = v.data_ptr()
         rc = self.lib.mp_linear_requests(
             self.h, w.handle, x.data_ptr(), ldx, bank.handle, plan.handle, out.data_ptr(), ldy, vp,
@@ -570,8 +580,7 @@ class Context:
         dxp = dap = dbp = xp = qp = sp = vp = None
         lddx = ldx = ldq = ldv = 0
         if need_dx:
-            dx = dy.new_empty((m, k)) if k % 8 == 0 else _alloc_out(m, k, dy.device)
-            lddx = _rows("dx", dx, m, k)
+            dx, lddx = _new_rows(dy, m, k)
             dxp = dx.data_ptr()
         if need_factors:
             if isinstance(x, Checkpoint):
@@ -616,8 +625,9 @@ class Context:
         ldq = _rows("codes", saved.codes, m, k, torch.int8)
         _check_scales(saved.scales, m, k)
         if out is None:
-            out = _alloc_out(m, k, saved.codes.device)
-        ldx = _rows("out", out, m, k)
+            out, ldx = _new_rows(saved.scales, m, k)
+        else:
+            ldx = _rows("out", out, m, k)
         rc = self.lib.mp_restore(self.h, saved.codes.data_ptr(), ldq, saved.scales.data_ptr(), m, k,
                                  out.data_ptr(), ldx, _stream_handle(stream))
         if rc != MP_OK:
