@@ -381,6 +381,20 @@ __global__ void __launch_bounds__(kGradThreads<TASKS>, TASKS == 1 ? 2 : 1)
   sm.done = sm.taken + 2;
   sm.tmem_slot = reinterpret_cast<uint32_t*>(sm.done + 1);
   sm.abort = sm.tmem_slot + 1;
+  if (count > 1) {
+    // an adapter without rows: its cluster writes zeros and leaves before any set-up
+    pdl_wait();
+    const Item item = item_of(p, item0);
+    if (p.plan.begin[item.a] == p.plan.begin[item.a + 1]) {
+      pdl_release();
+      const int f0 = item.f_tile * kTileF, width = min(kTileF, item.mb->width - f0);
+      float* out = item.mb->out + static_cast<int64_t>(item.a) * p.r * item.mb->width;
+      for (int e = rank * kGradThreads<TASKS> + threadIdx.x; e < p.r * width; e += count * kGradThreads<TASKS>)
+        out[item.mb->rank_major ? static_cast<int64_t>(e / width) * item.mb->width + f0 + e % width
+                                : static_cast<int64_t>(f0) * p.r + e] = 0.0f;
+      return;
+    }
+  }
   if (threadIdx.x == 0) {
     for (int s = 0; s < geo.stages; ++s) {
       mbar_init(smem_u32(&sm.full[s]), 33);  // the producer's lane 0 with the copies' bytes, and every lane

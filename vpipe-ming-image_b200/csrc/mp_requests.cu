@@ -458,10 +458,12 @@ __device__ __forceinline__ void few_x(const uint16_t* at, int col, int k, uint32
 // waits for it before the adapters' part. Rows past m repeat the last one: the
 // MMA's columns are independent, theirs are not stored.
 template <int BITS, int NT, int WARPS>
-__global__ void __launch_bounds__(32 * WARPS, NT > 2 ? 1 : 16 / WARPS)
+__global__ void __launch_bounds__(32 * WARPS, NT > 2 ? 1 : (NT == 1 && BITS == 4 ? 24 : 16) / WARPS)
     few_rows_kernel(const __grid_constant__ FewParams p) {
-  // K groups a warp loads at a time, one batch ahead: 128 bytes a lane in flight
-  constexpr int kBatch = BITS == 4 ? 4 : BITS == 8 ? 2 : 1;
+  // K groups a warp loads at a time, one batch ahead: 128 bytes a lane in flight;
+  // up to 8 rows of w4 half of that from 24 warps an SM, not 16 (10240x3840, one
+  // row: 13.8 -> 11.1 us; at 16 rows and w8 the registers do not stretch so far)
+  constexpr int kBatch = BITS == 4 ? (NT == 1 ? 2 : 4) : BITS == 8 ? 2 : 1;
   __shared__ float part[WARPS][16][8 * NT + 1];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, j = lane & 3;
   const int f0 = blockIdx.x * 16;
