@@ -118,7 +118,7 @@ __host__ __device__ inline GradGeo grad_geo(int rp, bool codes) {
   g.scale_off = g.code_off + (codes ? kCodeBytes : 0);
   g.stage_bytes = (g.scale_off + (codes ? kRows * 4 : 0) + 1023) / 1024 * 1024;
   // two CTAs an SM with up to 32 ranks (their accumulators take half of TMEM each)
-  const uint32_t half = 112 * 1024;
+  const uint32_t half = 113 * 1024;
   const bool two = rp <= 32 && 2 * g.stage_bytes + 1280 <= half;
   g.stages = static_cast<int>(((two ? half : kGradSmemMost) - 1280) / g.stage_bytes);
   if (g.stages > kMaxGradStages) g.stages = kMaxGradStages;
