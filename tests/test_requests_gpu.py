@@ -181,6 +181,31 @@ def test_long_requests(ctx, case, saved):
         h.free()
 
 
+@pytest.mark.parametrize("rank,saved", [(4, 8), (4, 16), (30, 16), (64, 8), (100, 16)])
+def test_gradients_repeat(ctx, rank, saved):
+    """Hundreds of passes in a row, nothing waited for between them: the same
+    bits every time, and no bounded wait given up."""
+    rng = np.random.default_rng(rank)
+    m, n, k, cap = 3000, 640, 896, 3
+    w, _, _ = _weight(ctx, rng, n, k, 0)
+    bank, _ = _bank(ctx, rng, n, k, cap, rank, [rank] * cap, training=True)
+    plan = ctx.requests(4, m, cap)
+    plan.plan([1300, 77, 900, 650], [0, 2, 2, 0], None, m)
+    x, dy = _bf16(rng, m, k), _bf16(rng, m, n)
+    wt = ctx.transposed(w)
+    _, v = ctx.linear_requests(w, x, bank, plan, ranks=True)
+    x_in = ctx.checkpoint(x) if saved == 8 else x
+    first = ctx.linear_requests_grad(wt, dy, x_in, v, bank, plan)
+    differ = torch.zeros((), dtype=torch.int64, device="cuda")
+    for _ in range(300):
+        for a, b in zip(first, ctx.linear_requests_grad(wt, dy, x_in, v, bank, plan)):
+            differ += (a != b).sum()
+    ctx.sync_check()
+    assert int(differ) == 0
+    for h in (w, wt, bank, plan):
+        h.free()
+
+
 def test_dense_any_k(ctx):
     """A dense weight with k not a multiple of 8, x's rows strided, NaN beside them."""
     rng = np.random.default_rng(5)

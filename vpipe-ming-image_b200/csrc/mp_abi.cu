@@ -813,10 +813,12 @@ int launch_projections(mp_ctx* c, const mp_weight* const* ws, void* const* ys,
   // split writes fp32 partial sums (the last one after the appended LoRA K
   // tiles), lora_reduce_kernel adds them in split order and rounds to bf16.
   // The split count and the token tile come from one image's rows, at most
-  // kSplitBytes of partial sums per image.
+  // kSplitBytes of partial sums per image. (With adapters by request the bytes
+  // alone are the limit: a gradient of 1497 rows with 8080 features in and 1280
+  // out has 15 tiles for 74 pairs unsplit.)
   mp::SplitChoice msplit{0, 1, 0.0};
-  if (may_alloc && count == 1 && swi == nullptr && hds == nullptr && pro == nullptr && mi <= kSplitRows &&
-      ns[0] % 4 == 0 && ldys[0] % 4 == 0 && reinterpret_cast<uintptr_t>(ys[0]) % 8 == 0) {
+  if (may_alloc && count == 1 && swi == nullptr && hds == nullptr && pro == nullptr &&
+      (mi <= kSplitRows || ext != nullptr) && ns[0] % 4 == 0 && ldys[0] % 4 == 0 && reinterpret_cast<uintptr_t>(ys[0]) % 8 == 0) {
     const int base_kt = (ws[0]->d.k + mp::kBlockK - 1) / mp::kBlockK;
     const size_t per_split = static_cast<size_t>(mi) * ns[0] * sizeof(float);
     const int most = static_cast<int>(
@@ -824,7 +826,7 @@ int launch_projections(mp_ctx* c, const mp_weight* const* ws, void* const* ys,
     msplit = ext != nullptr ? mp::choose_requests_tile(mi, pairs_of(ns[0]), base_kt, ns[0], most)
                             : mp::choose_ksplit(mi, pairs_of(ns[0]), base_kt, ns[0], most);
     if (msplit.ksplit > 1 || ext != nullptr) n_tok = msplit.n_tok;
-  } else if (ext != nullptr) {
+  } else if (ext != nullptr) {  // an output width that the partial sums' stores do not take
     n_tok = mp::choose_requests_tile(mi, pairs_of(ns[0]), (ws[0]->d.k + mp::kBlockK - 1) / mp::kBlockK, ns[0], 1).n_tok;
   }
   // With `sep` (live slots whose rank-space pre-GEMM has not run yet), a

@@ -44,7 +44,7 @@ constexpr int kChunk = 4;     // stages of an accumulator
 
 constexpr int kConvWarp0 = 2;
 constexpr int kConvThreads = 256;
-constexpr int kConvGroups = 2;  // of four warps, which take the stages in turn
+constexpr int kConvGroups = 2;  // of four warps: the even slots' and the odd slots'
 constexpr int kConvGroup = kConvThreads / kConvGroups;
 constexpr int kSumWarp0 = kConvWarp0 + kConvThreads / 32;
 // Warps that add up the accumulators: 4 hold a feature row of up to 64 ranks a
@@ -269,7 +269,6 @@ __device__ void convert(const GradParams& p, const GradSmem& sm, const GradGeo& 
     return __all_sync(0xFFFFFFFFu, mbar_wait<true>(bar, parity, sm.abort, site, p.wait_limit_ns)) != 0;
   };
   RingPos at_stage;
-  int turn = 0;  // the group of the next stage
   ItemIter items(p, item0, step);
   for (int i = items.next(); i >= 0; i = items.next()) {
     const Item item = item_of(p, i);
@@ -277,9 +276,11 @@ __device__ void convert(const GradParams& p, const GradSmem& sm, const GradGeo& 
     TileIter it(p.plan, item.a, rank, count);
     int t0, rows;
     for (; it.next(t0, rows); at_stage.next(geo.stages)) {
-      const bool ours = turn == group;
-      turn ^= 1;
-      if (!ours) continue;
+      // A slot is one group's for good: it then waits for each of the slot's phases,
+      // and none can pass without its arrival. (Stages in turn over an odd number
+      // of slots would have a group wait for every second phase of a slot, which a
+      // parity cannot tell from the one before.)
+      if (at_stage.slot % kConvGroups != group) continue;
       const int s = at_stage.slot;
       const uint32_t ph = at_stage.phase;
       // the tile has landed (so the stage's last MMAs are done)
@@ -381,17 +382,24 @@ __global__ void __launch_bounds__(kGradThreads<TASKS>, TASKS == 1 ? 2 : 1)
   sm.done = sm.taken + 2;
   sm.tmem_slot = reinterpret_cast<uint32_t*>(sm.done + 1);
   sm.abort = sm.tmem_slot + 1;
+  // Zeros of item i: an adapter without rows.
+  auto clear_item = [&](int i, int tid, int threads) {
+    const Item item = item_of(p, i);
+    const int f0 = item.f_tile * kTileF, width = min(kTileF, item.mb->width - f0);
+    float* out = item.mb->out + static_cast<int64_t>(item.a) * p.r * item.mb->width;
+    for (int e = tid; e < p.r * width; e += threads)
+      out[item.mb->rank_major ? static_cast<int64_t>(e / width) * item.mb->width + f0 + e % width
+                              : static_cast<int64_t>(f0) * p.r + e] = 0.0f;
+  };
   if (count > 1) {
-    // an adapter without rows: its cluster writes zeros and leaves before any set-up
+    // clusters of adapters without rows leave before any set-up
     pdl_wait();
     const Item item = item_of(p, item0);
     if (p.plan.begin[item.a] == p.plan.begin[item.a + 1]) {
       pdl_release();
-      const int f0 = item.f_tile * kTileF, width = min(kTileF, item.mb->width - f0);
-      float* out = item.mb->out + static_cast<int64_t>(item.a) * p.r * item.mb->width;
-      for (int e = rank * kGradThreads<TASKS> + threadIdx.x; e < p.r * width; e += count * kGradThreads<TASKS>)
-        out[item.mb->rank_major ? static_cast<int64_t>(e / width) * item.mb->width + f0 + e % width
-                                : static_cast<int64_t>(f0) * p.r + e] = 0.0f;
+      const int tid = rank * kGradThreads<TASKS> + threadIdx.x, threads = count * kGradThreads<TASKS>;
+      clear_item(item0, tid, threads);
+      for (int i = p.items + item0; i < p.all_items; i += step) clear_item(i, tid, threads);
       return;
     }
   }
@@ -624,6 +632,9 @@ __global__ void __launch_bounds__(kGradThreads<TASKS>, TASKS == 1 ? 2 : 1)
   }
   tc_fence_after();
   if (warp == 1) tmem_dealloc(tmem, pc.cols * pc.bufs);
+  // the adapters that are more than the requests
+  for (int i = p.items + item0; i < p.all_items; i += step)
+    clear_item(i, rank * kGradThreads<TASKS> + threadIdx.x, count * kGradThreads<TASKS>);
   if (threadIdx.x == 0 && aborted) atomicOr(p.err, kErrTimeout);
 }
 
@@ -659,13 +670,16 @@ cudaError_t launch_adapter_grad(const GradParams& p, cudaStream_t stream) {
     q.tiles += (p.mem[i].width + kTileF - 1) / kTileF;
     if (p.mem[i].scale != nullptr) q.codes = 1;
   }
-  const long long items = static_cast<long long>(q.tiles) * p.plan.cap;
-  if (items > (1 << 30)) return cudaErrorInvalidValue;
-  q.items = static_cast<int>(items);
+  const long long all_items = static_cast<long long>(q.tiles) * p.plan.cap;
+  if (all_items > (1 << 30)) return cudaErrorInvalidValue;
+  // Adapters come in the order of their rows, so those past the number of
+  // requests have none: their gradients are cleared by the way.
+  const int used = p.plan.cap < p.plan.n_req ? p.plan.cap : (p.plan.n_req > 0 ? p.plan.n_req : 1);
+  q.all_items = static_cast<int>(all_items);
+  q.items = q.tiles * used;
   const GradGeo geo = grad_geo(p.rp, q.codes != 0);
   // Row splits: while the CTAs of the adapters in use are fewer than the SMs
   // hold at once and each split keeps two stages of rows.
-  const int used = p.plan.cap < p.plan.n_req ? p.plan.cap : (p.plan.n_req > 0 ? p.plan.n_req : 1);
   const int rows = (p.plan.m + used - 1) / used;
   const int room = 148 * (geo.smem <= 113 * 1024 ? 2 : 1);
   q.splits = 1;

@@ -357,9 +357,10 @@ struct GradParams {
   GradMember mem[2];
   int32_t n_mem;
   int32_t r, rp;    // ranks written, and rounded up to 16
-  // set by the launch: feature tiles of both products, tiles * cap items, CTAs
-  // that share an adapter's rows, whether a member reads a checkpoint
-  int32_t tiles, items, splits, codes;
+  // set by the launch: feature tiles of both products, items of the adapters that
+  // may have rows and of all, CTAs that share an adapter's rows, whether a member
+  // reads a checkpoint
+  int32_t tiles, items, all_items, splits, codes;
   RequestPlan plan;
   uint64_t wait_limit_ns;
   uint32_t* err;
