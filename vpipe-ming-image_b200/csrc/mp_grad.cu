@@ -27,6 +27,8 @@
 // 2-9 widen them, and the scale of a (row, 128 features) goes into u, in f32.
 #include <cuda_runtime.h>
 
+#include <cmath>
+
 #include "mp_device.cuh"
 #include "mp_kernels.h"
 #include "mp_launch.h"
@@ -660,6 +662,27 @@ cudaError_t launch_tasks(const GradParams& p, uint32_t smem, unsigned grid, cuda
   return cudaLaunchKernelEx(&cfg, adapter_grad_kernel<TASKS>, p);
 }
 
+// CTAs that share an adapter's rows: the least of rounds x (9 us a CTA and 0.6 us a
+// stage) and 2 us for each CTA of a cluster. What the host does not know is put at
+// what it is for requests that pick their adapters at random: how many adapters
+// have rows, and that the one with the most has 1.7 times the average. With 1, 2,
+// 4, 8 CTAs a backward pass of 13705 rows 288 x 2880 and 2 adapters takes 200, 133,
+// 125, 149 us, one of 858 rows 4104 x 256 and 3 adapters 47, 66, 100, 197.
+int choose_splits(const RequestPlan& pl, int tiles, int room) {
+  const double live = pl.cap * (1.0 - std::pow(1.0 - 1.0 / pl.cap, pl.n_req > 0 ? pl.n_req : 1));
+  const double stages = std::fmax(1.7 * pl.m / (live * kRows), pl.n_req / live);
+  int best = 1;
+  double best_us = 1e300;
+  for (int s = 1; s <= kMaxGradSplits; s *= 2) {
+    const double us = std::fmax(1.0, tiles * live * s / room) * (9.0 + 0.6 * stages / s) + 2.0 * s;
+    if (us < best_us) {
+      best_us = us;
+      best = s;
+    }
+  }
+  return best;
+}
+
 }  // namespace
 
 cudaError_t launch_adapter_grad(const GradParams& p, cudaStream_t stream) {
@@ -678,13 +701,8 @@ cudaError_t launch_adapter_grad(const GradParams& p, cudaStream_t stream) {
   q.all_items = static_cast<int>(all_items);
   q.items = q.tiles * used;
   const GradGeo geo = grad_geo(p.rp, q.codes != 0);
-  // Row splits: while the CTAs of the adapters in use are fewer than the SMs
-  // hold at once and each split keeps two stages of rows.
-  const int rows = (p.plan.m + used - 1) / used;
   const int room = 148 * (geo.smem <= 113 * 1024 ? 2 : 1);
-  q.splits = 1;
-  while (q.splits < kMaxGradSplits && static_cast<long long>(q.tiles) * used * q.splits < room && rows > 4 * kRows * q.splits)
-    q.splits *= 2;
+  q.splits = choose_splits(p.plan, q.tiles, room);
   const unsigned grid = q.splits > 1 ? static_cast<unsigned>(q.items) * q.splits
                                      : static_cast<unsigned>(q.items < room ? q.items : room);
   if (p.rp <= 32) return launch_tasks<1>(q, geo.smem, grid, stream);
