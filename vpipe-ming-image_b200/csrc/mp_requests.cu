@@ -448,6 +448,13 @@ __device__ __forceinline__ void few_x(const uint16_t* at, int col, int k, uint32
   }
 }
 
+// Blocks an SM that the registers are cut to. With 17 to 32 rows and bf16 two
+// blocks of 8 warps, not one, take 3840x3840 from 23.0 to 16.8 us; the codes of
+// packed weights do not fit beside four tiles of x then.
+template <int BITS, int NT, int WARPS>
+constexpr int kFewBlocks = NT > 2 ? (WARPS == 4 ? 3 : BITS == 0 ? 2 : 1)
+                                  : (WARPS == 4 ? 5 : NT == 1 && BITS == 4 ? 3 : 2);
+
 // y[t] = W x[t] + B_a v[t] for up to 8 NT rows: bound by reading W once. A
 // block takes 16 features, its WARPS warps the 64-wide K groups in turn, lanes as in
 // rank_rows_kernel. Packed weights are not dequantized: a group's MMAs run on
@@ -458,7 +465,7 @@ __device__ __forceinline__ void few_x(const uint16_t* at, int col, int k, uint32
 // waits for it before the adapters' part. Rows past m repeat the last one: the
 // MMA's columns are independent, theirs are not stored.
 template <int BITS, int NT, int WARPS>
-__global__ void __launch_bounds__(32 * WARPS, NT > 2 ? 1 : (NT == 1 && BITS == 4 ? 24 : 16) / WARPS)
+__global__ void __launch_bounds__(32 * WARPS, kFewBlocks<BITS, NT, WARPS>)
     few_rows_kernel(const __grid_constant__ FewParams p) {
   // K groups a warp loads at a time, one batch ahead: 128 bytes a lane in flight;
   // up to 8 rows of w4 half of that from 24 warps an SM, not 16 (10240x3840, one
@@ -666,27 +673,34 @@ cudaError_t launch_rank_rows(const RankParams& p, cudaStream_t stream) {
 
 namespace {
 
-template <int BITS, int WARPS>
+template <int BITS, int NT>
 cudaError_t launch_few(const FewParams& p, cudaStream_t stream) {
-  const dim3 grid((p.n + 15) / 16), block(32 * WARPS);
+  const dim3 grid((p.n + 15) / 16);
   // it may start beside rank_rows_kernel, never beside what comes before that
   const bool over = p.chunks > 0;
-  if (p.m <= 8) return launch_overlapped(few_rows_kernel<BITS, 1, WARPS>, grid, block, p, stream, over);
-  if (p.m <= 16) return launch_overlapped(few_rows_kernel<BITS, 2, WARPS>, grid, block, p, stream, over);
-  if (p.m <= 32) return launch_overlapped(few_rows_kernel<BITS, 4, WARPS>, grid, block, p, stream, over);
-  return cudaErrorInvalidValue;
+  // Blocks of 8 warps, or of 4 with more of them on an SM where that takes the
+  // features in fewer rounds: a second round of a few blocks costs as much as the
+  // first. 8 / 4 warps at 10240x3840: 1 row w4 11.2 / 10.9 us, w8 17.9 / 13.9, bf16
+  // 19.9 / 18.5; 16 rows w4 21.9 / 23.2, w8 23.6 / 28.0 (the registers of five
+  // blocks do not hold the codes beside two tiles of x), bf16 30.7 / 24.0; 32 rows w4
+  // 39.7 / 33.9, w8 42.6 / 32.7, bf16 39.1 / 41.2. Up to 16 rows five blocks of 4
+  // an SM have to take all (1 row, w4 12288x3840: 13.5 / 15.8), and below three
+  // they leave SMs short of loads (5120x3840: 1 row bf16 11.5 / 15.5; but 32 rows w4
+  // 23.0 / 17.7).
+  constexpr bool kPays = NT == 4 ? BITS != 0 : NT == 1 || BITS == 0;
+  if constexpr (kPays) {
+    if (p.n > 16 * 148 * (NT == 4 ? 2 : 3) && (NT == 4 || p.n <= 16 * 148 * 5))
+      return launch_overlapped(few_rows_kernel<BITS, NT, 4>, grid, dim3(128), p, stream, over);
+  }
+  return launch_overlapped(few_rows_kernel<BITS, NT, 8>, grid, dim3(256), p, stream, over);
 }
 
-// Blocks of 8 warps; of 4 for a bf16 weight with many features, whose rows are
-// long enough to keep them busy: 10240x3840 takes 23.7 us with 4 and 30.8 with 8
-// at 16 rows, 3840x10240 39.2 and 29.9. Packed weights are faster with 8 at every
-// shape tried (w4 10240x3840, 16 rows: 23.8 and 21.9 us).
 template <int BITS>
 cudaError_t launch_few(const FewParams& p, cudaStream_t stream) {
-  if constexpr (BITS == 0) {
-    if (p.n >= 16 * 3 * 148) return launch_few<BITS, 4>(p, stream);
-  }
-  return launch_few<BITS, 8>(p, stream);
+  if (p.m <= 8) return launch_few<BITS, 1>(p, stream);
+  if (p.m <= 16) return launch_few<BITS, 2>(p, stream);
+  if (p.m <= kFewRows) return launch_few<BITS, 4>(p, stream);
+  return cudaErrorInvalidValue;
 }
 
 }  // namespace
