@@ -2075,13 +2075,16 @@ mp::RankParams rank_params(const mp_ctx* c, const RequestsLaunch& ext, const voi
 
 // The rank-space rows of a batch of requests: v = s_q (x F_q^T), into `r`'s
 // outputs. Where there is much to multiply, requests of 16 rows and more on
-// average go to the tensor core in tiles of 128 rows; else runs of 8 rows. At
-// m 4352, k 3840 the runs / the tiles take 12.7 / 14.4 us with 16 ranks (m k rp
-// = 2.7e8), 20.6 / 15.4 us with 32 (5.3e8); at m 16896 with 64, 175 / 37 us.
+// average go to the tensor core in tiles of 128 rows; else runs of 8 rows. The
+// runs / the tiles of 4 requests take, at k 3840, 9.1 / 11.1 us for 1024 rows of 32
+// ranks (m k rp = 1.3e8), 12.8 / 11.5 for 1536 (1.9e8), 16.6 / 14.4 for 4352 of 16
+// (2.7e8), 50.3 / 15.7 for 4352 of 64; at k 10240, 10.3 / 14.5 us for 256 rows of 64
+// (1.7e8), 17.2 / 15.0 for 512 (3.4e8). Requests of 64 rows fill half a tile: 15.2 /
+// 13.6 us for 32 of them with 32 ranks at k 3840 (2.5e8).
 int launch_ranks(mp_ctx* c, const RequestsLaunch& ext, mp::RankParams* r, cudaStream_t stream) {
   const mp::RequestPlan& pl = r->plan;
   const bool tiles = pl.m >= 16 * static_cast<int64_t>(pl.n_req) &&
-                     static_cast<double>(pl.m) * r->k * r->rp >= 1.0e8;
+                     static_cast<double>(pl.m) * r->k * r->rp >= 2.0e8;
   cudaError_t e;
   if (tiles) {
     if (!encode_2d(&r->tm_x, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, r->x, r->k, pl.m, static_cast<uint64_t>(r->ldx) * 2, 64,
