@@ -181,6 +181,21 @@ def test_long_requests(ctx, case, saved):
         h.free()
 
 
+NARROW = [
+    # many rows of few features: little to multiply, the tensor core's tiles all the same
+    (9000, 136, 64, 3, 64, [4100, 3, 64, 63, 4600], [2, 0, 1, -1, 0], [1.0, 0.5, 1.0, 1.0, -1.0]),
+    (3000, 64, 192, 1, 16, [1500, 1500], [0, 0], [1.0, 0.25]),
+    (2048, 72, 128, 4, 100, [16] * 128, [(3 * i) % 5 - 1 for i in range(128)], [1.0] * 128),
+    (2500, 320, 256, 8, 40, [17] * 147, [(3 * i) % 9 - 1 for i in range(147)], [0.5 + i / 100 for i in range(147)]),
+]
+
+
+@pytest.mark.parametrize("case", NARROW, ids=[f"m{c[0]}_n{c[1]}_k{c[2]}_r{c[4]}" for c in NARROW])
+@pytest.mark.parametrize("saved", [16, 8])
+def test_narrow_long_requests(ctx, case, saved):
+    test_long_requests(ctx, case, saved)
+
+
 @pytest.mark.parametrize("rank,saved", [(4, 8), (4, 16), (30, 16), (64, 8), (100, 16)])
 def test_gradients_repeat(ctx, rank, saved):
     """Hundreds of passes in a row, nothing waited for between them: the same

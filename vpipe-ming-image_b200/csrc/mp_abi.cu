@@ -2074,17 +2074,25 @@ mp::RankParams rank_params(const mp_ctx* c, const RequestsLaunch& ext, const voi
 }
 
 // The rank-space rows of a batch of requests: v = s_q (x F_q^T), into `r`'s
-// outputs. Where there is much to multiply, requests of 16 rows and more on
-// average go to the tensor core in tiles of 128 rows; else runs of 8 rows. The
-// runs / the tiles of 4 requests take, at k 3840, 9.1 / 11.1 us for 1024 rows of 32
-// ranks (m k rp = 1.3e8), 12.8 / 11.5 for 1536 (1.9e8), 16.6 / 14.4 for 4352 of 16
-// (2.7e8), 50.3 / 15.7 for 4352 of 64; at k 10240, 10.3 / 14.5 us for 256 rows of 64
-// (1.7e8), 17.2 / 15.0 for 512 (3.4e8). Requests of 64 rows fill half a tile: 15.2 /
-// 13.6 us for 32 of them with 32 ranks at k 3840 (2.5e8).
+// outputs. Two forms, the one that this model of their times takes to be the
+// faster: runs of 8 rows cost what their blocks do (8 rows by 16 ranks), the
+// tensor core's tiles of 128 rows a longer start and their reads of x. Runs / tiles
+// in us, measured:
+//     k   rows ranks requests           k    rows ranks requests
+//    256   500    16    4   5.1 / 6.8   2048  4000   16       62  13.3 / 15.7
+//    256  4000    16    4  11.5 / 6.7   2048  9000   16      562  31.3 / 38.2
+//    256  9000    64    4  65.2 / 7.9   3840  1024   32        4   9.1 / 11.1
+//    832  2000    16    4   8.1 / 10.0  3840  1536   32        4  12.8 / 11.5
+//    832  9000    16  562  30.2 / 20.2  3840  4352   64        4  50.3 / 15.7
+//   2048  9000    64  562  93.8 / 42.4  10240  256   64        4  10.3 / 14.5
+//   2048  1000    64   62  13.0 / 13.3  10240  512   64        4  17.2 / 15.0
+// Requests of less than 16 rows on average leave the tiles too empty.
 int launch_ranks(mp_ctx* c, const RequestsLaunch& ext, mp::RankParams* r, cudaStream_t stream) {
   const mp::RequestPlan& pl = r->plan;
-  const bool tiles = pl.m >= 16 * static_cast<int64_t>(pl.n_req) &&
-                     static_cast<double>(pl.m) * r->k * r->rp >= 2.0e8;
+  const double k = r->k, m = pl.m, q = pl.n_req;
+  const double runs_us = 4.0 + (m / 8 + q) * (r->rp / 16) * 3.5e-6 * (3200.0 + k);
+  const double tiles_us = 8.0 + 5.0e-4 * k + (m / 128 + q) * 3.0e-5 * k;
+  const bool tiles = m >= 16 * q && tiles_us < runs_us;
   cudaError_t e;
   if (tiles) {
     if (!encode_2d(&r->tm_x, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, r->x, r->k, pl.m, static_cast<uint64_t>(r->ldx) * 2, 64,
