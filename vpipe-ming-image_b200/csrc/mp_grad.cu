@@ -99,9 +99,10 @@ __host__ __device__ inline PartCols part_cols(int rp) {
   return c;
 }
 
-// Floats between the sums of two ranks in the exchange buffer: dB is written
-// rank fastest, and one more float puts consecutive ranks in different banks.
-__host__ __device__ inline int exchange_ld(bool rank_major) { return rank_major ? kTileF : kTileF + 1; }
+// A cluster's sums in the exchange buffer, four next to one another as the output
+// has them: dA [rank][feature]; dB [feature][rank], with four more floats that put
+// the 16 bytes of eight features into different banks.
+__host__ __device__ inline int exchange_ld(bool rank_major, int rp) { return rank_major ? kTileF : rp + 4; }
 
 // A stage: x as the A operand | u's parts, the B operand | u, f32 | with a
 // checkpoint its codes and the rows' scales.
@@ -125,7 +126,7 @@ __host__ __device__ inline GradGeo grad_geo(int rp, bool codes) {
   g.stages = static_cast<int>(((two ? half : kGradSmemMost) - 1280) / g.stage_bytes);
   if (g.stages > kMaxGradStages) g.stages = kMaxGradStages;
   const uint32_t tiles = g.stages * g.stage_bytes;
-  const uint32_t exchange = rp * (kTileF + 1) * 4;
+  const uint32_t exchange = kTileF * (rp + 4) * 4;
   g.smem = (tiles > exchange ? tiles : exchange) + 1024 + 256;
   return g;
 }
@@ -180,12 +181,6 @@ __device__ __forceinline__ uint64_t mn_desc(uint32_t tile, int kk) {
   d |= static_cast<uint64_t>(1u) << 46;  // descriptor version (sm_100)
   d |= static_cast<uint64_t>(2u) << 61;  // SWIZZLE_128B
   return d;
-}
-
-__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
-  return v;
 }
 
 // The next bf16 part of two values, which keep what is left of them.
@@ -367,7 +362,8 @@ __global__ void __launch_bounds__(kGradThreads<TASKS>, TASKS == 1 ? 2 : 1)
   extern __shared__ uint8_t grad_raw[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int count = p.splits, rank = count > 1 ? static_cast<int>(cluster_ctarank()) : 0;
-  const int item0 = static_cast<int>(blockIdx.x) / count, step = static_cast<int>(gridDim.x) / count;
+  const int item0 = static_cast<int>(blockIdx.x) / count, clusters = static_cast<int>(gridDim.x) / count;
+  const int step = p.workers;
   const int col0 = warp >= kSumWarp0 + 4 ? kSumCols<TASKS> : 0;  // the adding warp's first rank
   const PartCols pc = part_cols(p.rp);
   const GradGeo geo = grad_geo(p.rp, p.codes != 0);
@@ -384,24 +380,48 @@ __global__ void __launch_bounds__(kGradThreads<TASKS>, TASKS == 1 ? 2 : 1)
   sm.done = sm.taken + 2;
   sm.tmem_slot = reinterpret_cast<uint32_t*>(sm.done + 1);
   sm.abort = sm.tmem_slot + 1;
-  // Zeros of item i: an adapter without rows.
-  auto clear_item = [&](int i, int tid, int threads) {
+  // Zeros of item i (an adapter without rows) by this cluster's threads.
+  auto clear_item = [&](int i) {
+    const int tid = rank * kGradThreads<TASKS> + threadIdx.x, threads = count * kGradThreads<TASKS>;
     const Item item = item_of(p, i);
     const int f0 = item.f_tile * kTileF, width = min(kTileF, item.mb->width - f0);
     float* out = item.mb->out + static_cast<int64_t>(item.a) * p.r * item.mb->width;
-    for (int e = tid; e < p.r * width; e += threads)
-      out[item.mb->rank_major ? static_cast<int64_t>(e / width) * item.mb->width + f0 + e % width
-                              : static_cast<int64_t>(f0) * p.r + e] = 0.0f;
+    if (item.mb->rank_major) {
+      out += f0;
+      const bool quads = ((reinterpret_cast<uintptr_t>(out) | item.mb->width * 4u | width * 4u) & 15u) == 0;
+      for (int r = tid >> 5; r < p.r; r += threads >> 5) {
+        float* row = out + static_cast<int64_t>(r) * item.mb->width;
+        if (quads) {
+          if (lane * 4 < width) *reinterpret_cast<float4*>(row + lane * 4) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        } else {
+          for (int f = lane; f < width; f += 32) row[f] = 0.0f;
+        }
+      }
+    } else {
+      out += static_cast<int64_t>(f0) * p.r;
+      const int n = width * p.r;
+      if (((reinterpret_cast<uintptr_t>(out) | n * 4u) & 15u) == 0) {
+        for (int e = tid * 4; e < n; e += threads * 4)
+          *reinterpret_cast<float4*>(out + e) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      } else {
+        for (int e = tid; e < n; e += threads) out[e] = 0.0f;
+      }
+    }
   };
+  if (item0 >= p.workers) {
+    // clusters of their own clear the adapters that are more than the requests
+    pdl_wait();
+    pdl_release();
+    for (int i = p.items + item0 - p.workers; i < p.all_items; i += clusters - p.workers) clear_item(i);
+    return;
+  }
   if (count > 1) {
     // clusters of adapters without rows leave before any set-up
     pdl_wait();
     const Item item = item_of(p, item0);
     if (p.plan.begin[item.a] == p.plan.begin[item.a + 1]) {
       pdl_release();
-      const int tid = rank * kGradThreads<TASKS> + threadIdx.x, threads = count * kGradThreads<TASKS>;
-      clear_item(item0, tid, threads);
-      for (int i = p.items + item0; i < p.all_items; i += step) clear_item(i, tid, threads);
+      clear_item(item0);
       return;
     }
   }
@@ -586,10 +606,19 @@ __global__ void __launch_bounds__(kGradThreads<TASKS>, TASKS == 1 ? 2 : 1)
     // stages' memory takes a cluster's sums
     named_barrier(kAllBarrier, kGradThreads<TASKS>);
     if (count > 1) {
-      const int ld = exchange_ld(item_of(p, item0).mb->rank_major != 0);
+      const bool rank_major = item_of(p, item0).mb->rank_major != 0;
+      const int ld = exchange_ld(rank_major, p.rp);
 #pragma unroll
-      for (int c = 0; c < kSumCols<TASKS>; ++c)
-        if (col0 + c < p.rp) sm.exchange[(col0 + c) * ld + f] = sums[c];
+      for (int c = 0; c < kSumCols<TASKS>; c += 4) {
+        if (col0 + c >= p.rp) break;
+        if (rank_major) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) sm.exchange[(col0 + c + j) * ld + f] = sums[c + j];
+        } else {
+          *reinterpret_cast<float4*>(sm.exchange + f * ld + col0 + c) =
+              make_float4(sums[c], sums[c + 1], sums[c + 2], sums[c + 3]);
+        }
+      }
     }
   }
   __syncwarp();
@@ -601,31 +630,44 @@ __global__ void __launch_bounds__(kGradThreads<TASKS>, TASKS == 1 ? 2 : 1)
       // the CTAs share the adding up: each takes some ranks (dA) or features (dB)
       const Item item = item_of(p, item0);
       const GradMember& mb = *item.mb;
-      const int ld = exchange_ld(mb.rank_major != 0);
+      const int ld = exchange_ld(mb.rank_major != 0, p.rp);
       const int f0 = item.f_tile * kTileF, width = min(kTileF, mb.width - f0);
       float* out = mb.out + static_cast<int64_t>(item.a) * p.r * mb.width;
       const uint32_t ex = smem_u32(sm.exchange);
-      auto sum_at = [&](int r, int f) {
-        const uint32_t at = ex + static_cast<uint32_t>(r * ld + f) * 4u;
-        float o[kMaxGradSplits];  // all in flight, then added in CTA order
+      auto sums_at = [&](int e) {
+        const uint32_t at = ex + static_cast<uint32_t>(e) * 4u;
+        float4 o[kMaxGradSplits];  // all in flight, then added in CTA order
 #pragma unroll
         for (int z = 0; z < kMaxGradSplits; ++z)
-          if (z < count) o[z] = ld_cluster_f32(mapa_shared(at, z));
-        float s = o[0];
+          if (z < count) o[z] = ld_cluster_f4(mapa_shared(at, z));
+        float4 s = o[0];
 #pragma unroll
         for (int z = 1; z < kMaxGradSplits; ++z)
-          if (z < count) s += o[z];
+          if (z < count) s.x += o[z].x, s.y += o[z].y, s.z += o[z].z, s.w += o[z].w;
         return s;
       };
+      // the `n` first of four sums, 16 bytes at once where they all are and may be
+      auto put = [&](float* to, float4 s, int n) {
+        if (n >= 4 && (reinterpret_cast<uintptr_t>(to) & 15u) == 0) {
+          *reinterpret_cast<float4*>(to) = s;
+        } else {
+          if (n > 0) to[0] = s.x;
+          if (n > 1) to[1] = s.y;
+          if (n > 2) to[2] = s.z;
+          if (n > 3) to[3] = s.w;
+        }
+      };
       if (mb.rank_major) {
-        for (int e = threadIdx.x; e < p.r * kTileF; e += kGradThreads<TASKS>) {
-          const int r = e / kTileF, f = e % kTileF;
-          if (r % count == rank && f < width) out[static_cast<int64_t>(r) * mb.width + f0 + f] = sum_at(r, f);
+        for (int e = threadIdx.x; (e >> 5) * count + rank < p.r; e += kGradThreads<TASKS>) {
+          const int r = (e >> 5) * count + rank, f = (e & 31) * 4;
+          if (f < width) put(out + static_cast<int64_t>(r) * mb.width + f0 + f, sums_at(r * ld + f), width - f);
         }
       } else {
-        const int per = kTileF / count, lo = rank * per, hi = min(lo + per, width);
-        for (int e = lo * p.r + threadIdx.x; e < hi * p.r; e += kGradThreads<TASKS>)
-          out[static_cast<int64_t>(f0) * p.r + e] = sum_at(e % p.r, e / p.r);
+        const int quads = (p.r + 3) / 4, per = kTileF / count, lo = rank * per, hi = min(lo + per, width);
+        for (int e = threadIdx.x; e < (hi - lo) * quads; e += kGradThreads<TASKS>) {
+          const int f = lo + e / quads, r = e % quads * 4;
+          put(out + static_cast<int64_t>(f0 + f) * p.r + r, sums_at(f * ld + r), p.r - r);
+        }
       }
     }
     cluster_sync();  // no CTA leaves while another reads its sums
@@ -634,9 +676,6 @@ __global__ void __launch_bounds__(kGradThreads<TASKS>, TASKS == 1 ? 2 : 1)
   }
   tc_fence_after();
   if (warp == 1) tmem_dealloc(tmem, pc.cols * pc.bufs);
-  // the adapters that are more than the requests
-  for (int i = p.items + item0; i < p.all_items; i += step)
-    clear_item(i, rank * kGradThreads<TASKS> + threadIdx.x, count * kGradThreads<TASKS>);
   if (threadIdx.x == 0 && aborted) atomicOr(p.err, kErrTimeout);
 }
 
@@ -663,18 +702,23 @@ cudaError_t launch_tasks(const GradParams& p, uint32_t smem, unsigned grid, cuda
 }
 
 // CTAs that share an adapter's rows: the least of rounds x (9 us a CTA and 0.6 us a
-// stage) and 2 us for each CTA of a cluster. What the host does not know is put at
+// stage) and 1.5 us + 0.15 us a CTA for a cluster's joining. An SM takes `per_sm`
+// CTAs, the GPU 148, 74, 33, 15 clusters of 1, 2, 4, 8 of them; the `rest` items that
+// are only cleared count for half a CTA each. What the host does not know is put at
 // what it is for requests that pick their adapters at random: how many adapters
 // have rows, and that the one with the most has 1.7 times the average. With 1, 2,
-// 4, 8 CTAs a backward pass of 13705 rows 288 x 2880 and 2 adapters takes 200, 133,
-// 125, 149 us, one of 858 rows 4104 x 256 and 3 adapters 47, 66, 100, 197.
-int choose_splits(const RequestPlan& pl, int tiles, int room) {
+// 4, 8 CTAs the launch takes 85, 49, 31, 21 us at 7713 rows 440 x 576, 2 adapters of
+// 56 ranks; 135, 75, 44, 52 at 13705 rows 288 x 2880, 2 of 48; 36, 24, 31, 52 at 4352
+// rows 3840 x 3840, 4 of 16 (8 bit); 16, 25, 40, 75 at 1954 rows 832 x 1600, 6 of 52.
+int choose_splits(const RequestPlan& pl, int tiles, int rest, int per_sm) {
   const double live = pl.cap * (1.0 - std::pow(1.0 - 1.0 / pl.cap, pl.n_req > 0 ? pl.n_req : 1));
-  const double stages = std::fmax(1.7 * pl.m / (live * kRows), pl.n_req / live);
+  const double stages = std::fmax((1.7 - 0.7 / live) * pl.m / (live * kRows), pl.n_req / live);
   int best = 1;
   double best_us = 1e300;
   for (int s = 1; s <= kMaxGradSplits; s *= 2) {
-    const double us = std::fmax(1.0, tiles * live * s / room) * (9.0 + 0.6 * stages / s) + 2.0 * s;
+    const double room = per_sm * s * (s == 1 ? 148 : s == 2 ? 74 : s == 4 ? 33 : 15);
+    const double ctas = tiles * live * s + 0.5 * std::fmin(148.0, static_cast<double>(rest) * s);
+    const double us = std::fmax(1.0, ctas / room) * (9.0 + 0.6 * stages / s) + (s > 1 ? 1.5 + 0.15 * s : 0.0);
     if (us < best_us) {
       best_us = us;
       best = s;
@@ -701,10 +745,14 @@ cudaError_t launch_adapter_grad(const GradParams& p, cudaStream_t stream) {
   q.all_items = static_cast<int>(all_items);
   q.items = q.tiles * used;
   const GradGeo geo = grad_geo(p.rp, q.codes != 0);
-  const int room = 148 * (geo.smem <= 113 * 1024 ? 2 : 1);
-  q.splits = choose_splits(p.plan, q.tiles, room);
-  const unsigned grid = q.splits > 1 ? static_cast<unsigned>(q.items) * q.splits
-                                     : static_cast<unsigned>(q.items < room ? q.items : room);
+  const int per_sm = geo.smem <= 113 * 1024 ? 2 : 1, room = 148 * per_sm, rest = q.all_items - q.items;
+  q.splits = choose_splits(p.plan, q.tiles, rest, per_sm);
+  q.workers = q.splits > 1 ? q.items : (q.items < room ? q.items : room);
+  // Clusters of their own clear, beside those at work: with 10 of 12 adapters of
+  // 3672 x 192 and 64 ranks to clear, the working CTAs doing it took the launch
+  // from 10.6 to 26 us.
+  const int most = (148 + q.splits - 1) / q.splits;
+  const unsigned grid = static_cast<unsigned>(q.workers + (rest < most ? rest : most)) * q.splits;
   if (p.rp <= 32) return launch_tasks<1>(q, geo.smem, grid, stream);
   if (p.rp <= 64) return launch_tasks<2>(q, geo.smem, grid, stream);
   return launch_tasks<4>(q, geo.smem, grid, stream);

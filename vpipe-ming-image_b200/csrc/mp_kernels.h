@@ -358,9 +358,9 @@ struct GradParams {
   int32_t n_mem;
   int32_t r, rp;    // ranks written, and rounded up to 16
   // set by the launch: feature tiles of both products, items of the adapters that
-  // may have rows and of all, CTAs that share an adapter's rows, whether a member
-  // reads a checkpoint
-  int32_t tiles, items, all_items, splits, codes;
+  // may have rows and of all, CTAs that share an adapter's rows, clusters that work
+  // on items (those past them clear), whether a member reads a checkpoint
+  int32_t tiles, items, all_items, splits, workers, codes;
   RequestPlan plan;
   uint64_t wait_limit_ns;
   uint32_t* err;

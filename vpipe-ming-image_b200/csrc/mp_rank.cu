@@ -64,15 +64,6 @@ __host__ __device__ inline RankGeo rank_geo(int rp) {
   return g;
 }
 
-__device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
-  float4 v;
-  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-               : "r"(addr)
-               : "memory");
-  return v;
-}
-
 struct RankUnit {
   int unit;       // block of the plan at the units' level
   int row0;       // first row of x
