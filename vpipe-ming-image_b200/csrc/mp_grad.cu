@@ -25,6 +25,12 @@
 //
 // A checkpoint's codes are whole numbers of up to 8 bits, exact in bf16: warps
 // 2-9 widen them, and the scale of a (row, 128 features) goes into u, in f32.
+//
+// Measured: 92 us for 16896 rows 3840 x 3840, 24 requests, 16 adapters of up to 64
+// ranks (x and dy once, 260 MB, at 2.8 TB/s; 43 % of the issue slots); 24 us for 4352
+// rows, 4 adapters of 16, x in 8 bits (2.1 TB/s). What bounds it is not HBM but
+// cutting u: a stage's u is cut anew for each 128 features, 60 times here, and a CTA
+// takes 0.6 us a stage for its chain of copies, parts, MMAs and sums.
 #include <cuda_runtime.h>
 
 #include <cmath>

