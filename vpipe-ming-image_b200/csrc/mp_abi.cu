@@ -2137,7 +2137,6 @@ int launch_request_ranks(mp_ctx* c, ProjParams* p, const RequestsLaunch& ext, co
   p->ext_live = pl.live[level];
   p->ext_list = pl.list[level];
   p->ext_chunks = chunks;
-  p->late_wait = 1;
   return MP_OK;
 }
 

@@ -126,11 +126,10 @@ struct ProjParams {
   const int32_t* ext_first;
   const int32_t* ext_live;
   const int2* ext_list;
-  int32_t ext_chunks;
   // The launch right before on the stream is the one that writes tm_t's blocks:
   // this one starts beside it (everything else it touches was complete when that
   // one started) and waits for it before the first appended K tile.
-  int32_t late_wait;
+  int32_t ext_chunks;
   // Fused rank-space prologue (n_pre > 0): before their member tiles, the
   // pairs with the fewest member tiles run n_pre prologue units, each the
   // full-K product of 512 token rows x 256 rank rows of T = scale ⊙ (x ·

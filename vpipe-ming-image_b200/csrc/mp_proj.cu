@@ -207,6 +207,9 @@ struct Tile {
   int ext0;      // adapters by request: the tile's first list entry
 };
 
+// EXT: a launch whose requests bring their adapters (an instantiation of its own:
+// the tests in every role cost the other launches 0.8 %).
+template <bool EXT>
 __device__ __forceinline__ Tile decode_tile(const ProjParams& p, int tile, int rank, int base_kt) {
   Tile t;
   const int per_split = p.n_pairs * p.n_ttiles;
@@ -247,7 +250,7 @@ __device__ __forceinline__ Tile decode_tile(const ProjParams& p, int tile, int r
   t.kt_begin = 0;
   t.kt_end = base_kt + p.mem[mi].lora_ktiles;
   t.ext0 = 0;
-  if (p.ext_first != nullptr) {
+  if constexpr (EXT) {
     t.ext0 = p.ext_first[tt];
     t.kt_end = base_kt + p.ext_live[tt] * p.ext_chunks;
   }
@@ -320,8 +323,9 @@ __device__ __forceinline__ int units_next(const ProjParams& p, UnitIter& u) {
   return kNoUnit;
 }
 
+template <bool EXT>
 __device__ __forceinline__ Tile decode_unit(const ProjParams& p, int unit, int rank, int base_kt) {
-  return unit < 0 ? decode_pre(p, -1 - unit, rank, base_kt) : decode_tile(p, unit, rank, base_kt);
+  return unit < 0 ? decode_pre(p, -1 - unit, rank, base_kt) : decode_tile<EXT>(p, unit, rank, base_kt);
 }
 
 __device__ __forceinline__ const ProjMember& unit_member(const ProjParams& p, const Tile& t) {
@@ -358,7 +362,7 @@ __device__ bool wait_prologue(const ProjParams& p, const ProjMember& mb, const T
 }
 
 // Warp 0, one thread. Stage iteration `it` runs on across tiles.
-template <int NT>
+template <int NT, bool EXT>
 __device__ void pair_producer(const ProjParams& p, const PairSmem& sm, bool leader, int rank,
                               int base_kt) {
   using G = Geo<NT>;
@@ -373,14 +377,14 @@ __device__ void pair_producer(const ProjParams& p, const PairSmem& sm, bool lead
   bool waited = false;
   UnitIter units = units_begin(p);
   for (int unit = units_next(p, units); unit != kNoUnit && !aborted; unit = units_next(p, units)) {
-    const Tile t = decode_unit(p, unit, rank, base_kt);
+    const Tile t = decode_unit<EXT>(p, unit, rank, base_kt);
     const ProjMember& mb = unit_member(p, t);
     const bool quant = mb.bits != 0;
     const uint32_t sub_bytes = static_cast<uint32_t>(t.half) * 128u;  // one sub-tile, one CTA
     const uint32_t xbytes_pair = 2u * static_cast<uint32_t>(t.n_sub) * sub_bytes;
     const uint32_t codes_bytes = static_cast<uint32_t>(kBlockN * kBlockK * mb.bits / 8);
     // adapters by request: the next list entry, loaded one entry ahead
-    const bool ext = p.ext_first != nullptr && t.kt_end > base_kt;
+    const bool ext = EXT && t.kt_end > base_kt;
     int2 ext_next = ext ? p.ext_list[t.ext0] : make_int2(0, 0);
     int2 ext_now = ext_next;
     for (int kt = t.kt_begin; kt < t.kt_end; ++kt, ++it) {
@@ -409,7 +413,7 @@ __device__ void pair_producer(const ProjParams& p, const PairSmem& sm, bool lead
       int xrow = t.t0;                               // first row of the tile in xmap
       int brow = mb.swiglu ? 2 * t.f0 : t.f0;        // SwiGLU: the interleaved B stack holds 128 rows per 64 features
       if (lora && ext) {
-        if (p.late_wait && !waited) {  // the rank-space blocks are complete
+        if (!waited) {  // the rank-space blocks are complete
           pdl_wait();
           fence_proxy_async_global();
           waited = true;
@@ -480,7 +484,7 @@ __device__ void pair_producer(const ProjParams& p, const PairSmem& sm, bool lead
 }
 
 // Warp 1 of the leader, one thread.
-template <int NT>
+template <int NT, bool EXT>
 __device__ void pair_mma(const ProjParams& p, const PairSmem& sm, uint32_t tmem, int base_kt) {
   using G = Geo<NT>;
   constexpr uint32_t stages = G::kStages;
@@ -490,7 +494,7 @@ __device__ void pair_mma(const ProjParams& p, const PairSmem& sm, uint32_t tmem,
   UnitIter units = units_begin(p);
   for (int unit = units_next(p, units); unit != kNoUnit && !aborted;
        unit = units_next(p, units), ++tcount) {
-    const Tile t = decode_unit(p, unit, 0, base_kt);
+    const Tile t = decode_unit<EXT>(p, unit, 0, base_kt);
     // token-row tiles: D[token][feature] (A = the x sub-tile, M = its tokens
     // across the pair; B = the weight tile, N = the pair's 256 features);
     // narrower tiles: D[feature][token] (A = weights, B = x)
@@ -556,7 +560,7 @@ __device__ void pair_mma(const ProjParams& p, const PairSmem& sm, uint32_t tmem,
 // Warps 2-9. Warpgroup g converts columns [32g, 32g + 32) of every stage for
 // the 128 feature rows of this CTA: thread (warp % 4, lane) owns row r. The
 // codes tile is 64-byte (w8) or 32-byte (w4) swizzled by its TMA map.
-template <int NT>
+template <int NT, bool EXT>
 __device__ void pair_dequant(const ProjParams& p, const PairSmem& sm, int rank, int base_kt) {
   using G = Geo<NT>;
   constexpr uint32_t stages = G::kStages;
@@ -570,7 +574,7 @@ __device__ void pair_dequant(const ProjParams& p, const PairSmem& sm, int rank, 
   bool aborted = false;
   UnitIter units = units_begin(p);
   for (int unit = units_next(p, units); unit != kNoUnit && !aborted; unit = units_next(p, units)) {
-    const Tile t = decode_unit(p, unit, rank, base_kt);
+    const Tile t = decode_unit<EXT>(p, unit, rank, base_kt);
     const ProjMember& mb = unit_member(p, t);
     const int base_end = min(base_kt, t.kt_end);
     if (mb.bits == 0) {  // no dequant stages: keep the stage count in step
@@ -669,7 +673,8 @@ __device__ __forceinline__ void release_accumulator(const PairSmem& sm, int j) {
 
 // Epilogue variants, one kernel instantiation each (they differ in register
 // needs): plain projections, SwiGLU pairs, attention heads.
-enum : int { kEpiPlain = 0, kEpiSwiGlu = 1, kEpiHeads = 2 };
+// kEpiRequests: the plain epilogue of a launch whose requests bring their adapters.
+enum : int { kEpiPlain = 0, kEpiSwiGlu = 1, kEpiHeads = 2, kEpiRequests = 3 };
 
 
 // ---- token-row epilogue (256- and 512-token tiles) -------------------------
@@ -1020,6 +1025,7 @@ __device__ void rows_heads(const ProjParams& p, const ProjMember& mb, uint32_t a
 template <int EPI>
 __device__ void pair_epilogue_rows(const ProjParams& p, const PairSmem& sm, uint32_t tmem, int rank,
                                    int base_kt) {
+  constexpr bool EXT = EPI == kEpiRequests;
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   const int q = warp & 3;
@@ -1032,7 +1038,7 @@ __device__ void pair_epilogue_rows(const ProjParams& p, const PairSmem& sm, uint
   uint32_t round = 0;
   UnitIter units = units_begin(p);
   for (int unit = units_next(p, units); unit != kNoUnit; unit = units_next(p, units), ++tcount) {
-    const Tile t = decode_unit(p, unit, rank, base_kt);
+    const Tile t = decode_unit<EXT>(p, unit, rank, base_kt);
     const ProjMember& mb = unit_member(p, t);
     // strengths apply to a rank-space pre-GEMM launch and to prologue units
     const bool scaled = p.scale.enabled && (p.n_pre == 0 || t.mi < 0);
@@ -1091,6 +1097,7 @@ __device__ void pair_epilogue_rows(const ProjParams& p, const PairSmem& sm, uint
 // one thread stores both halves with TMA bulk stores (they clip rows past M
 // and columns past N). Two staging buffers alternate. In split-K mode the fp32
 // sums go straight to the partial-sum array instead.
+template <bool EXT>
 __device__ void pair_epilogue_cols(const ProjParams& p, const PairSmem& sm, uint32_t tmem,
                                    int rank, int base_kt) {
   const int warp = threadIdx.x >> 5;
@@ -1108,7 +1115,7 @@ __device__ void pair_epilogue_cols(const ProjParams& p, const PairSmem& sm, uint
   uint32_t round = 0;
   UnitIter units = units_begin(p);
   for (int unit = units_next(p, units); unit != kNoUnit; unit = units_next(p, units), ++tcount) {
-    const Tile t = decode_unit(p, unit, rank, base_kt);
+    const Tile t = decode_unit<EXT>(p, unit, rank, base_kt);
     const ProjMember& mb = unit_member(p, t);
     const int f = t.f0 + fl;
     // strengths apply to a rank-space pre-GEMM launch and to prologue units
@@ -1238,6 +1245,7 @@ extern "C" int mp_trace_read(long long* host, int n) {
 template <int NT, int EPI>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     proj_pair_kernel(const __grid_constant__ ProjParams p) {
+  constexpr bool kExt = EPI == kEpiRequests;
   extern __shared__ uint8_t smem_raw[];
   const PairSmem sm = carve_pair(smem_raw);
   const int warp = threadIdx.x >> 5;
@@ -1282,24 +1290,24 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
   tc_fence_after();
   const uint32_t tmem = *sm.tmem_slot;
   // set-up done (shared memory, TMEM, tensor maps): global memory from here on
-  if (!p.late_wait) pdl_wait();
+  if (!kExt) pdl_wait();
   pdl_release();
 
   if (warp == 0) {
-    if (lane == 0) pair_producer<NT>(p, sm, leader, rank, base_kt);
+    if (lane == 0) pair_producer<NT, kExt>(p, sm, leader, rank, base_kt);
   } else if (warp == 1) {
-    if (lane == 0 && leader) pair_mma<NT>(p, sm, tmem, base_kt);
+    if (lane == 0 && leader) pair_mma<NT, kExt>(p, sm, tmem, base_kt);
   } else if (warp < kEpiWarp0) {
-    pair_dequant<NT>(p, sm, rank, base_kt);
+    pair_dequant<NT, kExt>(p, sm, rank, base_kt);
   } else {
     if constexpr (kTokRows<NT>)
       pair_epilogue_rows<EPI>(p, sm, tmem, rank, base_kt);
     else
-      pair_epilogue_cols(p, sm, tmem, rank, base_kt);
+      pair_epilogue_cols<kExt>(p, sm, tmem, rank, base_kt);
   }
 
   // whoever waits for this launch waits for the one it ran beside, too
-  if (p.late_wait) pdl_wait();
+  if (kExt) pdl_wait();
 
   if (*sm.abort != 0u) {
     // Error path only: let copies issued before the abort land (their
@@ -1472,7 +1480,9 @@ cudaError_t configure(int* dev_out) {
   for (cudaError_t r : {opt_in_smem<512, kEpiPlain>(), opt_in_smem<256, kEpiPlain>(),
                         opt_in_smem<128, kEpiPlain>(), opt_in_smem<64, kEpiPlain>(),
                         opt_in_smem<512, kEpiSwiGlu>(), opt_in_smem<256, kEpiSwiGlu>(),
-                        opt_in_smem<512, kEpiHeads>(), opt_in_smem<256, kEpiHeads>()})
+                        opt_in_smem<512, kEpiHeads>(), opt_in_smem<256, kEpiHeads>(),
+                        opt_in_smem<512, kEpiRequests>(), opt_in_smem<256, kEpiRequests>(),
+                        opt_in_smem<128, kEpiRequests>(), opt_in_smem<64, kEpiRequests>()})
     if (r != cudaSuccess) return r;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(2, 1, 1);
@@ -1561,6 +1571,15 @@ cudaError_t launch_proj_pair(const ProjParams& p, cudaStream_t stream) {
     switch (p.n_tok) {
       case 512: return launch_nt<512, kEpiHeads>(q, pairs, coop, stream);
       case 256: return launch_nt<256, kEpiHeads>(q, pairs, coop, stream);
+      default: return cudaErrorInvalidValue;
+    }
+  }
+  if (p.ext_first != nullptr) {
+    switch (p.n_tok) {
+      case 512: return launch_nt<512, kEpiRequests>(q, pairs, coop, stream);
+      case 256: return launch_nt<256, kEpiRequests>(q, pairs, coop, stream);
+      case 128: return launch_nt<128, kEpiRequests>(q, pairs, coop, stream);
+      case 64: return launch_nt<64, kEpiRequests>(q, pairs, coop, stream);
       default: return cudaErrorInvalidValue;
     }
   }
