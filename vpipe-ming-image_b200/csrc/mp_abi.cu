@@ -324,9 +324,12 @@ bool capturing(mp_ctx* c, cudaStream_t stream) {
 
 template <class T>
 int ensure_buf(mp_ctx* c, T** p, size_t* cap, size_t elems, cudaStream_t stream) {
+  // noted at every use, not only where a buffer grows: a graph captured after a
+  // warm-up holds the address of one that is large enough
+  if (!c->captured) (void)capturing(c, stream);
   if (*cap >= elems && *p != nullptr) return MP_OK;
   if (*p != nullptr) {
-    if (capturing(c, stream) || c->captured) {
+    if (c->captured) {
       // a graph may read the old buffer on replay: keep it until destroy
       // (no synchronisation and no free are allowed during a capture)
       c->retired.push_back(*p);
