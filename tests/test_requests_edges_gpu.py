@@ -58,3 +58,58 @@ def test_graph_outlives_larger_calls(m, larger):
     for h in (a[0], b[0], small, large, wt, w):
         h.free()
     ctx.close()
+
+
+@pytest.mark.parametrize("m", [6, 260])
+def test_calls_on_a_stream_given(ctx, m):
+    """stream=: what a call converts is ordered on that stream, not on the busy
+    current one, and its results take no memory that the current one still uses."""
+    rng = np.random.default_rng(m)
+    n, k, cap, r = 256, 128, 3, 16
+    w, _, _ = _weight(ctx, rng, n, k, 8)
+    wt = ctx.transposed(w)
+    bank, fac = _bank(ctx, rng, n, k, cap, r, [r] * cap, training=True)
+    plan = ctx.requests(3, m, cap)
+    third = m // 3
+    # int64, strided, a factor that is not contiguous: each is converted by the call
+    lengths = torch.tensor([[third, 9], [third - 1, 9], [third, 9]], device="cuda")[:, 0]
+    owners = torch.tensor([2, 0, 1], device="cuda")
+    strengths = torch.tensor([1.0, 0.5, -2.0], dtype=torch.float64, device="cuda")
+    a_t = fac[0][0].to(torch.bfloat16).T.contiguous().T
+    b_t = fac[0][1].to(torch.bfloat16).T.contiguous().T
+    x, dy = _bf16(rng, m, k), _bf16(rng, m, n)
+
+    def step(stream=None):
+        bank.set(1, a_t, b_t, stream=stream)
+        plan.plan(lengths, owners, strengths, m, stream=stream)
+        y, v = ctx.linear_requests(w, x, bank, plan, ranks=True, stream=stream)
+        saved = ctx.checkpoint(x, stream=stream)
+        back = ctx.restore(saved, stream=stream)
+        return (y, v, saved.codes, saved.scales, back) + ctx.linear_requests_grad(wt, dy, saved, v, bank, plan,
+                                                                                 stream=stream)
+
+    want = step()
+    torch.cuda.synchronize()
+    # another plan and factor in place, so that a stale conversion would show
+    bank.set(1, -a_t, b_t)
+    plan.plan([m], [1], None, m)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    busy = torch.randn(4096, 4096, device="cuda")
+    for _ in range(3):
+        # memory given back whose last use on the current stream is still to come
+        old = [torch.empty_like(t) for t in want for _ in range(2)]
+        for _ in range(20):
+            busy @ busy
+        for t in old:
+            t.fill_(7)
+        del old, t
+        got = step(stream=side)
+        side.synchronize()
+        kept = [t.clone() for t in got]
+        torch.cuda.synchronize()
+        for p, q, s in zip(want, kept, got):
+            assert torch.equal(p, q) and torch.equal(p, s)
+    ctx.sync_check()
+    for h in (w, wt, bank, plan):
+        h.free()

@@ -166,6 +166,8 @@ class Adapters:
     def set(self, index: int, a, b, stream=None) -> None:
         """a: bf16 [rank, k] (alpha folded in), b: bf16 [n, rank]; torch bf16
         tensors or uint16 numpy arrays, host or device."""
+        if stream is not None:
+            return _on_stream(stream, (a, b), self.set, index, a, b)
         a = _as_bf16_bits(a)
         b = _as_bf16_bits(b)
         rank = a.shape[0]
@@ -174,8 +176,7 @@ class Adapters:
                           f"adapter factors {tuple(a.shape)} / {tuple(b.shape)} do not fit "
                           f"[{self.n}, {self.k}]")
         self.ctx._check(self.ctx.lib.mp_adapters_set(self.ctx.h, self.handle, index, _ptr(a),
-                                                     _ptr(b), rank, _stream_handle(stream)))
-        _keep_for(stream, a, b)
+                                                     _ptr(b), rank, _stream_handle(None)))
 
     def free(self) -> None:
         if self.handle:
@@ -194,6 +195,9 @@ class Requests:
         None (all 1); sequences, or tensors on the device. m: rows of the
         batch (rows past the last request have no adapter); by default the
         sum of the lengths, which has to be on the host then."""
+        if stream is not None:
+            return _on_stream(stream, (lengths, adapters, strengths), self.plan, lengths, adapters,
+                              strengths, m)
         dev = torch.device("cuda", self.ctx.device)
         if m is None:
             if isinstance(lengths, torch.Tensor) and lengths.is_cuda:
@@ -208,8 +212,7 @@ class Requests:
             raise ValueError("lengths, adapters and strengths must have one entry per request")
         self.ctx._check(self.ctx.lib.mp_requests_plan(
             self.ctx.h, self.handle, _ptr(lengths), _ptr(adapters), _ptr(strengths), n, int(m),
-            _stream_handle(stream)))
-        _keep_for(stream, lengths, adapters, strengths)
+            _stream_handle(None)))
 
     def free(self) -> None:
         if self.handle:
@@ -229,12 +232,29 @@ class Checkpoint:
         return self.codes.shape
 
 
-def _keep_for(stream, *tensors) -> None:
-    """Memory read on `stream` is not reused before that stream has read it."""
-    if stream is not None:
-        for t in tensors:
-            if isinstance(t, torch.Tensor) and t.is_cuda:
-                t.record_stream(stream)
+def _on_stream(stream, tensors, call, *args):
+    """call(*args) with `stream` current: conversions of the arguments, memory
+    allocated for results and the launches are all ordered on it (the caller
+    orders it after the work that makes `tensors`, and what reads the results
+    after it). No memory is reused before both streams are done with it: that
+    of `tensors` waits for `stream`, that of the results for the caller's."""
+    callers = torch.cuda.current_stream()
+    with torch.cuda.stream(stream):
+        results = call(*args)
+    _record(stream, tensors)
+    _record(callers, results)
+    return results
+
+
+def _record(stream, t) -> None:
+    if isinstance(t, torch.Tensor):
+        if t.is_cuda:
+            t.record_stream(stream)
+    elif isinstance(t, Checkpoint):
+        _record(stream, (t.codes, t.scales))
+    elif isinstance(t, tuple):
+        for e in t:
+            _record(stream, e)
 
 
 def _rows(name: str, t: torch.Tensor, m: int, k: int, dtype=torch.bfloat16) -> int:
@@ -536,7 +556,10 @@ class Context:
         """y[t] = x[t] · deq(W)^T + s_q (x[t] A_a^T) B_a^T, a the adapter of row
         t's request q; x bf16 [m, k], m as planned. With ranks=True (or an f32
         [m, bank.rank_pad] tensor) returns (y, v), v = s_q x A_a^T, which
-        linear_requests_grad takes."""
+        linear_requests_grad takes. With `stream` the results belong to it."""
+        if stream is not None:
+            return _on_stream(stream, (x, out, ranks), self.linear_requests, w, x, bank, plan, out,
+                              ranks)
         m = x.shape[0]
         n, k = w.info.n, w.info.k
         ldx = _rows("x", x, m, k)
@@ -555,7 +578,7 @@ class Context:
             vp = v.data_ptr()
         rc = self.lib.mp_linear_requests(
             self.h, w.handle, x.data_ptr(), ldx, bank.handle, plan.handle, out.data_ptr(), ldy, vp,
-            ldv, m, _stream_handle(stream))
+            ldv, m, _stream_handle(None))
         if rc != MP_OK:
             self._check(rc)
         return out if v is None else (out, v)
@@ -573,7 +596,11 @@ class Context:
         """The backward pass of linear_requests, W held fixed: (dx bf16 [m, k],
         da f32 [capacity, max_rank, k], db f32 [capacity, n, max_rank]), None
         for what is not needed; capacity is the plan's. wt: transposed(w); x:
-        bf16 [m, k] or its Checkpoint; v: the forward call's ranks."""
+        bf16 [m, k] or its Checkpoint; v: the forward call's ranks. With
+        `stream` the results belong to it."""
+        if stream is not None:
+            return _on_stream(stream, (dy, x, v), self.linear_requests_grad, wt, dy, x, v, bank, plan,
+                              need_dx, need_factors)
         m, n, k = dy.shape[0], wt.info.k, wt.info.n
         ldy = _rows("dy", dy, m, n)
         dx = da = db = None
@@ -599,28 +626,34 @@ class Context:
             dap, dbp = da.data_ptr(), db.data_ptr()
         rc = self.lib.mp_linear_requests_grad(
             self.h, wt.handle, dy.data_ptr(), ldy, xp, ldx, qp, ldq, sp, vp, ldv, bank.handle,
-            plan.handle, dxp, lddx, dap, dbp, m, _stream_handle(stream))
+            plan.handle, dxp, lddx, dap, dbp, m, _stream_handle(None))
         if rc != MP_OK:
             self._check(rc)
         return dx, da, db
 
     # -- activation checkpoints --------------------------------------------------
     def checkpoint(self, x: torch.Tensor, stream=None) -> Checkpoint:
-        """bf16 rows [m, k] in 8 bits, a scale for every 128 features of a row."""
+        """bf16 rows [m, k] in 8 bits, a scale for every 128 features of a row.
+        With `stream` the result belongs to it."""
+        if stream is not None:
+            return _on_stream(stream, (x,), self.checkpoint, x)
         m, k = x.shape
         ldx = _rows("x", x, m, k)
         ldq = (k + 15) // 16 * 16
         q = x.new_empty((m, ldq), dtype=torch.int8)
         scale = x.new_empty(((k + 127) // 128, m), dtype=torch.float32)
         rc = self.lib.mp_checkpoint(self.h, x.data_ptr(), ldx, m, k, q.data_ptr(), ldq,
-                                    scale.data_ptr(), _stream_handle(stream))
+                                    scale.data_ptr(), _stream_handle(None))
         if rc != MP_OK:
             self._check(rc)
         return Checkpoint(q if ldq == k else q[:, :k], scale.t())
 
     def restore(self, saved: Checkpoint, out: torch.Tensor | None = None,
                 stream=None) -> torch.Tensor:
-        """The bf16 rows a checkpoint stands for."""
+        """The bf16 rows a checkpoint stands for. With `stream` the result
+        belongs to it."""
+        if stream is not None:
+            return _on_stream(stream, (saved, out), self.restore, saved, out)
         m, k = saved.codes.shape
         ldq = _rows("codes", saved.codes, m, k, torch.int8)
         _check_scales(saved.scales, m, k)
@@ -629,7 +662,7 @@ class Context:
         else:
             ldx = _rows("out", out, m, k)
         rc = self.lib.mp_restore(self.h, saved.codes.data_ptr(), ldq, saved.scales.data_ptr(), m, k,
-                                 out.data_ptr(), ldx, _stream_handle(stream))
+                                 out.data_ptr(), ldx, _stream_handle(None))
         if rc != MP_OK:
             self._check(rc)
         return out
