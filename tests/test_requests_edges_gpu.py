@@ -113,3 +113,46 @@ def test_calls_on_a_stream_given(ctx, m):
     ctx.sync_check()
     for h in (w, wt, bank, plan):
         h.free()
+
+
+def _like(got, ref, name):
+    """Infinities and NaN where the formula in 64 bits has them, with its signs."""
+    got = got.double()
+    assert torch.equal(torch.isnan(got), torch.isnan(ref)), f"{name}: NaN in other places"
+    wild = torch.isinf(ref)
+    assert torch.equal(torch.isinf(got), wild) and torch.equal(got[wild], ref[wild]), f"{name}: other infinities"
+
+
+# rank-space rows in runs; runs, then the projection; the tensor core's tiles with and without a cluster
+@pytest.mark.parametrize("m,k,bits", [(6, 640, 0), (90, 640, 8), (2100, 640, 0), (3000, 128, 4)])
+def test_infinite_rows_and_ranks_below_the_banks(ctx, m, k, bits):
+    """An infinity in x meets an adapter's own ranks and not the padding up to the
+    bank's; an adapter that was never set adds nothing to it."""
+    rng = np.random.default_rng(m + k)
+    n, cap, ranks = 256, 3, [3, 20]
+    w, w64, _ = _weight(ctx, rng, n, k, bits)
+    bank, fac = _bank(ctx, rng, n, k, cap, 20, ranks)  # adapter 2: never set
+    plan = ctx.requests(3, m, cap)
+    q = m // 3
+    x = _bf16(rng, m, k)
+    rows = [0, q - 1, q, 2 * q, m - 1]
+    for i, t in enumerate(rows):
+        x[t, (17 * i + 5) % k] = float("inf") * (-1) ** i
+    plan.plan([q, q, m - 2 * q], [0, 1, 2], [0.5, -1.0, 1.0], m)
+    y, v = ctx.linear_requests(w, x, bank, plan, ranks=True)
+    plan.plan([q, q, m - 2 * q], [0, 1, -1], [0.5, -1.0, 1.0], m)
+    y0, v0 = ctx.linear_requests(w, x, bank, plan, ranks=True)
+    ctx.sync_check()
+    assert torch.equal(y[2 * q:].view(torch.int16), y0[2 * q:].view(torch.int16)), "never set: the base's bits"
+    assert not v[:q, 3:].any() and not v[:, 20:].any() and not v[2 * q:].any() and not v0[2 * q:].any()
+    rv = torch.zeros(m, bank.rank_pad, dtype=torch.float64, device="cuda")
+    ry = x.double() @ w64.T
+    for at, a, s in ((slice(0, q), 0, 0.5), (slice(q, 2 * q), 1, -1.0)):
+        t = s * (x[at].double() @ fac[a][0].T)
+        rv[at, :ranks[a]] = t
+        ry[at] += t @ fac[a][1].T
+    assert torch.isinf(ry).any()
+    _like(v, rv, "v")
+    _like(y, ry, "y")
+    for h in (w, bank, plan):
+        h.free()

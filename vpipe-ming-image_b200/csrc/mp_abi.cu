@@ -117,7 +117,7 @@ struct mp_adapters {
   uint16_t* b = nullptr;   // [cap][n][rp]
   uint16_t* at = nullptr;  // [cap][k][rp] (training)
   uint16_t* bt = nullptr;  // [cap][rp][np] (training)
-  int32_t* bad = nullptr;  // [cap]: a factor held a value that is not finite
+  mp::AdapterInfo* info = nullptr;  // [cap]
   CUtensorMap tm_b;        // [cap * n, rp], box {64, 128}, SW128
   CUtensorMap tm_at;       // [cap * k, rp]
   CUtensorMap tm_a;        // [cap * rp, k], box {64, rp}, SW128
@@ -2065,7 +2065,7 @@ mp::RankParams rank_params(const mp_ctx* c, const RequestsLaunch& ext, const voi
   r.fp = ext.fp;
   r.k = k;
   r.rp = ext.bank->rp;
-  r.bad = ext.bank->bad;
+  r.info = ext.bank->info;
   r.plan = ext.req->plan;
   r.v32 = ext.v32;
   r.ld32 = ext.ld32;
@@ -2241,7 +2241,7 @@ int mp_adapters_create(mp_ctx* c, int n, int k, int capacity, int max_rank, int 
   // one allocation, zeroed: an adapter that was never set adds nothing
   const size_t cr = static_cast<size_t>(capacity) * b->rp;  // a multiple of 16: every part is 16-byte aligned
   const size_t ea = cr * b->kp, eb = cr * n, eat = training ? cr * k : 0, ebt = training ? cr * b->np : 0;
-  const size_t bytes = (ea + eb + eat + ebt) * sizeof(uint16_t) + static_cast<size_t>(capacity) * sizeof(int32_t);
+  const size_t bytes = (ea + eb + eat + ebt) * sizeof(uint16_t) + static_cast<size_t>(capacity) * sizeof(mp::AdapterInfo);
   cudaError_t e = cudaMalloc(&b->a, bytes);
   if (e == cudaSuccess) e = cudaMemset(b->a, 0, bytes);
   if (e == cudaSuccess) e = cudaStreamSynchronize(nullptr);  // a call on any stream may follow
@@ -2254,7 +2254,7 @@ int mp_adapters_create(mp_ctx* c, int n, int k, int capacity, int max_rank, int 
   b->b = b->a + ea;
   b->at = training ? b->b + eb : nullptr;
   b->bt = training ? b->at + eat : nullptr;
-  b->bad = reinterpret_cast<int32_t*>(b->b + eb + eat + ebt);
+  b->info = reinterpret_cast<mp::AdapterInfo*>(b->b + eb + eat + ebt);
   const uint64_t pitch = static_cast<uint64_t>(b->rp) * 2, cap = static_cast<uint64_t>(capacity);
   if (!encode_2d(&b->tm_b, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, b->b, b->rp, cap * n, pitch, 64, 128,
                  CU_TENSOR_MAP_SWIZZLE_128B) ||
@@ -2294,7 +2294,7 @@ int mp_adapters_set(mp_ctx* c, mp_adapters* b, int index, const uint16_t* fa, co
   p.b = b->b + i * b->n;
   p.at = b->at != nullptr ? b->at + i * b->k : nullptr;
   p.bt = b->bt != nullptr ? b->bt + i * b->np : nullptr;
-  p.bad = b->bad + index;
+  p.info = b->info + index;
   p.n = b->n;
   p.k = b->k;
   p.rank = rank;
@@ -2304,7 +2304,7 @@ int mp_adapters_set(mp_ctx* c, mp_adapters* b, int index, const uint16_t* fa, co
   const size_t ka = static_cast<size_t>(b->k) * 2, rb = static_cast<size_t>(rank) * 2;
   MP_CUDA(c, cudaMemcpy2DAsync(p.a, static_cast<size_t>(b->kp) * 2, fa, ka, ka, rank, cudaMemcpyDefault, s));
   MP_CUDA(c, cudaMemcpy2DAsync(p.b, static_cast<size_t>(b->rp) * 2, fb, rb, rb, b->n, cudaMemcpyDefault, s));
-  MP_CUDA(c, cudaMemsetAsync(p.bad, 0, sizeof(int32_t), s));
+  MP_CUDA(c, cudaMemsetAsync(p.info, 0, sizeof(mp::AdapterInfo), s));
   MP_CUDA(c, mp::launch_bank_set(p, s));
   c->eng.kernels += 1;
   return MP_OK;

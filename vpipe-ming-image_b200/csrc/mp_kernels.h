@@ -194,15 +194,23 @@ struct PlanParams {
   uint32_t* err;
 };
 
+// What a bank knows of an adapter. Rank-space columns from `rank` on are zero by
+// definition, not by a product with the factor's padding (an infinity in x times
+// its zeros would be NaN); rank 0: never set.
+struct alignas(8) AdapterInfo {
+  int32_t bad;  // 1: a factor held a value that is not finite
+  int32_t rank;
+};
+
 // Finishes adapter `index` of a bank after its factors' valid parts were
-// copied in: zeros past rank, zeros in place of values that are not finite
-// (then bad[index] = 1), and the transposed copies of a training bank.
+// copied in: zeros past rank, zeros in place of values that are not finite,
+// the adapter's entry of `info`, and the transposed copies of a training bank.
 struct BankSetParams {
   uint16_t* a;   // [rp][kp] of this adapter
   uint16_t* b;   // [n][rp]
   uint16_t* at;  // [k][rp] or null
   uint16_t* bt;  // [rp][np] or null
-  int32_t* bad;
+  AdapterInfo* info;
   int32_t n, k, rank, rp, kp, np;
 };
 
@@ -215,7 +223,7 @@ struct RankParams {
   int64_t ldx;
   const uint16_t* f;  // bf16 [cap][rp][fp]
   int32_t fp, k, rp;
-  const int32_t* bad;
+  const AdapterInfo* info;  // [cap]
   RequestPlan plan;
   // outputs (either may be null)
   float* v32;         // f32 [m][ld32], columns < rp; with clear_v32 zeros in the
@@ -323,7 +331,7 @@ struct AttnParams {
 };
 
 // 8-bit activation checkpoint (mp_checkpoint.cu): per row and group of
-// kCkGroup features, scale = max|x| / 127 and q = rint(x * (127 / max|x|));
+// kCkGroup features, scale = max|x| / 127 and q = rint(x * (127 * (1 / max|x|)));
 // groups whose max|x| is below kCkTiny hold zeros.
 constexpr int kCkGroup = 128;
 constexpr float kCkTiny = 7.703719777548943e-34f;  // 2^-110

@@ -111,9 +111,15 @@ __device__ __forceinline__ RankUnit rank_unit(const RankParams& p, int i) {
 }
 
 // The request's strength; NaN with a factor that is not finite (it is stored as
-// zeros, and its request's rows are NaN).
-__device__ __forceinline__ float unit_scale(const RankParams& p, const RankUnit& u) {
-  return p.bad[u.adapter] != 0 ? __int_as_float(0x7FC00000) : p.plan.block_s[unit_level(p)][u.unit];
+// zeros, and its request's rows are NaN). And the adapter's own ranks: the columns
+// past them are zeros.
+struct UnitScale {
+  float by;
+  int ranks;
+};
+__device__ __forceinline__ UnitScale unit_scale(const RankParams& p, const RankUnit& u) {
+  const AdapterInfo info = p.info[u.adapter];
+  return {info.bad != 0 ? __int_as_float(0x7FC00000) : p.plan.block_s[unit_level(p)][u.unit], info.rank};
 }
 
 // The unit's rows of vblk outside its 128, or its rows of v32 if its request is
@@ -277,9 +283,10 @@ __global__ void __launch_bounds__(kRankThreads, COLS <= 64 ? 2 : 1) rank_tiles_k
       clear_rows(p, u, threadIdx.x - 32 * kSumWarp0, 32 * 4);
       if (r >= rows) continue;
       const bool mine = r >= u.lo && r < u.hi;
-      const float scale = unit_scale(p, u);
+      const UnitScale scale = unit_scale(p, u);
+      const int ranks = mine ? scale.ranks : 0;
 #pragma unroll
-      for (int c = 0; c < COLS; ++c) sums[c] = mine ? sums[c] * scale : 0.0f;
+      for (int c = 0; c < COLS; ++c) sums[c] = c < ranks ? sums[c] * scale.by : 0.0f;
       if (mine && p.v32 != nullptr) {
         float* at = p.v32 + static_cast<int64_t>(u.row0 + r) * p.ld32;
 #pragma unroll
@@ -312,7 +319,7 @@ __global__ void __launch_bounds__(kRankThreads, COLS <= 64 ? 2 : 1) rank_tiles_k
     if (!aborted) {
       // each CTA adds up and writes its share of the rows
       const RankUnit u = rank_unit(p, unit0);
-      const float scale = u.work ? unit_scale(p, u) : 0.0f;
+      const UnitScale scale = u.work ? unit_scale(p, u) : UnitScale{0.0f, 0};
       clear_rows(p, u, rank * kRankThreads + threadIdx.x, count * kRankThreads);
       const int share = (rows + count - 1) / count, first = rank * share, last = min(first + share, rows);
       const int quads = (p.vblk != nullptr ? p.ldb : p.rp) / 4;
@@ -330,7 +337,8 @@ __global__ void __launch_bounds__(kRankThreads, COLS <= 64 ? 2 : 1) rank_tiles_k
 #pragma unroll
           for (int z = 1; z < kMaxRankSplits; ++z)
             if (z < count) s.x += o[z].x, s.y += o[z].y, s.z += o[z].z, s.w += o[z].w;
-          s.x *= scale, s.y *= scale, s.z *= scale, s.w *= scale;
+          s.x = c < scale.ranks ? s.x * scale.by : 0.0f, s.y = c + 1 < scale.ranks ? s.y * scale.by : 0.0f;
+          s.z = c + 2 < scale.ranks ? s.z * scale.by : 0.0f, s.w = c + 3 < scale.ranks ? s.w * scale.by : 0.0f;
           if (p.v32 != nullptr) *reinterpret_cast<float4*>(p.v32 + static_cast<int64_t>(u.row0 + r) * p.ld32 + c) = s;
         }
         if (p.vblk != nullptr)

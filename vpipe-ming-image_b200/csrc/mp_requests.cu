@@ -241,12 +241,13 @@ __global__ void __launch_bounds__(256) bank_set_kernel(const __grid_constant__ B
   __shared__ uint16_t sm[32][33];
   const int rt = (p.rp + 31) / 32, kt = (p.kp + 31) / 32, nt = (p.n + 31) / 32;
   int i = blockIdx.x;
+  if (i == 0 && threadIdx.x == 0) p.info->rank = p.rank;
   if (i < rt * kt) {  // A [rp][kp], transposed [k][rp]
-    finish_tile(p.a, p.kp, p.at, p.rp, p.rp, p.kp, p.rank, p.k, p.k, i / kt * 32, i % kt * 32, p.bad, sm);
+    finish_tile(p.a, p.kp, p.at, p.rp, p.rp, p.kp, p.rank, p.k, p.k, i / kt * 32, i % kt * 32, &p.info->bad, sm);
   } else {  // B [n][rp], transposed [rp][np]
     i -= rt * kt;
     if (i < rt * nt)
-      finish_tile(p.b, p.rp, p.bt, p.np, p.n, p.rp, p.n, p.rank, p.rp, i / rt * 32, i % rt * 32, p.bad, sm);
+      finish_tile(p.b, p.rp, p.bt, p.np, p.n, p.rp, p.n, p.rank, p.rp, i / rt * 32, i % rt * 32, &p.info->bad, sm);
   }
 }
 
@@ -373,8 +374,10 @@ __global__ void __launch_bounds__(32 * kRankWarps) rank_rows_kernel(const __grid
 #pragma unroll
   for (int w = 1; w < kRankWarps; ++w) sum += part[w][r][row];
   sum *= __int_as_float(ch.w);
+  const AdapterInfo info = p.info[adapter];
   // a factor that is not finite is stored as zeros; its request's rows are NaN
-  if (p.bad[adapter] != 0) sum = __int_as_float(0x7FC00000);
+  if (info.bad != 0) sum = __int_as_float(0x7FC00000);
+  if (r0 + r >= info.rank) sum = 0.0f;
   const int t = ch.x + row;
   if (p.v32 != nullptr) p.v32[static_cast<int64_t>(t) * p.ld32 + r0 + r] = sum;
   if (p.vblk != nullptr) {
