@@ -7,8 +7,8 @@ import numpy as np
 import pytest
 import torch
 
-from mingproj.proj import Context
-from test_requests_gpu import _bank, _bf16, _weight
+from mingproj.proj import Context, MP_QUANT_SYMMETRIC
+from test_requests_gpu import _bank, _bf16, _forward_ref, _segments, _weight, _within
 
 pytestmark = pytest.mark.gpu
 
@@ -154,5 +154,39 @@ def test_infinite_rows_and_ranks_below_the_banks(ctx, m, k, bits):
     assert torch.isinf(ry).any()
     _like(v, rv, "v")
     _like(y, ry, "y")
+    for h in (w, bank, plan):
+        h.free()
+
+
+@pytest.mark.parametrize("bits,mode", [(0, 0), (8, 0), (4, 0), (8, MP_QUANT_SYMMETRIC)])
+@pytest.mark.parametrize("m", [1, 6, 16, 32, 33])
+def test_wild_rows_of_few(ctx, m, bits, mode):
+    """Up to 32 rows the codes of a packed weight are multiplied as whole numbers:
+    infinities, and values whose products with the codes overflow where those
+    with the weights do not, come out as the formula has them."""
+    rng = np.random.default_rng(m + bits)
+    n, k, cap, r = 264, 320, 2, 16
+    w, w64, wround = _weight(ctx, rng, n, k, bits, mode)
+    bank, fac = _bank(ctx, rng, n, k, cap, r, [r, 5])
+    lengths, owners, strengths = [m - m // 2, m // 4], [1, 0], [0.5, -1.0]
+    plan = ctx.requests(2, m, cap)
+    plan.plan(lengths, owners, strengths, m)
+    segs = list(_segments(m, lengths, owners, strengths))
+    for value in (float("inf"), float("-inf"), float("nan"), 3e37, -1e38):
+        x = _bf16(rng, m, k)
+        for t in range(0, m, 2):
+            x[t, (7 * t + 64) % k] = value
+        y, v = ctx.linear_requests(w, x, bank, plan, ranks=True)
+        ctx.sync_check()
+        ry, by, rv, bv = _forward_ref(x, w64, wround, fac, segs, bank.rank_pad)
+        # (the bound's NaN and infinities stand where the formula's are)
+        fine = torch.isfinite(ry)
+        assert fine.all() or not np.isfinite(value)
+        if not np.isfinite(value):
+            _like(y, ry, "y")
+        zero = torch.zeros_like(ry)
+        _within("y", torch.where(fine, y.double(), zero), torch.where(fine, ry, zero), torch.where(fine, by, zero + 1))
+        if np.isfinite(value):
+            _within("v", v, rv, bv)
     for h in (w, bank, plan):
         h.free()

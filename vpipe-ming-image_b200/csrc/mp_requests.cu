@@ -456,6 +456,28 @@ __device__ __forceinline__ void few_x(const uint16_t* at, int col, int k, uint32
   }
 }
 
+// W x of one feature and row of a packed weight, weight by weight, for a sum that
+// the codes' arithmetic does not hold: scale sum_k q x and offset sum_k x are of
+// opposite signs and up to 255 times x, so an infinity in x came out as inf - inf,
+// and x beyond 1e36 overflowed where W x does not. Rare, and never inlined: the
+// kernel's loop keeps its registers. Ends at a NaN, which stays one.
+template <int BITS>
+__device__ __noinline__ float few_dot(const FewParams& p, int n, int t) {
+  const uint8_t* w = p.w + static_cast<size_t>(n) * p.w_pitch;
+  const uint32_t* sb = p.sb + static_cast<size_t>(n) * p.sb_stride;
+  const uint16_t* x = p.x + static_cast<int64_t>(t) * p.ldx;
+  float sum = 0.0f;
+  for (int i = 0; i < p.k / 64 && sum == sum; ++i) {
+    const float scale = bf16_bits_to_f32(sb[i] & 0xFFFFu), bias = bf16_bits_to_f32(sb[i] >> 16);
+    for (int c = 64 * i; c < 64 * i + 64; ++c) {
+      const float q = BITS == 8 ? static_cast<float>(w[c] ^ (p.code_xor & 0xFFu)) - p.zero
+                                : static_cast<float>((w[c >> 1] >> (4 * (c & 1))) & 0xFu);
+      sum = fmaf(fmaf(q, scale, bias), bf16_bits_to_f32(x[c]), sum);
+    }
+  }
+  return sum;
+}
+
 // Blocks an SM that the registers are cut to. With 17 to 32 rows and bf16 two
 // blocks of 8 warps, not one, take 3840x3840 from 23.0 to 16.8 us; the codes of
 // packed weights do not fit beside four tiles of x then.
@@ -589,6 +611,9 @@ __global__ void __launch_bounds__(32 * WARPS, kFewBlocks<BITS, NT, WARPS>)
     float sum = part[0][f][t];
 #pragma unroll
     for (int w = 1; w < WARPS; ++w) sum += part[w][f][t];
+    if constexpr (BITS != 0) {
+      if (!isfinite(sum)) sum = few_dot<BITS>(p, f0 + f, t);
+    }
     const int a = p.row_adapter[t];
     if (a >= 0) {
       const uint16_t* br = p.b + (static_cast<size_t>(a) * p.n + f0 + f) * p.rp;
