@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from mingproj.proj import Context, MP_QUANT_SYMMETRIC
-from test_requests_gpu import _bank, _bf16, _forward_ref, _segments, _weight, _within
+from test_requests_gpu import _bank, _bf16, _forward_ref, _grad_ref, _segments, _weight, _within
 
 pytestmark = pytest.mark.gpu
 
@@ -189,4 +189,64 @@ def test_wild_rows_of_few(ctx, m, bits, mode):
         if np.isfinite(value):
             _within("v", v, rv, bv)
     for h in (w, bank, plan):
+        h.free()
+
+
+# m, n, k, capacity, bank's rank, rows of the requests (adapter 0, 1, 0): clusters and walking CTAs, every width of sums
+WILD_GRADS = [
+    (33, 136, 200, 2, 7, [11, 10, 9]),
+    (700, 264, 640, 3, 16, [300, 100, 299]),
+    (1500, 1280, 1024, 40, 12, [500, 480, 510]),
+    (900, 640, 520, 2, 64, [300, 300, 300]),
+    (1200, 1280, 1024, 24, 50, [400, 380, 410]),
+    (640, 512, 392, 2, 128, [200, 200, 200]),
+    (700, 1280, 1280, 16, 100, [230, 210, 240]),
+]
+
+
+@pytest.mark.parametrize("saved", [16, 8])
+@pytest.mark.parametrize("case", WILD_GRADS, ids=[f"m{c[0]}_cap{c[3]}_r{c[4]}" for c in WILD_GRADS])
+def test_wild_values_in_gradients(ctx, case, saved):
+    """u and v are multiplied in three parts: an infinity in x or dy meets what
+    they are and not their parts; a checkpoint's scale that overflows with u does
+    not reach the codes that are 0."""
+    m, n, k, cap, max_rank, lengths = case
+    rng = np.random.default_rng(m + max_rank + saved)
+    ranks = [max_rank, max(1, max_rank // 3)]
+    owners, strengths = [0, 1, 0], [1.0, -0.5, 0.75]
+    w, w64, wround = _weight(ctx, rng, n, k, 0)
+    wt = ctx.transposed(w)
+    bank, fac = _bank(ctx, rng, n, k, cap, max_rank, ranks, training=True)
+    plan = ctx.requests(3, m, cap)
+    plan.plan(lengths, owners, strengths, m)
+    segs = list(_segments(m, lengths, owners, strengths))
+    rows = [0, lengths[0] + 1, lengths[0] + lengths[1] + 2, sum(lengths) - 1]
+    for which, value in (("x", float("inf")), ("dy", float("-inf")), ("x", float("nan")), ("x", 3e38)):
+        x, dy = _bf16(rng, m, k), _bf16(rng, m, n)
+        for i, t in enumerate(rows):
+            (x if which == "x" else dy)[t, 3 + 131 * (i % 2)] = value * (-1) ** i
+        if value == 3e38:
+            dy *= 64.0  # u past 1 / 2.4e36 of f32's largest
+        _, v = ctx.linear_requests(w, x, bank, plan, ranks=True)
+        v = torch.where(torch.isfinite(v), v, torch.zeros_like(v)) if which == "x" else v
+        x_in = ctx.checkpoint(x) if saved == 8 else x
+        kept = x if saved == 16 else x_in.codes.double() * x_in.scales.double().repeat_interleave(128, 1)[:, :k]
+        dx, da, db = ctx.linear_requests_grad(wt, dy, x_in, v, bank, plan)
+        again = ctx.linear_requests_grad(wt, dy, x_in, v, bank, plan)
+        ctx.sync_check()
+        refs = _grad_ref(kept, dy, w64, wround, fac, segs, v, cap, max_rank)
+        for a, r in enumerate(ranks):  # a product with the padding is none
+            refs[2][0][a, :, r:] = 0.0
+            refs[2][1][a, :, r:] = 1e-30
+        for name, got, twice, (ref, bound) in zip(("dx", "da", "db"), (dx, da, db), again, refs):
+            assert torch.equal(got.view(torch.int16), twice.view(torch.int16)), "the same call twice"
+            if value != 3e38:
+                _like(got, ref, name)
+            # where the sum of the products' magnitudes (at most 2^16 of the bound) fits f32
+            fine = torch.isfinite(ref) & (bound < 2.0 ** -16 * 1e38)
+            assert fine.any()
+            zero = torch.zeros_like(ref)
+            _within(name, torch.where(fine, got.double(), zero), torch.where(fine, ref, zero),
+                    torch.where(fine, bound, zero + 1))
+    for h in (w, wt, bank, plan):
         h.free()

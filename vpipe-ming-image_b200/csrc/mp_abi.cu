@@ -2510,6 +2510,7 @@ int mp_linear_requests_grad(mp_ctx* c, const mp_weight* wt, const void* dy, int6
   mp::GradParams g;
   std::memset(&g, 0, sizeof(g));
   g.r = b->max_rank;
+  g.info = b->info;
   g.plan = r->plan;
   g.rp = b->rp;
   g.wait_limit_ns = c->wait_limit_ns;

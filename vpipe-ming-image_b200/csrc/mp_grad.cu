@@ -189,12 +189,24 @@ __device__ __forceinline__ uint64_t mn_desc(uint32_t tile, int kk) {
   return d;
 }
 
-// The next bf16 part of two values, which keep what is left of them.
+// The next bf16 part of two values, which keep what is left of them. Parts are cut
+// off towards zero, 8 bits each, and the rest is taken 2^-24 of the part too large:
+// so all parts of a value that is not 0 have its sign and none is 0, and an infinity
+// in x meets three that agree (0 would make it a NaN, the other sign inf - inf). In
+// all they are the value and up to 2^-24 of it, half a unit in its last place.
 __device__ __forceinline__ uint32_t take_part(float& a, float& b) {
-  const uint32_t w = pack_bf16x2(a, b);
-  a -= __uint_as_float(w << 16);
-  b -= __uint_as_float(w & 0xFFFF0000u);
-  return w;
+  constexpr float kLess = -0.99999994f;  // 2^-24 - 1
+  const uint32_t wa = __float_as_uint(a), wb = __float_as_uint(b);
+  a = fmaf(__uint_as_float(wa & 0xFFFF0000u), kLess, a);
+  b = fmaf(__uint_as_float(wb & 0xFFFF0000u), kLess, b);
+  return __byte_perm(wa, wb, 0x7632);
+}
+
+// `f`, or with its sign f32's largest where it is an infinity. A NaN stays one.
+__device__ __forceinline__ float no_infinity(float f) {
+  float d;
+  asm("min.NaN.xorsign.abs.f32 %0, %1, %2;" : "=f"(d) : "f"(f), "f"(3.4028235e38f));
+  return d;
 }
 
 // 4 bytes, asynchronously; and their arrival on an mbarrier whose count has a
@@ -252,8 +264,10 @@ struct ItemIter {
 
 // Warps 2-9, in two groups: a stage's work is a chain of latencies (its copies'
 // arrival, shared memory, the conversions, the fence), so two stages are worked on
-// at once. TASKS: 16-value pieces of a 64-row stage of u per thread.
-template <int TASKS>
+// at once. TASKS: 16-value pieces of a 64-row stage of u per thread. CODES: a
+// member's x is a checkpoint (an instantiation of its own, so that the others do
+// not carry its steps).
+template <int TASKS, bool CODES>
 __device__ void convert(const GradParams& p, const GradSmem& sm, const GradGeo& geo, const PartCols& pc, int item0,
                         int step, int rank, int count) {
   const int tid = (threadIdx.x - 32 * kConvWarp0) % kConvGroup, lane = threadIdx.x & 31;
@@ -275,7 +289,7 @@ __device__ void convert(const GradParams& p, const GradSmem& sm, const GradGeo& 
   ItemIter items(p, item0, step);
   for (int i = items.next(); i >= 0; i = items.next()) {
     const Item item = item_of(p, i);
-    const bool codes = item.mb->scale != nullptr;
+    const bool codes = CODES && item.mb->scale != nullptr;
     TileIter it(p.plan, item.a, rank, count);
     int t0, rows;
     for (; it.next(t0, rows); at_stage.next(geo.stages)) {
@@ -299,30 +313,43 @@ __device__ void convert(const GradParams& p, const GradSmem& sm, const GradGeo& 
           const float4 a = ld_shared_f4(at), b = ld_shared_f4(at + 16);
           f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w;
           f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
-          if (codes) {
-            float by;
-            asm volatile("ld.shared.f32 %0, [%1];" : "=f"(by) : "r"(xs + geo.scale_off + row_of[j] * 4u));
-#pragma unroll
-            for (int e = 0; e < 8; ++e) f[e] *= by;
-          }
         }
         float top = 0.0f;
 #pragma unroll
         for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(f[e]));
+        if (codes && row_of[j] < rows) {
+          float by;
+          asm volatile("ld.shared.f32 %0, [%1];" : "=f"(by) : "r"(xs + geo.scale_off + row_of[j] * 4u));
+          // u times the scale. A product past f32's largest stays there: a code of 0
+          // then gives 0, not the NaN of 0 and an infinity
+#pragma unroll
+          for (int e = 0; e < 8; ++e) f[e] = no_infinity(f[e] * by);
+        }
         const uint32_t row = parts + row_of[j] * 128u, sw = static_cast<uint32_t>(row_of[j] & 7);
 #pragma unroll
         for (int part = 0; part < kParts; ++part) {
           uint32_t w[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) w[e] = take_part(f[2 * e], f[2 * e + 1]);
-          if (part == 0 && top > 3.38e38f) {
-            // an infinity is all in its first part (inf - inf would be NaN)
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-              if ((w[e >> 1] >> (16 * (e & 1)) & 0x7FFFu) == 0x7F80u) f[e] = 0.0f;
-          }
           const uint32_t col = col_of[j] + (part == 2 ? pc.third : part * p.rp);
           st_shared_v4(row + (col >> 6) * kBoxBytes + (((col >> 3 & 7u) ^ sw) << 4), w[0], w[1], w[2], w[3]);
+        }
+        if (isinf(top)) {
+          // all parts of an infinite u are what it is (inf - inf gave NaN)
+#pragma unroll 1
+          for (int e = col_of[j]; e < col_of[j] + 8; ++e) {
+            float u, by = 1.0f;
+            asm volatile("ld.shared.f32 %0, [%1];" : "=f"(u) : "r"(xs + geo.u_off + (row_of[j] * p.rp + e) * 4u));
+            if (!isinf(u)) continue;
+            if (codes) asm volatile("ld.shared.f32 %0, [%1];" : "=f"(by) : "r"(xs + geo.scale_off + row_of[j] * 4u));
+            const uint16_t v = static_cast<uint16_t>(__float_as_uint(u * by) >> 16);
+#pragma unroll 1
+            for (int part = 0; part < kParts; ++part) {
+              const uint32_t col = e + (part == 2 ? pc.third : part * p.rp);
+              const uint32_t at = row + (col >> 6) * kBoxBytes + (((col >> 3 & 7u) ^ sw) << 4) + (col & 7u) * 2u;
+              asm volatile("st.shared.u16 [%0], %1;" ::"r"(at), "h"(v) : "memory");
+            }
+          }
         }
       }
       if (codes) {
@@ -362,7 +389,7 @@ __device__ void convert(const GradParams& p, const GradSmem& sm, const GradGeo& 
   }
 }
 
-template <int TASKS>
+template <int TASKS, bool CODES>
 __global__ void __launch_bounds__(kGradThreads<TASKS>, TASKS == 1 ? 2 : 1)
     adapter_grad_kernel(const __grid_constant__ GradParams p) {
   extern __shared__ uint8_t grad_raw[];
@@ -372,7 +399,7 @@ __global__ void __launch_bounds__(kGradThreads<TASKS>, TASKS == 1 ? 2 : 1)
   const int step = p.workers;
   const int col0 = warp >= kSumWarp0 + 4 ? kSumCols<TASKS> : 0;  // the adding warp's first rank
   const PartCols pc = part_cols(p.rp);
-  const GradGeo geo = grad_geo(p.rp, p.codes != 0);
+  const GradGeo geo = grad_geo(p.rp, CODES);
   GradSmem sm;
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(grad_raw) + 1023u) & ~uintptr_t(1023u));
   sm.tiles = smem_u32(base);
@@ -468,7 +495,7 @@ __global__ void __launch_bounds__(kGradThreads<TASKS>, TASKS == 1 ? 2 : 1)
     for (int i = items.next(); i >= 0 && ok; i = items.next()) {
       const Item item = item_of(p, i);
       const GradMember& mb = *item.mb;
-      const bool codes = mb.scale != nullptr;
+      const bool codes = CODES && mb.scale != nullptr;
       TileIter it(p.plan, item.a, rank, count);
       int t0, rows;
       for (; ok && it.next(t0, rows); at_stage.next(geo.stages), ++sent) {
@@ -546,7 +573,7 @@ __global__ void __launch_bounds__(kGradThreads<TASKS>, TASKS == 1 ? 2 : 1)
         }
     }
   } else if (warp < kSumWarp0) {
-    convert<TASKS>(p, sm, geo, pc, item0, step, rank, count);
+    convert<TASKS, CODES>(p, sm, geo, pc, item0, step, rank, count);
   } else {
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const int f = (warp & 3) * 32 + lane;
@@ -584,6 +611,15 @@ __global__ void __launch_bounds__(kGradThreads<TASKS>, TASKS == 1 ? 2 : 1)
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&sm.taken[b]));
+      }
+      bool nan = false;
+#pragma unroll
+      for (int c = 0; c < kSumCols<TASKS>; ++c) nan = nan || sums[c] != sums[c];
+      if (nan) {
+        // past the adapter's own ranks u is 0: so are the sums, whatever x held
+        const int own = p.info[item.a].rank;
+#pragma unroll
+        for (int c = 0; c < kSumCols<TASKS>; ++c) sums[c] = col0 + c < own ? sums[c] : 0.0f;
       }
       if (count > 1 || !ok) break;  // a cluster has one item
       const int ff = item.f_tile * kTileF + f;
@@ -685,10 +721,10 @@ __global__ void __launch_bounds__(kGradThreads<TASKS>, TASKS == 1 ? 2 : 1)
   if (threadIdx.x == 0 && aborted) atomicOr(p.err, kErrTimeout);
 }
 
-template <int TASKS>
+template <int TASKS, bool CODES>
 cudaError_t launch_tasks(const GradParams& p, uint32_t smem, unsigned grid, cudaStream_t stream) {
   static SmemOptIn opted;
-  cudaError_t e = opted.allow(reinterpret_cast<const void*>(adapter_grad_kernel<TASKS>));
+  cudaError_t e = opted.allow(reinterpret_cast<const void*>(adapter_grad_kernel<TASKS, CODES>));
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid);
@@ -704,7 +740,7 @@ cudaError_t launch_tasks(const GradParams& p, uint32_t smem, unsigned grid, cuda
   attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  return cudaLaunchKernelEx(&cfg, adapter_grad_kernel<TASKS>, p);
+  return cudaLaunchKernelEx(&cfg, adapter_grad_kernel<TASKS, CODES>, p);
 }
 
 // CTAs that share an adapter's rows: the least of rounds x (9 us a CTA and 0.6 us a
@@ -759,9 +795,14 @@ cudaError_t launch_adapter_grad(const GradParams& p, cudaStream_t stream) {
   // from 10.6 to 26 us.
   const int most = (148 + q.splits - 1) / q.splits;
   const unsigned grid = static_cast<unsigned>(q.workers + (rest < most ? rest : most)) * q.splits;
-  if (p.rp <= 32) return launch_tasks<1>(q, geo.smem, grid, stream);
-  if (p.rp <= 64) return launch_tasks<2>(q, geo.smem, grid, stream);
-  return launch_tasks<4>(q, geo.smem, grid, stream);
+  if (q.codes != 0) {
+    if (p.rp <= 32) return launch_tasks<1, true>(q, geo.smem, grid, stream);
+    if (p.rp <= 64) return launch_tasks<2, true>(q, geo.smem, grid, stream);
+    return launch_tasks<4, true>(q, geo.smem, grid, stream);
+  }
+  if (p.rp <= 32) return launch_tasks<1, false>(q, geo.smem, grid, stream);
+  if (p.rp <= 64) return launch_tasks<2, false>(q, geo.smem, grid, stream);
+  return launch_tasks<4, false>(q, geo.smem, grid, stream);
 }
 
 }  // namespace mp

@@ -368,6 +368,7 @@ struct GradParams {
   // may have rows and of all, CTAs that share an adapter's rows, clusters that work
   // on items (those past them clear), whether a member reads a checkpoint
   int32_t tiles, items, all_items, splits, workers, codes;
+  const AdapterInfo* info;  // [cap]
   RequestPlan plan;
   uint64_t wait_limit_ns;
   uint32_t* err;
