@@ -158,9 +158,10 @@ int mp_set_strengths_rows(mp_ctx* ctx, const float* s, const int32_t* row_starts
  * segments are set, whose longest segment then counts. The token tile and
  * the K splits of a projection and of its rank-space pre-GEMM (which fix the
  * fp32 summation order) are chosen from this count, so each image of such a
- * batch has the bits of its own launch. Not part of the state version: a
- * graph keeps the choices of its capture. No counterpart in the reference,
- * whose batches are per image. */
+ * batch has the bits of its own launch. mp_linear_requests and its backward
+ * pass do not take part: see there. Not part of the state version: a graph
+ * keeps the choices of its capture. No counterpart in the reference, whose
+ * batches are per image. */
 int mp_set_image_rows(mp_ctx* ctx, int rows);
 
 /* A counter that every change of a strength (to another value), of the row
@@ -393,7 +394,10 @@ int mp_requests_plan(mp_ctx* ctx, mp_requests* req, const int32_t* lengths,
 /* y[t] = x[t] deq(W)^T + s_q (x[t] A_a^T) B_a^T for every row t of every
  * request q, a its adapter; x, y as in mp_linear. Slots bound to `w` are not
  * applied. A row without an adapter has the bits of the same call with an empty
- * plan. `ranks` (nullable): f32 [m, >= mp_adapters_rank_pad], 16-byte aligned,
+ * plan; the kernels, the token tile and the K splits are chosen from m, the
+ * number of requests and the shape of the whole call, whatever
+ * mp_set_image_rows and the row segments say, so a row's bits may differ between
+ * batches of another size. `ranks` (nullable): f32 [m, >= mp_adapters_rank_pad], 16-byte aligned,
  * ldr a multiple of 4: s_q x[t] A_a^T (0 without an adapter), which the
  * backward pass takes as v. */
 int mp_linear_requests(mp_ctx* ctx, const mp_weight* w, const void* x, int64_t ldx,

@@ -250,3 +250,32 @@ def test_wild_values_in_gradients(ctx, case, saved):
                     torch.where(fine, bound, zero + 1))
     for h in (w, wt, bank, plan):
         h.free()
+
+
+# shapes whose K splits differ between the whole call's rows, a quarter and a sixteenth
+@pytest.mark.parametrize("m,n,k", [(2048, 512, 3840), (1024, 1024, 2560)])
+def test_image_rows_do_not_enter(ctx, m, n, k):
+    """Kernel, tile and splits of a call with adapters by request come from the
+    whole call: a count of rows an image, or row segments, set for other launches
+    change no bit."""
+    rng = np.random.default_rng(m)
+    cap, r = 2, 16
+    w, _, _ = _weight(ctx, rng, n, k, 8)
+    bank, _ = _bank(ctx, rng, n, k, cap, r, [r, r])
+    plan = ctx.requests(2, m, cap)
+    plan.plan([m // 2, m // 2], [0, 1], None, m)
+    x = _bf16(rng, m, k)
+    want = ctx.linear_requests(w, x, bank, plan)
+    try:
+        ctx.set_image_rows(m // 16)
+        by_images = ctx.linear_requests(w, x, bank, plan)
+        ctx.set_image_rows(0)
+        ctx.set_strengths_rows(np.ones((4, 8), np.float32), [i * m // 4 for i in range(5)])
+        by_segments = ctx.linear_requests(w, x, bank, plan)
+    finally:
+        ctx.set_image_rows(0)
+        ctx.clear_strengths_rows()
+    ctx.sync_check()
+    assert torch.equal(want, by_images) and torch.equal(want, by_segments)
+    for h in (w, bank, plan):
+        h.free()

@@ -804,7 +804,7 @@ int launch_projections(mp_ctx* c, const mp_weight* const* ws, void* const* ys,
   const int members = swi != nullptr ? 1 : count;
   // SwiGLU pairs and attention-head launches run on 256- or 512-token tiles
   // only (their kernel instantiations)
-  const int mi = image_rows(c, m);
+  const int mi = ext != nullptr ? m : image_rows(c, m);
   int n_tok = 0;
   if (swi != nullptr) n_tok = std::max(mp::kMaxTok, mp::pick_ntok_pair(mi, pairs_of(ns[0])));
   if (hds != nullptr) {
@@ -816,9 +816,11 @@ int launch_projections(mp_ctx* c, const mp_weight* const* ws, void* const* ys,
   // split writes fp32 partial sums (the last one after the appended LoRA K
   // tiles), lora_reduce_kernel adds them in split order and rounds to bf16.
   // The split count and the token tile come from one image's rows, at most
-  // kSplitBytes of partial sums per image. (With adapters by request the bytes
-  // alone are the limit: a gradient of 1497 rows with 8080 features in and 1280
-  // out has 15 tiles for 74 pairs unsplit.)
+  // kSplitBytes of partial sums per image. (With adapters by request they come
+  // from the whole call, since the form of its rank-space rows does: an image's
+  // share of the requests is not known here. And the bytes alone are the limit: a
+  // gradient of 1497 rows with 8080 features in and 1280 out has 15 tiles for 74
+  // pairs unsplit.)
   mp::SplitChoice msplit{0, 1, 0.0};
   if (may_alloc && count == 1 && swi == nullptr && hds == nullptr && pro == nullptr &&
       (mi <= kSplitRows || ext != nullptr) && ns[0] % 4 == 0 && ldys[0] % 4 == 0 && reinterpret_cast<uintptr_t>(ys[0]) % 8 == 0) {
