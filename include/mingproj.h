@@ -97,7 +97,8 @@ const char* mp_last_error(const mp_ctx* ctx);
 const char* mp_status_string(int status);
 /* Synchronizes `stream` and reports device-side failures: MP_ETIMEOUT when
  * any kernel of this context gave up a bounded wait since the last check,
- * MP_EINVAL when a request plan met a length or an adapter out of range.
+ * MP_EINVAL when a request plan met a length or an adapter out of range; when
+ * both happened MP_ETIMEOUT, and MP_EINVAL from the check after it.
  * Replaces: the commit/wait of the forward (src/ming-dit.cc:2564-2571). */
 int mp_sync_check(mp_ctx* ctx, void* stream);
 /* Device-side wait limit in nanoseconds (default 2e9). */

@@ -7,7 +7,8 @@ import numpy as np
 import pytest
 import torch
 
-from mingproj.proj import Context, MP_QUANT_SYMMETRIC
+from mingproj._lib import MP_EINVAL, MP_ETIMEOUT
+from mingproj.proj import Context, MP_QUANT_SYMMETRIC, MPError
 from test_requests_gpu import _bank, _bf16, _forward_ref, _grad_ref, _segments, _weight, _within
 
 pytestmark = pytest.mark.gpu
@@ -279,3 +280,19 @@ def test_image_rows_do_not_enter(ctx, m, n, k):
     assert torch.equal(want, by_images) and torch.equal(want, by_segments)
     for h in (w, bank, plan):
         h.free()
+
+
+def test_a_cut_plan_is_reported_beside_a_timeout(ctx):
+    plan = ctx.requests(1, 8, 1)
+    for timeout in (True, False):
+        plan.plan([9], [0], None, 8)  # a row too many
+        if timeout:
+            ctx.selftest_wait(1_000_000)  # 1 ms
+            with pytest.raises(MPError) as e:
+                ctx.sync_check()
+            assert e.value.status == MP_ETIMEOUT
+        with pytest.raises(MPError, match="out of range") as e:
+            ctx.sync_check()
+        assert e.value.status == MP_EINVAL
+        ctx.sync_check()
+    plan.free()

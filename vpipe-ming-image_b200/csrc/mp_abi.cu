@@ -1244,7 +1244,9 @@ int mp_sync_check(mp_ctx* c, void* stream) {
   uint32_t word = 0;
   MP_CUDA(c, cudaMemcpy(&word, c->err_word, sizeof(word), cudaMemcpyDeviceToHost));
   if (word != 0) {
-    MP_CUDA(c, cudaMemset(c->err_word, 0, sizeof(uint32_t)));
+    // one failure a check: beside a timeout a cut plan stays for the next one
+    const uint32_t left = (word & mp::kErrTimeout) != 0 ? word & ~mp::kErrTimeout : 0u;
+    MP_CUDA(c, cudaMemcpy(c->err_word, &left, sizeof(left), cudaMemcpyHostToDevice));
     if ((word & mp::kErrTimeout) == 0)
       return fail(c, MP_EINVAL,
                   "a request plan met a length or an adapter index out of range (the rows concerned "

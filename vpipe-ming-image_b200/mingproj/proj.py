@@ -314,7 +314,8 @@ class Context:
 
     def sync_check(self, stream=None) -> None:
         """Synchronizes and raises MPError(MP_ETIMEOUT) if a kernel gave up a
-        bounded device-side wait."""
+        bounded device-side wait, MPError(MP_EINVAL) if a request plan met a
+        length or an adapter out of range; one failure a call, that one first."""
         self._check(self.lib.mp_sync_check(self.h, _stream_handle(stream)))
 
     def selftest_wait(self, limit_ns: int, stream=None) -> None:
