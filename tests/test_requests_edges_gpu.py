@@ -3,6 +3,8 @@ promise: captured graphs, streams given, infinities, ranks below the bank's.
 
 Tolerances are the bounds of test_requests_gpu.py, element by element.
 """
+import contextlib
+
 import numpy as np
 import pytest
 import torch
@@ -296,3 +298,34 @@ def test_a_cut_plan_is_reported_beside_a_timeout(ctx):
         assert e.value.status == MP_EINVAL
         ctx.sync_check()
     plan.free()
+
+
+@contextlib.contextmanager
+def _refusing_stream():
+    """A stream whose capture was broken off: every launch on it fails on the host."""
+    from cuda.bindings import runtime
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    relaxed = runtime.cudaStreamCaptureMode.cudaStreamCaptureModeRelaxed
+    assert runtime.cudaStreamBeginCapture(side.cuda_stream, relaxed)[0] == runtime.cudaError_t.cudaSuccess
+    assert runtime.cudaStreamSynchronize(side.cuda_stream)[0] != runtime.cudaError_t.cudaSuccess  # not allowed there
+    try:
+        with torch.cuda.stream(side):
+            yield
+    finally:
+        assert runtime.cudaStreamEndCapture(side.cuda_stream)[0] != runtime.cudaError_t.cudaSuccess
+
+
+def test_a_failed_launch_fails_one_call(ctx):
+    """The call after a failed one does not report its error again."""
+    rng = np.random.default_rng(1)
+    n, k = 128, 64
+    bank, fac = _bank(ctx, rng, n, k, 1, 8, [8])
+    plan = ctx.requests(4, 40, 1)
+    lengths, owners = (torch.tensor([v] * 4, dtype=torch.int32, device="cuda") for v in (10, 0))
+    with _refusing_stream(), pytest.raises(MPError):
+        plan.plan(lengths, owners, None, 40)
+    bank.set(0, *(f.to(torch.bfloat16) for f in fac[0]))
+    ctx.sync_check()
+    for h in (bank, plan):
+        h.free()

@@ -206,7 +206,10 @@ int fail(mp_ctx* c, int code, const char* fmt, ...) {
   return code;
 }
 
+// The failure is reported here and once: the runtime's own record of it is
+// cleared, or the next launch that asks for it would fail in its place.
 int cuda_fail(mp_ctx* c, cudaError_t e, const char* what) {
+  (void)cudaGetLastError();
   return fail(c, e == cudaErrorMemoryAllocation ? MP_ENOMEM : MP_ECUDA, "%s: %s", what,
               cudaGetErrorString(e));
 }
