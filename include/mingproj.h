@@ -387,7 +387,8 @@ int mp_requests_free(mp_ctx* ctx, mp_requests* req);
  * after the last request have no adapter. All three: device arrays. A negative
  * length, lengths that pass m, and an adapter outside [-1, capacity) are cut
  * to what is valid, and the next mp_sync_check reports MP_EINVAL. Calls that
- * use the plan follow on the same stream, or are ordered after it. */
+ * use the plan follow on the same stream, or are ordered after it. A call that
+ * fails leaves the plan as it was. */
 int mp_requests_plan(mp_ctx* ctx, mp_requests* req, const int32_t* lengths,
                      const int32_t* adapters, const float* strengths, int n_requests, int m,
                      void* stream);

@@ -329,3 +329,24 @@ def test_a_failed_launch_fails_one_call(ctx):
     ctx.sync_check()
     for h in (bank, plan):
         h.free()
+
+
+def test_a_plan_that_fails_leaves_the_one_before(ctx):
+    """Calls of the rows planned before still run, calls of the new ones are refused."""
+    rng = np.random.default_rng(2)
+    m, n, k = 40, 128, 64
+    w, _, _ = _weight(ctx, rng, n, k, 8)
+    bank, _ = _bank(ctx, rng, n, k, 1, 8, [8])
+    plan = ctx.requests(4, 4 * m, 1)
+    x = _bf16(rng, 4 * m, k)
+    lengths, owners = (torch.tensor([v] * 4, dtype=torch.int32, device="cuda") for v in (m, 0))
+    plan.plan([m], [0])
+    want = ctx.linear_requests(w, x[:m], bank, plan)
+    with _refusing_stream(), pytest.raises(MPError):
+        plan.plan(lengths, owners, None, 4 * m)
+    with pytest.raises(MPError, match="rows were planned"):
+        ctx.linear_requests(w, x, bank, plan)
+    assert torch.equal(ctx.linear_requests(w, x[:m], bank, plan), want)
+    ctx.sync_check()
+    for h in (w, bank, plan):
+        h.free()

@@ -2396,16 +2396,18 @@ int mp_requests_plan(mp_ctx* c, mp_requests* r, const int32_t* lengths, const in
   if (m <= 0 || m > r->max_rows) return fail(c, MP_EINVAL, "m = %d outside [1, %d]", m, r->max_rows);
   int rc = use_device(c);
   if (rc != MP_OK) return rc;
-  r->plan.n_req = n_requests;
-  r->plan.m = m;
   mp::PlanParams p;
   p.plan = r->plan;
+  p.plan.n_req = n_requests;
+  p.plan.m = m;
   p.lengths = lengths;
   p.adapters = adapters;
   p.strengths = strengths;
   p.err = c->err_word;
+  // a launch that fails leaves the plan before it, sizes and all
   MP_CUDA(c, mp::launch_plan_requests(p, static_cast<cudaStream_t>(stream)));
   c->eng.kernels += 1;
+  r->plan = p.plan;
   r->planned = true;
   return MP_OK;
 }
