@@ -406,8 +406,12 @@ int mp_linear_requests(mp_ctx* ctx, const mp_weight* w, const void* x, int64_t l
                        const mp_adapters* bank, const mp_requests* req, void* y, int64_t ldy,
                        float* ranks, int64_t ldr, int m, void* stream);
 
-/* The dense bf16 transpose [k, n] of a projection weight [n, k]: the values
- * the projections multiply with. Freed with mp_weight_free. */
+/* The dense bf16 transpose [k, n] of a projection weight [n, k], 2 bytes a
+ * weight beside the packed 0.5 (4 bits) or 1 (8 bits): every weight
+ * dequantized and rounded to bf16, as the projections over more than 32 rows
+ * multiply with it. Up to 32 rows mp_linear_requests multiplies with the codes
+ * and applies scale and bias in f32: there the forward weight and this one
+ * differ by that rounding, 2^-8 of a weight. Freed with mp_weight_free. */
 int mp_weight_transpose(mp_ctx* ctx, const mp_weight* w, void* stream, mp_weight** out);
 
 /* The backward pass of mp_linear_requests, W held fixed. With u[t] =

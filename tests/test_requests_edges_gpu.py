@@ -11,7 +11,7 @@ import torch
 
 from mingproj._lib import MP_EINVAL, MP_ETIMEOUT
 from mingproj.proj import Context, MP_QUANT_SYMMETRIC, MPError
-from test_requests_gpu import _bank, _bf16, _forward_ref, _grad_ref, _segments, _weight, _within
+from test_requests_gpu import ADD, BF, _bank, _bf16, _forward_ref, _grad_ref, _segments, _weight, _within
 
 pytestmark = pytest.mark.gpu
 
@@ -349,4 +349,33 @@ def test_a_plan_that_fails_leaves_the_one_before(ctx):
     assert torch.equal(ctx.linear_requests(w, x[:m], bank, plan), want)
     ctx.sync_check()
     for h in (w, bank, plan):
+        h.free()
+
+
+@pytest.mark.parametrize("bits,mode", [(8, 0), (4, 0), (8, MP_QUANT_SYMMETRIC)])
+def test_transposed_weight_and_few_rows(ctx, bits, mode):
+    """Up to 32 rows the forward weight is the codes' own, scale and bias in f32;
+    the transpose holds it rounded to bf16. Unit rows show both: each within one
+    rounding of the weight, so within two of one another."""
+    rng = np.random.default_rng(bits + mode)
+    n, k, top = 192, 128, 2 ** bits
+    w, w64, _ = _weight(ctx, rng, n, k, bits, mode)
+    wt = ctx.transposed(w)
+    bank, _ = _bank(ctx, rng, n, k, 1, 8, [8])
+    plan = ctx.requests(1, 33, 1)
+    rows = torch.eye(k, dtype=torch.bfloat16, device="cuda").repeat(2, 1)  # whole calls of 33 rows
+    back = ctx.linear(wt, torch.eye(n, dtype=torch.bfloat16, device="cuda"))  # [n, k]
+    # sums of scale * code and bias in f32 may cancel: codes reach 2^bits, or 128 + 2^4, steps
+    step = (w64.max(1).values - w64.min(1).values)[:, None] / (top - 1) * 1.5
+    near = 4 * ADD * step * max(top, 144)
+    for m in (32, 33):
+        plan.plan([], [], None, m)
+        few = torch.cat([ctx.linear_requests(w, rows[i:i + m], bank, plan).T for i in range(0, k, m)], 1)[:, :k]
+        ctx.sync_check()
+        if m == 33:
+            assert torch.equal(few, back), "above 32 rows: the same bf16 weight"
+        rounding = BF * w64.abs() * (1 + BF) + near
+        assert ((few.double() - w64).abs() <= rounding).all()
+        assert ((few.double() - back.double()).abs() <= 2 * rounding).all()
+    for h in (w, wt, bank, plan):
         h.free()

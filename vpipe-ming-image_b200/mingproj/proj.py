@@ -585,7 +585,8 @@ class Context:
         return out if v is None else (out, v)
 
     def transposed(self, w: Weight, stream=None) -> Weight:
-        """The dense bf16 transpose [k, n] of a projection weight [n, k]."""
+        """The dense bf16 transpose [k, n] of a projection weight [n, k] (2 bytes
+        a weight), a packed one dequantized and rounded to bf16."""
         h = C.c_void_p()
         self._check(self.lib.mp_weight_transpose(self.h, w.handle, _stream_handle(stream),
                                                  C.byref(h)))
