@@ -26,8 +26,8 @@
 // A checkpoint's codes are whole numbers of up to 8 bits, exact in bf16: warps
 // 2-9 widen them, and the scale of a (row, 128 features) goes into u, in f32.
 //
-// Measured: 92 us for 16896 rows 3840 x 3840, 24 requests, 16 adapters of up to 64
-// ranks (x and dy once, 260 MB, at 2.8 TB/s; 43 % of the issue slots); 24 us for 4352
+// Measured: 88 us for 16896 rows 3840 x 3840, 24 requests, 16 adapters of up to 64
+// ranks (x and dy once, 260 MB, at 3.0 TB/s), 129 with x in 8 bits; 24 us for 4352
 // rows, 4 adapters of 16, x in 8 bits (2.1 TB/s). What bounds it is not HBM but
 // cutting u: a stage's u is cut anew for each 128 features, 60 times here, and a CTA
 // takes 0.6 us a stage for its chain of copies, parts, MMAs and sums.
@@ -389,6 +389,8 @@ __device__ void convert(const GradParams& p, const GradSmem& sm, const GradGeo& 
   }
 }
 
+// Registers: two CTAs an SM at up to 32 ranks leave 72 a thread, the 576 threads of
+// more than 64 ranks 96; 72 and 132 bytes a thread spill, at 64 ranks none.
 template <int TASKS, bool CODES>
 __global__ void __launch_bounds__(kGradThreads<TASKS>, TASKS == 1 ? 2 : 1)
     adapter_grad_kernel(const __grid_constant__ GradParams p) {

@@ -123,12 +123,12 @@ struct ProjParams {
   // .. [+ ext_live[tt] - 1], ext_chunks 64-wide tiles each. An entry {b, a}
   // takes its rank-space rows from the n_tok rows of tm_t from row b * n_tok
   // (zero in the rows of other requests) and the factor B from row a * N of tm_b.
+  // The launch right before on the stream is then the one that writes tm_t's
+  // blocks: this one starts beside it (everything else it touches was complete
+  // when that one started) and waits for it before the first appended K tile.
   const int32_t* ext_first;
   const int32_t* ext_live;
   const int2* ext_list;
-  // The launch right before on the stream is the one that writes tm_t's blocks:
-  // this one starts beside it (everything else it touches was complete when that
-  // one started) and waits for it before the first appended K tile.
   int32_t ext_chunks;
   // Fused rank-space prologue (n_pre > 0): before their member tiles, the
   // pairs with the fewest member tiles run n_pre prologue units, each the
