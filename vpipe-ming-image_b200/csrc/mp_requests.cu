@@ -456,58 +456,44 @@ __device__ __forceinline__ void few_x(const uint16_t* at, int col, int k, uint32
   }
 }
 
-// W x of 16 features and one row of a packed weight, weight by weight, for sums
-// that the codes' arithmetic does not hold: scale sum_k q x and offset sum_k x are
-// of opposite signs and up to 255 times x, so an infinity in x came out as inf -
-// inf, and x beyond 1e36 overflowed where W x does not. A warp: lanes share K in 16
-// columns each; lane l gets feature f0 + l % 16. Rare, and never inlined: the
-// kernel's loop keeps its registers.
+// W x of one feature and row of a packed weight, weight by weight, for a sum that
+// the codes' arithmetic does not hold: scale sum_k q x and offset sum_k x are of
+// opposite signs and up to 255 times x, so an infinity in x came out as inf - inf,
+// and x beyond 1e36 overflowed where W x does not. Rare, and never inlined: the
+// kernel's loop keeps its registers. Ends at a NaN, which stays one. A thread does
+// a whole sum: a call of one such row takes 60 us (w4 10240x3840), of 16 such rows
+// 247. A warp a row took 33 and 206, but a barrier or a larger function behind the
+// loop cost every call of up to 8 rows 1.1 us of 11.
 template <int BITS>
-__device__ __noinline__ float few_again(const FewParams& p, int f0, int t) {
-  constexpr int kAt = 4;  // features at a time
-  const int lane = threadIdx.x & 31;
+__device__ __noinline__ float few_dot(const FewParams& p, int n, int t) {
+  const uint8_t* w = p.w + static_cast<size_t>(n) * p.w_pitch;
+  const uint32_t* sb = p.sb + static_cast<size_t>(n) * p.sb_stride;
   const uint16_t* x = p.x + static_cast<int64_t>(t) * p.ldx;
-  float mine = 0.0f;
+  float sum = 0.0f;
 #pragma unroll 1
-  for (int h0 = 0; h0 < 16; h0 += kAt) {
-    float sum[kAt];
+  for (int c = 0; c < p.k && sum == sum; c += 64) {  // k is a multiple of 64
+    const uint32_t z = sb[c / 64];
+    const float scale = bf16_bits_to_f32(z & 0xFFFFu), bias = bf16_bits_to_f32(z >> 16);
+#pragma unroll 4
+    for (int h = 0; h < 64; h += 8) {
+      const uint4 xv = *reinterpret_cast<const uint4*>(x + c + h);
+      const uint32_t xw[4] = {xv.x, xv.y, xv.z, xv.w};
+      uint32_t q[2];
+      if constexpr (BITS == 8) {
+        const uint2 v = *reinterpret_cast<const uint2*>(w + c + h);
+        q[0] = v.x ^ p.code_xor, q[1] = v.y ^ p.code_xor;
+      } else {
+        q[0] = *reinterpret_cast<const uint32_t*>(w + (c + h) / 2);
+      }
 #pragma unroll
-    for (int h = 0; h < kAt; ++h) sum[h] = 0.0f;
-#pragma unroll 1
-    for (int c = 16 * lane; c < p.k; c += 512) {  // k is a multiple of 64
-      const uint4 xa = *reinterpret_cast<const uint4*>(x + c), xb = *reinterpret_cast<const uint4*>(x + c + 8);
-      const uint32_t xw[8] = {xa.x, xa.y, xa.z, xa.w, xb.x, xb.y, xb.z, xb.w};
-#pragma unroll
-      for (int h = 0; h < kAt; ++h) {
-        const size_t n = min(f0 + h0 + h, p.n - 1);
-        const uint8_t* w = p.w + n * p.w_pitch + c * BITS / 8;
-        uint32_t q[4];
-        if constexpr (BITS == 8) {
-          const uint4 v = *reinterpret_cast<const uint4*>(w);
-          q[0] = v.x ^ p.code_xor, q[1] = v.y ^ p.code_xor, q[2] = v.z ^ p.code_xor, q[3] = v.w ^ p.code_xor;
-        } else {
-          const uint2 v = *reinterpret_cast<const uint2*>(w);
-          q[0] = v.x, q[1] = v.y;
-        }
-        const uint32_t sb = p.sb[n * p.sb_stride + c / 64];
-        const float scale = bf16_bits_to_f32(sb & 0xFFFFu), bias = bf16_bits_to_f32(sb >> 16);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float code = BITS == 8 ? static_cast<float>(q[i / 4] >> (8 * (i % 4)) & 0xFFu) - p.zero
-                                       : static_cast<float>(q[i / 8] >> (4 * (i % 8)) & 0xFu);
-          const float xi = __uint_as_float(i % 2 == 0 ? xw[i / 2] << 16 : xw[i / 2] & 0xFFFF0000u);
-          sum[h] = fmaf(fmaf(code, scale, bias), xi, sum[h]);
-        }
+      for (int i = 0; i < 8; ++i) {
+        const float code = BITS == 8 ? static_cast<float>(q[i / 4] >> (8 * (i % 4)) & 0xFFu) - p.zero
+                                     : static_cast<float>(q[0] >> (4 * i) & 0xFu);
+        sum = fmaf(fmaf(code, scale, bias), __uint_as_float(i % 2 == 0 ? xw[i / 2] << 16 : xw[i / 2] & 0xFFFF0000u), sum);
       }
     }
-#pragma unroll
-    for (int h = 0; h < kAt; ++h) {
-#pragma unroll
-      for (int d = 16; d > 0; d >>= 1) sum[h] += __shfl_xor_sync(0xFFFFFFFFu, sum[h], d);
-      if (lane % 16 == h0 + h) mine = sum[h];
-    }
   }
-  return mine;
+  return sum;
 }
 
 // Blocks an SM that the registers are cut to. With 17 to 32 rows and bf16 two
@@ -637,22 +623,15 @@ __global__ void __launch_bounds__(32 * WARPS, kFewBlocks<BITS, NT, WARPS>)
   __syncthreads();
   pdl_wait();  // v is complete; y may be written
   pdl_release();
-  // a warp: 16 features of two rows
-  const int f = lane & 15;
-  for (int t0 = 2 * warp; t0 < p.m; t0 += 2 * WARPS) {
-    const int t = t0 + (lane >> 4);
+  const int f = threadIdx.x & 15;
+  if (f0 + f >= p.n) return;
+  for (int t = threadIdx.x >> 4; t < p.m; t += 2 * WARPS) {
     float sum = part[0][f][t];
 #pragma unroll
     for (int w = 1; w < WARPS; ++w) sum += part[w][f][t];
     if constexpr (BITS != 0) {
-      const uint32_t wild = __ballot_sync(0xFFFFFFFFu, t < p.m && !isfinite(sum));
-      if (wild != 0u) {
-        const float a = wild & 0xFFFFu ? few_again<BITS>(p, f0, t0) : 0.0f;
-        const float b = wild >> 16 ? few_again<BITS>(p, f0, t0 + 1) : 0.0f;
-        if (!isfinite(sum)) sum = lane < 16 ? a : b;
-      }
+      if (!isfinite(sum)) sum = few_dot<BITS>(p, f0 + f, t);
     }
-    if (t >= p.m || f0 + f >= p.n) continue;
     const int a = p.row_adapter[t];
     if (a >= 0) {
       const uint16_t* br = p.b + (static_cast<size_t>(a) * p.n + f0 + f) * p.rp;
