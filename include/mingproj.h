@@ -24,6 +24,9 @@
  *     mp_last_error() says why.
  *   - One host thread per context. Launches are stream-ordered on the
  *     stream passed in (a cudaStream_t; NULL = the legacy default stream).
+ *     The calls of a context share its buffers (rank-space rows, partial
+ *     sums): calls on several streams, and replays of graphs that hold some,
+ *     are ordered by the caller so that they do not overlap on the GPU.
  *   - Strengths in force when a projection is enqueued are captured by
  *     value into that launch.
  */
